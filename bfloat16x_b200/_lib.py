@@ -29,6 +29,7 @@ class Bf16xError(RuntimeError):
 
 
 _i64, _i32, _p, _u32p = ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.POINTER(ctypes.c_uint32)
+_f32 = ctypes.c_float
 
 # name -> (restype, argtypes)
 _SIGS = {
@@ -68,6 +69,13 @@ _SIGS = {
     "bf16x_add_rmsnorm": (_i32, [_p, _p, _p, ctypes.c_float, _i64, _i64, _p, _p, _p]),
     "bf16x_rope_qkv": (_i32, [_p, _i64, _i32, _i32, _i32, _i32, _p, _p, _p, _p, _p, _p, _i64, _i64, _p]),
     "bf16x_silu_mul": (_i32, [_p, _i64, _i64, _p, _p]),
+    "bf16x_kv4_block_bytes": (_i64, [_i64]),
+    "bf16x_kv4_append": (_i32, [_p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i32, _p, _p, _p, _p, _i64, _p]),
+    "bf16x_kv4_read": (_i32, [_p, _i64, _i64, _i64, _i64, _i64, _p, _i32, _p, _p, _p]),
+    "bf16x_kv4_attend_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64]),
+    "bf16x_kv4_attend": (_i32, [_p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i32, _f32, _p, _i64, _p, _p,
+                                _i64, _p]),
+    "bf16x_sample": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _p, _f32, _p, _i32, _p, _f32, _p, _f32, _p, _p]),
     "bf16x_peer_handle_bytes": (_i64, []),
     "bf16x_peer_export": (_i32, [_p, _p, _p]),
     "bf16x_peer_import": (_i32, [_p, _p]),

@@ -1,0 +1,102 @@
+// bf16x_kv4.cuh -- the 4-bit key/value cache: its layout and the warp-level
+// pieces shared by the kernels that write, read and attend to it.
+//
+// The cache of one layer is a byte array [batch][kv_heads][ceil(max_seq/16)]
+// of blocks of 20 * D bytes.  A block holds 16 positions of one kv head.  Each
+// group of 32 neighbouring channels of a position has a scale d >= 0 and a
+// minimum m (bf16), and its 4-bit codes stand for d * code + m: 5 bits per
+// value.  With NG = D / 32 groups, the parts of a block are
+//
+//   K codes  [16 r][4 t][NG j][8 n]          position r, channel 32 j + 8 t + n
+//   V codes  [2 p][8 g][4 t][NG j][2 h][4 n] position 8 p + 2 t + h, channel 32 j + 4 g + n
+//   K scales [16 r][NG], K minima [16 r][NG], V scales [16 r][NG]   bf16
+//   V minima [8 pairs][NG][2]                bf16, positions 2 pair, 2 pair + 1
+//
+// The order is that of the mma.sync fragments: lane (g, t) = (lane / 4,
+// lane % 4) of a warp reads its K codes of row g with one 16-byte access (D =
+// 128) and its V codes of each half p with another, both contiguous over the
+// warp.  A nibble that sits in bits 0..3 or 4..7 of a 16-bit half is, read as
+// fp16, the subnormal number code * 2^-24 or code * 2^-20: exact, so one AND
+// turns a packed pair of codes into a matrix operand, and the powers of two
+// are taken out of the other operand (K) or of the sums (V).
+#pragma once
+
+#include "bf16x_common.cuh"
+#include "bf16x_status.cuh"
+
+namespace bf16x {
+
+constexpr int kKvBlock = 16;                   // positions per block
+
+template <int D>
+struct KvLayout {
+    static constexpr int NG = D / 32;
+    static constexpr int kV = 8 * D;           // byte offset of each part
+    static constexpr int kKd = 16 * D;
+    static constexpr int kKm = 17 * D;
+    static constexpr int kVd = 18 * D;
+    static constexpr int kVm = 19 * D;
+    static constexpr int kBytes = 20 * D;
+};
+
+__device__ __forceinline__ float fmin_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float fmax_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float lg2(float x) {
+    float r;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// bf16 in the low / high half of a word, as fp32
+__device__ __forceinline__ float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// D[16][8] += A[16][16] B[16][8], fp32 sums
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                 "{%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                 "{%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// transposed 8x8 tile of 16-bit values: row g, columns 2t, 2t+1 -> row 2t.. as column
+__device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+    return r;
+}
+
+}  // namespace bf16x

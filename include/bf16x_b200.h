@@ -318,6 +318,58 @@ int bf16x_rope_qkv(const uint16_t *qkv, int64_t tokens, int T, int H, int KV, in
                    uint16_t *cache_v, int64_t cache_ld_b, int64_t max_pos, void *stream);
 int bf16x_silu_mul(const uint16_t *gu, int64_t rows, int64_t F, uint16_t *out, void *stream);
 
+/* ---- 4-bit key/value cache ------------------------------------------------ */
+/* No counterpart in the reference.  Keys and values of the decoder's attention
+ * held in 4 bits.  The cache of one layer is a byte array [batch][kv_heads]
+ * [ceil(max_seq / 16)][bf16x_kv4_block_bytes(D)], 16-byte aligned, D (head_dim)
+ * 64 or 128: blocks of 16 positions of one head, every 32 channels with a scale
+ * d and a minimum m (bf16) standing for d * code + m (5 bits per value; the
+ * order within a block is given in csrc/bf16x_kv4.cuh).  Positions come from
+ * device memory: sequence b's tokens are at pos0[b * pos_stride] + 0 .. T - 1
+ * (pos_stride 0: one position for all).  A negative position is padding (left-
+ * padded prompts of different lengths); a position >= max_seq is skipped and
+ * sets a status bit (bf16x_device_status).
+ * bf16x_kv4_append: qkv [B][T][(H + 2 KV) * D] bf16 (batch and token strides
+ *   ld_b, ld_t in elements, multiples of 8): q and k heads turned pairwise by
+ *   cos/sin (fp32 [>= max_seq][D/2], both NULL: not turned), q to q_out
+ *   [B][T][H][D], k and v into the cache; q rows of positions outside the
+ *   cache are zeros.  A group of 32 that holds an infinity or NaN reads as NaN.
+ * bf16x_kv4_read: k_out, v_out [B][T][KV][D] bf16: the values the cache holds,
+ *   zeros outside it.
+ * bf16x_kv4_attend: out[b][t][h] = softmax(scale * q . K) V over positions 0 ..
+ *   pos0[b] + t of kv head h / (H / KV), out [B][T][H][D] bf16; a row that sees
+ *   no position (padding, or past the cache) is zeros.  q strides in elements,
+ *   multiples of 8; everything 16-byte aligned.  workspace:
+ *   bf16x_kv4_attend_workspace_bytes(...) bytes that no other call in flight
+ *   uses; its contents never need initialising. */
+int64_t bf16x_kv4_block_bytes(int64_t head_dim);
+int bf16x_kv4_append(const uint16_t *qkv, int64_t ld_b, int64_t ld_t, int64_t B, int64_t T, int64_t H, int64_t KV,
+                     int64_t D, const int64_t *pos0, int pos_stride, const float *cos_t, const float *sin_t,
+                     uint16_t *q_out, uint8_t *blocks, int64_t max_seq, void *stream);
+int bf16x_kv4_read(const uint8_t *blocks, int64_t max_seq, int64_t B, int64_t T, int64_t KV, int64_t D,
+                   const int64_t *pos0, int pos_stride, uint16_t *k_out, uint16_t *v_out, void *stream);
+int64_t bf16x_kv4_attend_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t KV, int64_t D, int64_t max_seq);
+int bf16x_kv4_attend(const uint16_t *q, int64_t ldq_b, int64_t ldq_t, int64_t ldq_h, int64_t B, int64_t T, int64_t H,
+                     int64_t KV, int64_t D, const int64_t *pos0, int pos_stride, float scale, const uint8_t *blocks,
+                     int64_t max_seq, uint16_t *out, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* ---- token sampling -------------------------------------------------------- */
+/* No counterpart in the reference.  tokens[b] drawn from logits [B][V] (bf16 or
+ * fp32 by dtype, row stride ld) with the given numbers u[b] in [0, 1).  The
+ * tokens of a row are ordered by logit, ties by index, and weigh
+ * exp((logit - max) / temperature); top_k (> 0) keeps the first k of the order,
+ * top_p (< 1) the shortest prefix that reaches top_p of what top_k kept, min_p
+ * (> 0) the tokens that weigh at least min_p times the heaviest; the token is
+ * the first kept one, in index order, whose running weight exceeds u times
+ * the kept weight.  temperature <= 0: the largest logit (the lowest index of
+ * equal ones).  NaN logits count as -infinity; a row without any logit above
+ * -infinity gives -1.  Each setting is a device array of B values or, where
+ * that is NULL, one value for all.  V <= 327680.  Results do not depend on the
+ * order of any sum. */
+int bf16x_sample(const void *logits, int dtype, int64_t ld, int64_t B, int64_t V, const float *u,
+                 const float *temperature, float temperature0, const int32_t *top_k, int32_t top_k0,
+                 const float *top_p, float top_p0, const float *min_p, float min_p0, int64_t *tokens, void *stream);
+
 /* ---- self-test of the bounded waits ------------------------------------- */
 /* No counterpart in the reference.  Runs one of the library's bounded device
  * waits -- which: 0 the GEMV's mbarrier wait, 1 the tcgen05 GEMM roles' wait,
