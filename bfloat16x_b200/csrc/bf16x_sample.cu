@@ -18,7 +18,11 @@
 // one draw in a hundred to a neighbour.
 //
 // One cluster of C CTAs per row; each holds its part of the row as ordered
-// 32-bit keys in shared memory and the logits are read once.
+// 32-bit keys in shared memory and the logits are read once.  A histogram of
+// (top - l) in 1/32 octaves of weight then says in which bin a cut lies.  If
+// all tokens down to that bin are few, one CTA sorts them and finishes alone
+// (the usual top-k, and top-p over a peaked row).  Otherwise the weight above
+// the bin is summed exactly and only the bin's own tokens are sorted.
 #include <algorithm>
 
 #include <cooperative_groups.h>
@@ -33,7 +37,8 @@ namespace bf16x {
 
 constexpr int kSampleWarps = 16;
 constexpr int kSampleThreads = kSampleWarps * 32;
-constexpr int kSampleBins = 2048;
+constexpr int kSampleBins = 1600;                     // 50 octaves: weights below 2^-49 are 0
+constexpr int kSampleCap = 1024;                      // tokens that one CTA sorts
 constexpr int kSampleMaxKeys = 40960;                 // keys per CTA (160 KB)
 constexpr int kSampleMaxCluster = 8;
 constexpr uint32_t kKeyNegInf = 0x007FFFFFu;          // key of -infinity
@@ -49,16 +54,24 @@ struct SampleParams {
     int64_t *tokens;
 };
 
-// 2^(-i/32)
-__constant__ double c_exp2_tab[32] = {
-    1, 0.97857206208770009, 0.9576032806985737, 0.93708381705514998,
-    0.91700404320467122, 0.89735453750155358, 0.87812608018664973, 0.85930964906123897,
-    0.8408964152537145, 0.82287773907698247, 0.80524516597462714, 0.78799042255394325,
-    0.77110541270397037, 0.75458221379671142, 0.73841307296974967, 0.72259040348852333,
-    0.70710678118654757, 0.69195494098191601, 0.67712777346844633, 0.66261832157987066,
-    0.64841977732550482, 0.63452547859586661, 0.620928906036742, 0.60762367999023448,
-    0.59460355750136051, 0.58186242938878874, 0.56939431737834578, 0.55719337129794622,
-    0.54525386633262884, 0.53357020033841185, 0.52213689121370688, 0.51094857432705831};
+// 2^(-i/64)
+__constant__ double c_exp2_tab[64] = {
+    1, 0.98922801319397546, 0.97857206208770009, 0.96803089674614717,
+    0.9576032806985737, 0.9472879907934828, 0.93708381705514998, 0.92698956254169274,
+    0.91700404320467122, 0.90712608775019943, 0.89735453750155358, 0.88768824626326059,
+    0.87812608018664973, 0.86866691763685311, 0.85930964906123897, 0.85005317685926174,
+    0.8408964152537145, 0.83183829016336819, 0.82287773907698247, 0.81401371092867392,
+    0.80524516597462714, 0.7965710756711335, 0.78799042255394325, 0.77950220011891846,
+    0.77110541270397037, 0.76279907537226921, 0.75458221379671142, 0.74645386414563242,
+    0.73841307296974967, 0.73045889709032352, 0.72259040348852333, 0.71480666919598501,
+    0.70710678118654757, 0.69948983626915562, 0.69195494098191601, 0.68450121148729526,
+    0.67712777346844633, 0.66983376202665146, 0.66261832157987066, 0.65548060576238221,
+    0.64841977732550482, 0.64143500803938913, 0.63452547859586661, 0.62769037851234555,
+    0.620928906036742, 0.61424026805343501, 0.60762367999023448, 0.60107836572635154,
+    0.59460355750136051, 0.58819849582514061, 0.58186242938878874, 0.57559461497649134,
+    0.56939431737834578, 0.56326080930412092, 0.55719337129794622, 0.55119129165392045,
+    0.54525386633262884, 0.53938039887855993, 0.53357020033841185, 0.52782258918027858,
+    0.52213689121370688, 0.51651243951061421, 0.51094857432705831, 0.50544464302585024};
 
 // order-preserving key of a logit; NaN counts as -infinity, -0 as 0
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -70,11 +83,13 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
     return __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
 }
 
-// w = 2^-y in steps of 2^-sh: y = k/32 + g with |g| <= 1/64, so 2^-y =
-// 2^(-k/32) e^(-g ln 2), the last factor by its Taylor series to the 6th power
-// (|g ln 2| <= 0.0109: the rest is below 4e-18).
+// w = 2^-y in steps of 2^-sh: y = k/64 + g with |g| <= 1/128, so 2^-y =
+// 2^(-k/64) e^(-g ln 2), the last factor by its Taylor series to the 4th power
+// (|g ln 2| <= 0.0055: the rest is below 5e-14).  One call is a dozen fp64
+// operations, which is what a pass over many tokens costs.
 struct Weigher {
-    double top, inv;                                  // maximum logit, log2(e) / temperature
+    double top, inv, scale;                           // maximum logit, log2(e) / temperature, 2^sh
+    float topf, invf;
     int sh;
     uint32_t top_key;
     const double *tab;
@@ -82,131 +97,384 @@ struct Weigher {
         if (key == top_key) return 1ull << sh;
         const double y = (top - (double)logit_of(key)) * inv;
         if (!(y < (double)(sh + 2))) return 0;
-        const double magic = 6755399441055744.0 / 32.0;            // 1.5 * 2^52 / 32: rounds to a multiple of 1/32
+        const double magic = 6755399441055744.0 / 64.0;            // 1.5 * 2^52 / 64: rounds to a multiple of 1/64
         const double yr = y + magic;
         const int k = (int)(__double_as_longlong(yr) & 0xFFFFFFFFll);
-        const double x = ((yr - magic) - y) * 0.6931471805599453094;
-        double p = 1.0 / 720.0;
-        p = fma(p, x, 1.0 / 120.0);
-        p = fma(p, x, 1.0 / 24.0);
-        p = fma(p, x, 1.0 / 6.0);
-        p = fma(p, x, 0.5);
-        p = fma(p, x, 1.0);
-        p = fma(p, x, 1.0);
-        const double m = tab[k & 31] * p;                           // in (0.48, 1.02)
-        const uint64_t v = (uint64_t)__double2ll_rn(m * (double)(1ull << sh));
-        const int n = k >> 5;
+        const double g = (yr - magic) - y;
+        constexpr double L = 0.6931471805599453094;
+        double p = L * L * L * L / 24.0;
+        p = fma(p, g, L * L * L / 6.0);
+        p = fma(p, g, L * L / 2.0);
+        p = fma(p, g, L);
+        p = fma(p, g, 1.0);
+        const double m = fma(tab[k & 63] * scale, p, 4503599627370496.0);      // + 2^52: the sum's low bits are the integer
+        const uint64_t v = (uint64_t)__double_as_longlong(m) & 0xFFFFFFFFFFFFFull;
+        const int n = k >> 6;
         return n == 0 ? v : (v + (1ull << (n - 1))) >> n;
     }
+    // which 1/32 octave below the maximum a key lies in: rounded fp32 operations, so it never falls as the logit does
+    __device__ __forceinline__ float pos(uint32_t key) const { return (topf - logit_of(key)) * invf; }
+    __device__ __forceinline__ int bin(uint32_t key) const {
+        return key == top_key ? 0 : (int)fminf(pos(key), (float)(kSampleBins - 1));
+    }
 };
 
-struct SampleShared {
+struct alignas(16) SampleShared {
     uint32_t cnt[kSampleBins];
-    uint32_t limb[3][kSampleBins];                    // 16-bit limbs of the weights, summed
-    uint64_t tot_w[kSampleBins];
-    uint32_t tot_c[kSampleBins];
-    uint64_t scan_w[kSampleWarps];
+    uint32_t low[kSampleBins];                        // sum over the bin of (1 - weight / weight at the bin's start) 2^21
+    uint64_t list[kSampleCap];                        // this CTA's tokens of a bin; later the weights of `all`
+    uint64_t all[kSampleCap];                         // the cluster's (first CTA)
+    uint64_t red_w[2][kSampleWarps];
+    uint32_t red_c[2][kSampleWarps];
+    uint64_t cta_w[2];
+    uint32_t cta_c[2];
+    uint32_t n_list;
+    uint64_t scan[kSampleWarps];
     uint32_t scan_c[kSampleWarps];
-    uint32_t red_key[kSampleWarps];
-    uint64_t warp_w[kSampleWarps];
-    uint32_t warp_c[kSampleWarps];
-    uint64_t cta_w;
-    uint32_t cta_c, cta_key;
-    uint32_t pick_bin, pick_before_c;
-    uint64_t pick_before_w;
-    double tab[32];
+    // results of the first CTA, read by all
+    uint64_t out_w;
+    uint32_t out_key, out_idx;
+    int out_move;
+    int pick_bin;
+    int last_bin;
+    uint32_t pick_before, pick_count;
+    double tab[64];
 };
 
-// One digit of a search over the keys that agree with `prefix` above bit
-// `shift + bits`: the bin that holds the cut, and what lies before it.
-template <bool WEIGHT>
-__device__ void sample_digit(cg::cluster_group &cl, int C, SampleShared &sm, const uint32_t *keys, int n,
-                             const Weigher &weigh, uint32_t prefix, int shift, int bits, double target,
-                             uint64_t &before_w, uint32_t &before_c, uint32_t &bin) {
-    const int tid = threadIdx.x, nb = 1 << bits;
-    for (int i = tid; i < kSampleBins; i += kSampleThreads) {
-        sm.cnt[i] = 0;
-        sm.limb[0][i] = sm.limb[1][i] = sm.limb[2][i] = 0;
+static_assert(sizeof(SampleShared) % 16 == 0, "the keys behind it are stored 16 bytes at a time");
+
+struct SampleCtx {
+    SampleShared &sm;
+    const uint32_t *keys;
+    int n, C, rank;
+    uint32_t base;
+    int turn;                                         // of the two exchange slots
+    Weigher weigh;
+};
+
+// Sums of w and c over the cluster; before_*: those of the CTAs and warps in
+// front of this warp.  Two slots in turn: a slot is written again only after
+// another cluster barrier, when everyone has read it.
+__device__ __forceinline__ void cluster_sums(SampleCtx &x, uint64_t w, uint32_t c, uint64_t &tot_w, uint32_t &tot_c,
+                                             uint64_t &before_w) {
+    SampleShared &sm = x.sm;
+    cg::cluster_group cl = cg::this_cluster();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, s = x.turn;
+    x.turn ^= 1;
+    for (int o = 16; o; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+    c = __reduce_add_sync(0xffffffffu, c);
+    if (lane == 0) {
+        sm.red_w[s][warp] = w;
+        sm.red_c[s][warp] = c;
     }
     __syncthreads();
-    const int hi = shift + bits;
-    for (int i = tid; i < n; i += kSampleThreads) {
-        const uint32_t k = keys[i];
-        if (hi < 32 && (k >> hi) != (prefix >> hi)) continue;
-        const uint32_t d = (k >> shift) & (nb - 1);
-        const uint64_t w = weigh(k);
-        atomicAdd(&sm.cnt[d], 1u);
-        if (w) {
-            atomicAdd(&sm.limb[0][d], (uint32_t)(w & 0xFFFFu));
-            atomicAdd(&sm.limb[1][d], (uint32_t)((w >> 16) & 0xFFFFu));
-            atomicAdd(&sm.limb[2][d], (uint32_t)(w >> 32));
+    if (warp == 0) {
+        uint64_t a = lane < kSampleWarps ? sm.red_w[s][lane] : 0;
+        uint32_t b = lane < kSampleWarps ? sm.red_c[s][lane] : 0;
+        for (int o = 16; o; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+        b = __reduce_add_sync(0xffffffffu, b);
+        if (lane == 0) {
+            sm.cta_w[s] = a;
+            sm.cta_c[s] = b;
         }
     }
     cl.sync();
-    // every CTA adds up all bins of the cluster
-    for (int i = tid; i < nb; i += kSampleThreads) {
-        uint32_t c = 0;
-        uint64_t w = 0;
-        for (int r = 0; r < C; ++r) {
-            const SampleShared *o = cl.map_shared_rank(&sm, r);
-            c += o->cnt[i];
-            w += (uint64_t)o->limb[0][i] + ((uint64_t)o->limb[1][i] << 16) + ((uint64_t)o->limb[2][i] << 32);
-        }
-        sm.tot_c[i] = c;
-        sm.tot_w[i] = w;
+    tot_w = 0, tot_c = 0, before_w = 0;
+    for (int r = 0; r < x.C; ++r) {
+        const SampleShared *o = cl.map_shared_rank(&sm, r);
+        const uint64_t a = o->cta_w[s];
+        if (r < x.rank) before_w += a;
+        tot_w += a;
+        tot_c += o->cta_c[s];
     }
+    for (int i = 0; i < warp; ++i) before_w += sm.red_w[s][i];
+}
+
+// Inclusive scan over the block (w in thread order).
+__device__ __forceinline__ uint64_t block_scan(SampleShared &sm, uint64_t w) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t y = __shfl_up_sync(0xffffffffu, w, o);
+        if (lane >= o) w += y;
+    }
+    if (lane == 31) sm.scan[warp] = w;
     __syncthreads();
+    for (int i = 0; i < warp; ++i) w += sm.scan[i];
+    __syncthreads();
+    return w;
+}
+
+// Ascending sort of a[0, n2), n2 a power of two >= 64, by the whole block.
+// Pairs within a warp's own 64 elements need only the warp.
+__device__ void block_sort(uint64_t *a, int n2) {
+    const int tid = threadIdx.x;
+    for (int size = 2; size <= n2; size <<= 1)
+        for (int j = size >> 1; j; j >>= 1) {
+            for (int p = tid; p < n2 / 2; p += kSampleThreads) {
+                const int i = ((p & ~(j - 1)) << 1) | (p & (j - 1));
+                const uint64_t u = a[i], v = a[i + j];
+                const bool up = (i & size) == 0;
+                if ((u > v) == up) {
+                    a[i] = v;
+                    a[i + j] = u;
+                }
+            }
+            const int next = j > 1 ? j >> 1 : size;                 // distance of the following step
+            if (j > 32 || next > 32) __syncthreads();
+            else __syncwarp();
+        }
+    __syncthreads();
+}
+
+// The first CTA's `all` filled with the cluster's listed tokens, sorted into
+// the order (key down, index up).  Called by all; returns their number there.
+__device__ int gather_sorted(SampleCtx &x, int &n2) {
+    SampleShared &sm = x.sm;
+    cg::cluster_group cl = cg::this_cluster();
+    int m = 0;
+    for (int r = 0; r < x.C; ++r) {
+        const SampleShared *o = cl.map_shared_rank(&sm, r);
+        const int k = (int)o->n_list;
+        for (int i = threadIdx.x; i < k; i += kSampleThreads) sm.all[m + i] = o->list[i];
+        m += k;
+    }
+    n2 = 64;
+    while (n2 < m) n2 <<= 1;
+    for (int i = m + threadIdx.x; i < n2; i += kSampleThreads) sm.all[i] = ~0ull;
+    __syncthreads();
+    block_sort(sm.all, n2);
+    return m;
+}
+
+// Token i of this CTA into its list, if `take` (called by whole warps).
+__device__ __forceinline__ void list_tokens(SampleCtx &x, int i, bool take) {
+    SampleShared &sm = x.sm;
+    const uint32_t mask = __ballot_sync(0xffffffffu, take);
+    if (mask == 0) return;
+    const int lane = threadIdx.x & 31, lead = __ffs(mask) - 1;
+    uint32_t at = 0;
+    if (lane == lead) at = atomicAdd(&sm.n_list, (uint32_t)__popc(mask));
+    at = __shfl_sync(0xffffffffu, at, lead) + __popc(mask & ((1u << lane) - 1u));
+    if (take && at < kSampleCap) sm.list[at] = (uint64_t)(~x.keys[i]) << 32 | (x.base + (uint32_t)i);
+}
+
+// The first bin at which the running count reaches k (k > 0) or the running
+// weight, as far as the histogram knows it, reaches target; the last occupied
+// bin if none does.  Sets pick_bin, pick_before (tokens before the bin),
+// pick_count (in it, 0 where none reaches it).
+__device__ void find_bin(SampleCtx &x, uint32_t k, double target) {
+    SampleShared &sm = x.sm;
+    cg::cluster_group cl = cg::this_cluster();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    uint32_t run_c = 0;
+    uint64_t run_w = 0;
+    if (tid == 0) sm.pick_bin = -1, sm.pick_before = 0, sm.pick_count = 0, sm.last_bin = 0;
+    __syncthreads();
+    for (int b0 = 0; b0 < kSampleBins; b0 += kSampleThreads) {
+        const int b = b0 + tid;
+        uint32_t c = 0, low = 0;
+        uint64_t lows = 0;
+        if (b < kSampleBins)
+            for (int r = 0; r < x.C; ++r) {
+                const SampleShared *o = cl.map_shared_rank(&sm, r);
+                c += o->cnt[b];
+                low = o->low[b];
+                lows += low;
+            }
+        const double start = x.weigh.tab[(2 * b) & 63] * x.weigh.scale;
+        uint64_t w = c ? (uint64_t)(start * ((double)c - (double)lows * 0x1p-21)) >> (b >> 5) : 0;
+        // inclusive scans of c and w
+        uint32_t sc = c;
+        uint64_t sw = w;
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t yc = __shfl_up_sync(0xffffffffu, sc, o);
+            const uint64_t yw = __shfl_up_sync(0xffffffffu, sw, o);
+            if (lane >= o) sc += yc, sw += yw;
+        }
+        if (lane == 31) sm.scan[warp] = sw, sm.scan_c[warp] = sc;
+        __syncthreads();
+        uint32_t all_c = run_c;
+        uint64_t all_w = run_w;
+        for (int i = 0; i < kSampleWarps; ++i) {
+            if (i == warp) sc += all_c, sw += all_w;
+            all_c += sm.scan_c[i];
+            all_w += sm.scan[i];
+        }
+        const bool after = k ? sc >= k : (double)sw >= target, before = k ? sc - c >= k : (double)(sw - w) >= target;
+        if (c && after && !before) {                                // one thread at most
+            sm.pick_bin = b;
+            sm.pick_before = sc - c;
+            sm.pick_count = c;
+        }
+        if (c) atomicMax(&sm.last_bin, b);
+        const int found = __syncthreads_or(c && after);
+        run_c = all_c, run_w = all_w;
+        if (found) return;
+    }
+    // not reached: the whole row
     if (tid == 0) {
-        // from the largest digit down
-        uint64_t bw = before_w;
-        uint32_t bc = before_c;
-        int i = nb - 1;
-        int last = -1;
-        uint64_t lw = 0;
-        uint32_t lc = 0;
-        for (; i >= 0; --i) {
-            if (sm.tot_c[i] == 0) continue;
-            last = i, lw = bw, lc = bc;
-            if (WEIGHT ? (double)(bw + sm.tot_w[i]) >= target : (double)(bc + sm.tot_c[i]) >= target) break;
-            bw += sm.tot_w[i];
-            bc += sm.tot_c[i];
-        }
-        // never reached (rounding of the target, or fewer tokens than k): the last bin there is
-        sm.pick_bin = (uint32_t)max(last, 0);
-        sm.pick_before_w = lw;
-        sm.pick_before_c = lc;
+        sm.pick_bin = sm.last_bin;
+        sm.pick_before = run_c;
+        sm.pick_count = 0;
     }
     __syncthreads();
-    bin = sm.pick_bin;
-    before_w = sm.pick_before_w;
-    before_c = sm.pick_before_c;
-    cl.sync();                                        // the bins are read by all before they are cleared again
 }
 
-// The shortest prefix of the order that reaches the target: its last key, how
-// many of that key's ties belong to it, and the weight of the prefix.
-template <bool WEIGHT>
-__device__ void sample_select(cg::cluster_group &cl, int C, SampleShared &sm, const uint32_t *keys, int n,
-                              const Weigher &weigh, double target, uint32_t &cut, uint32_t &ties, uint64_t &sum) {
-    uint64_t bw = 0;
-    uint32_t bc = 0, bin, prefix = 0;
-    sample_digit<WEIGHT>(cl, C, sm, keys, n, weigh, prefix, 21, 11, target, bw, bc, bin);
-    prefix |= bin << 21;
-    sample_digit<WEIGHT>(cl, C, sm, keys, n, weigh, prefix, 10, 11, target, bw, bc, bin);
-    prefix |= bin << 10;
-    sample_digit<WEIGHT>(cl, C, sm, keys, n, weigh, prefix, 0, 10, target, bw, bc, bin);
-    prefix |= bin;
-    const uint64_t w = weigh(prefix);
-    const uint32_t have = sm.tot_c[bin];
-    double need;
-    if (WEIGHT) need = w ? ceil((target - (double)bw) / (double)w) : 1.0;
-    else need = target - (double)bc;
-    ties = (uint32_t)fmin(fmax(need, 1.0), (double)have);
-    cut = prefix;
-    sum = bw + (uint64_t)ties * w;
+// Bisection over keys, then over indices, for bins with more tokens than one
+// CTA sorts (rows of a few distinct values): one exact sum over the cluster per
+// step.  K: by count (target = tokens still to take from the bin), else by
+// weight.  The cut and the weight of the bin's part before and with it.
+template <bool K>
+__device__ void bisect(SampleCtx &x, int b, double target, uint32_t &cut_key, uint32_t &cut_idx, uint64_t &part) {
+    const int tid = threadIdx.x;
+    uint32_t lo = 0, hi = x.weigh.top_key;
+    uint64_t tw, bw;
+    uint32_t tc;
+    while (lo < hi) {                                               // the largest key down to which the target is reached
+        const uint32_t mid = lo + (hi - lo) / 2 + 1;
+        uint64_t w = 0;
+        uint32_t c = 0;
+        for (int i = tid; i < x.n; i += kSampleThreads) {
+            const uint32_t k = x.keys[i];
+            if (k >= mid && x.weigh.bin(k) == b) {
+                if (K) ++c;
+                else w += x.weigh(k);
+            }
+        }
+        cluster_sums(x, w, c, tw, tc, bw);
+        if (K ? (double)tc >= target : (double)tw >= target) lo = mid;
+        else hi = mid - 1;
+    }
+    cut_key = lo;
+    uint64_t w = 0;
+    uint32_t c = 0;
+    for (int i = tid; i < x.n; i += kSampleThreads) {
+        const uint32_t k = x.keys[i];
+        if (k > lo && x.weigh.bin(k) == b) ++c, w += x.weigh(k);
+    }
+    cluster_sums(x, w, c, tw, tc, bw);
+    const uint64_t each = x.weigh(lo);
+    const double need = K ? target - (double)tc : each ? ceil((target - (double)tw) / (double)each) : 1.0;
+    const uint32_t want = (uint32_t)fmin(fmax(need, 1.0), 4294967295.0);
+    uint32_t j0 = 0, j1 = 0xFFFFFFFFu;                              // the lowest index up to which `want` ties lie
+    uint32_t ties = 0;
+    while (j0 < j1) {
+        const uint32_t mid = j0 + (j1 - j0) / 2;
+        c = 0;
+        for (int i = tid; i < x.n; i += kSampleThreads) c += x.keys[i] == lo && x.base + (uint32_t)i <= mid;
+        uint64_t zero;
+        cluster_sums(x, 0, c, zero, ties, bw);
+        if (ties >= want) j1 = mid;
+        else j0 = mid + 1;
+    }
+    cut_idx = j0;
+    part = tw + (uint64_t)want * each;
 }
 
-__global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleParams p) {
+// The occupied bin next to b in direction d (b where there is none).
+__device__ int next_bin(SampleCtx &x, int b, int d) {
+    cg::cluster_group cl = cg::this_cluster();
+    for (int i = b + d; i >= 0 && i < kSampleBins; i += d)
+        for (int r = 0; r < x.C; ++r)
+            if (cl.map_shared_rank(&x.sm, r)->cnt[i]) return i;
+    return b;
+}
+
+// The exact cut at or near bin b: K: the first `k` tokens of the order (`count`
+// of them lie before the bin); else the shortest prefix that weighs `target`.
+// `sum`: the weight of the prefix.
+template <bool K>
+__device__ void resolve(SampleCtx &x, int b, uint32_t count, uint32_t k, double target,
+                        uint32_t &cut_key, uint32_t &cut_idx, uint64_t &sum) {
+    SampleShared &sm = x.sm;
+    cg::cluster_group cl = cg::this_cluster();
+    const int tid = threadIdx.x;
+    for (;;) {
+        if (tid == 0) sm.n_list = 0;
+        __syncthreads();
+        uint64_t w = 0;
+        uint32_t c = 0;
+        for (int i0 = 0; i0 < x.n; i0 += kSampleThreads) {
+            const int i = i0 + tid;
+            const uint32_t key = i < x.n ? x.keys[i] : 0u;
+            const int kb = i < x.n ? x.weigh.bin(key) : kSampleBins;
+            if (kb < b) w += x.weigh(key);
+            if (kb == b) ++c;
+            list_tokens(x, min(i, x.n - 1), kb == b);
+        }
+        uint64_t before, skip;
+        uint32_t m;
+        cluster_sums(x, w, c, before, m, skip);
+        if (m > (uint32_t)kSampleCap) {
+            uint64_t part;
+            double need = K ? (double)(k - count) : target - (double)before;
+            if (!K) {                                               // whether the cut lies in this bin at all
+                uint64_t bin_w = 0, t2, s2;
+                uint32_t c2;
+                for (int i = tid; i < x.n; i += kSampleThreads)
+                    if (x.weigh.bin(x.keys[i]) == b) bin_w += x.weigh(x.keys[i]);
+                cluster_sums(x, bin_w, 0, t2, c2, s2);
+                const int to = need <= 0.0 ? next_bin(x, b, -1) : need > (double)t2 ? next_bin(x, b, 1) : b;
+                if (to != b) {
+                    b = to;
+                    continue;
+                }
+                need = fmin(need, (double)t2);
+            }
+            bisect<K>(x, b, need, cut_key, cut_idx, part);
+            sum = before + part;
+            return;
+        }
+        if (x.rank == 0) {
+            int n2;
+            const int got = gather_sorted(x, n2);
+            // prefix weights, n2 / 512 tokens per thread
+            const int per = (n2 + kSampleThreads - 1) / kSampleThreads;
+            uint64_t mine[kSampleCap / kSampleThreads], s = 0;
+#pragma unroll
+            for (int q = 0; q < kSampleCap / kSampleThreads; ++q) {
+                const int e = tid * per + q;
+                mine[q] = q < per && e < got ? x.weigh(~(uint32_t)(sm.all[e] >> 32)) : 0;
+                s += mine[q];
+            }
+            uint64_t run = block_scan(sm, s) - s;
+            if (tid == 0) sm.out_move = got == 0 || (!K && target <= (double)before) ? -1 : 1;
+            __syncthreads();
+            const bool down = sm.out_move < 0;
+            __syncthreads();
+#pragma unroll
+            for (int q = 0; q < kSampleCap / kSampleThreads; ++q) {
+                const int e = tid * per + q;
+                if (q >= per || e >= got) break;
+                const uint64_t upto = before + run + mine[q];
+                const bool hit = K ? (uint32_t)e + 1 == k - count
+                                   : !down && (double)upto >= target && (double)(before + run) < target;
+                if (hit) {
+                    sm.out_move = 0;
+                    sm.out_key = ~(uint32_t)(sm.all[e] >> 32);
+                    sm.out_idx = (uint32_t)sm.all[e];
+                    sm.out_w = upto;
+                }
+                run += mine[q];
+            }
+            __syncthreads();
+        }
+        cl.sync();
+        const SampleShared *o = cl.map_shared_rank(&sm, 0);
+        const int move = o->out_move;
+        cut_key = o->out_key, cut_idx = o->out_idx, sum = o->out_w;
+        cl.sync();
+        if (move == 0) return;
+        const int to = next_bin(x, b, move);
+        if (to == b) {                                              // no such bin: the cut is at the end of the row
+            cut_key = move < 0 ? x.weigh.top_key : kKeyNegInf, cut_idx = 0xFFFFFFFFu;
+            return;
+        }
+        b = to;
+    }
+}
+
+__global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const SampleParams p) {
     extern __shared__ __align__(16) uint8_t smem_raw[];
     SampleShared &sm = *reinterpret_cast<SampleShared *>(smem_raw);
     uint32_t *keys = reinterpret_cast<uint32_t *>(smem_raw + sizeof(SampleShared));
@@ -214,146 +482,247 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SamplePara
     const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     griddep_launch_dependents();
+    if (tid < 64) sm.tab[tid] = c_exp2_tab[tid];
+    for (int i = tid; i < kSampleBins; i += kSampleThreads) sm.cnt[i] = sm.low[i] = 0;
+    if (tid == 0) sm.n_list = 0;
     griddep_wait();
     const int64_t row = blockIdx.x / C;
     const int64_t chunk = (int64_t)p.seg * kSampleWarps, base = rank * chunk;
     const int n = (int)max((int64_t)0, min(chunk, p.V - base));
-    if (tid < 32) sm.tab[tid] = c_exp2_tab[tid];
     // ---- the row's part as keys, and the maximum
     uint32_t top = 0;
-    for (int i = tid; i < n; i += kSampleThreads) {
-        const int64_t at = row * p.ld + base + i;
-        const float x = p.bf16 ? bf16_bits_to_f32(static_cast<const uint16_t *>(p.logits)[at])
-                               : static_cast<const float *>(p.logits)[at];
-        const uint32_t k = key_of(x);
-        keys[i] = k;
-        top = max(top, k);
+    {
+        const uint8_t *src = static_cast<const uint8_t *>(p.logits) + (row * p.ld + base) * (p.bf16 ? 2 : 4);
+        const bool vec = ((uintptr_t)src & 15) == 0;
+        int done = 0;
+        if (vec && p.bf16) {
+            done = n & ~7;
+#pragma unroll 4
+            for (int i = 8 * tid; i < done; i += 8 * kSampleThreads) {
+                const uint4 v = __ldcs(reinterpret_cast<const uint4 *>(src + 2 * i));
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                uint32_t k[8];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    k[2 * j] = key_of(__uint_as_float(w[j] << 16));
+                    k[2 * j + 1] = key_of(__uint_as_float(w[j] & 0xFFFF0000u));
+                    top = max(top, max(k[2 * j], k[2 * j + 1]));
+                }
+                *reinterpret_cast<uint4 *>(keys + i) = make_uint4(k[0], k[1], k[2], k[3]);
+                *reinterpret_cast<uint4 *>(keys + i + 4) = make_uint4(k[4], k[5], k[6], k[7]);
+            }
+        } else if (vec) {
+            done = n & ~3;
+#pragma unroll 8
+            for (int i = 4 * tid; i < done; i += 4 * kSampleThreads) {
+                const float4 v = __ldcs(reinterpret_cast<const float4 *>(src + 4 * i));
+                const uint4 k = make_uint4(key_of(v.x), key_of(v.y), key_of(v.z), key_of(v.w));
+                top = max(max(top, max(k.x, k.y)), max(k.z, k.w));
+                *reinterpret_cast<uint4 *>(keys + i) = k;
+            }
+        }
+        for (int i = done + tid; i < n; i += kSampleThreads) {
+            const float v = p.bf16 ? bf16_bits_to_f32(reinterpret_cast<const uint16_t *>(src)[i])
+                                   : reinterpret_cast<const float *>(src)[i];
+            const uint32_t k = key_of(v);
+            keys[i] = k;
+            top = max(top, k);
+        }
     }
     top = __reduce_max_sync(0xffffffffu, top);
-    if (lane == 0) sm.red_key[warp] = top;
+    if (lane == 0) sm.red_c[0][warp] = top;
     __syncthreads();
-    if (tid == 0) {
-        for (int w = 0; w < kSampleWarps; ++w) top = max(top, sm.red_key[w]);
-        sm.cta_key = top;
+    if (warp == 0) {
+        top = __reduce_max_sync(0xffffffffu, lane < kSampleWarps ? sm.red_c[0][lane] : 0u);
+        if (lane == 0) sm.cta_c[0] = top;
     }
     cl.sync();
     top = 0;
-    for (int r = 0; r < C; ++r) top = max(top, cl.map_shared_rank(&sm, r)->cta_key);
+    for (int r = 0; r < C; ++r) top = max(top, cl.map_shared_rank(&sm, r)->cta_c[0]);
     const float temp = p.temperature ? p.temperature[row] : p.temperature0;
     const float top_p = p.top_p ? p.top_p[row] : p.top_p0, min_p = p.min_p ? p.min_p[row] : p.min_p0;
     const int32_t top_k = p.top_k ? p.top_k[row] : p.top_k0;
-    // ---- the cut
-    Weigher weigh;
+    const float u = p.u[row];
+    SampleCtx x = {sm, keys, n, C, rank, (uint32_t)base, 1, {}};
+    Weigher &weigh = x.weigh;
     weigh.top = (double)logit_of(top);
     weigh.inv = 1.4426950408889634074 / (double)temp;
+    weigh.scale = (double)(1ull << p.sh);
+    weigh.topf = logit_of(top);
+    weigh.invf = 32.f * (1.44269504f / temp);
     weigh.sh = p.sh;
     weigh.top_key = top;
     weigh.tab = sm.tab;
-    uint32_t cut = kKeyNegInf, ties = 0;              // keep keys above the cut, and the first `ties` of its own
-    uint64_t min_w = 1;
-    const bool none = top <= kKeyNegInf;              // nothing to choose from
-    if (none) {
-        cut = 0xFFFFFFFFu;
-    } else if (!(temp > 0.f) || top_k == 1) {
-        cut = top;
-        ties = 1;
-    } else {
-        uint64_t sum = 0;
-        bool have_sum = false;
-        if (top_k > 0 && top_k < p.V) {
-            sample_select<false>(cl, C, sm, keys, n, weigh, (double)top_k, cut, ties, sum);
-            have_sum = true;
-        }
-        if (top_p < 1.f) {
-            if (!have_sum) {
-                uint64_t w = 0;
-                for (int i = tid; i < n; i += kSampleThreads) w += weigh(keys[i]);
-                for (int o = 16; o; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
-                if (lane == 0) sm.warp_w[warp] = w;
-                __syncthreads();
-                if (tid == 0) {
-                    w = 0;
-                    for (int i = 0; i < kSampleWarps; ++i) w += sm.warp_w[i];
-                    sm.cta_w = w;
+    const bool none = top <= kKeyNegInf, greedy = !(temp > 0.f) || top_k == 1;
+    if (none || greedy) {
+        // ---- the lowest index of the maximum
+        uint32_t at = 0xFFFFFFFFu;
+        if (!none)
+            for (int i = tid; i < n; i += kSampleThreads)
+                if (keys[i] == top) {
+                    at = (uint32_t)base + (uint32_t)i;
+                    break;
                 }
-                cl.sync();
-                for (int r = 0; r < C; ++r) sum += cl.map_shared_rank(&sm, r)->cta_w;
-                cl.sync();
-            }
-            sample_select<true>(cl, C, sm, keys, n, weigh, (double)top_p * (double)sum, cut, ties, sum);
+        at = __reduce_min_sync(0xffffffffu, at);
+        if (lane == 0) sm.red_c[1][warp] = at;
+        __syncthreads();
+        if (tid == 0) {
+            for (int w = 0; w < kSampleWarps; ++w) at = min(at, sm.red_c[1][w]);
+            sm.cta_c[1] = at;
         }
-        if (min_p > 0.f) min_w = max((uint64_t)1, (uint64_t)ceil(fmin((double)min_p, 1.0) * (double)(1ull << p.sh)));
+        cl.sync();
+        if (rank == 0 && tid == 0) {
+            for (int r = 0; r < C; ++r) at = min(at, cl.map_shared_rank(&sm, r)->cta_c[1]);
+            p.tokens[row] = none ? -1 : (int64_t)at;
+        }
+        cl.sync();
+        return;
     }
-    // ---- ties before each warp's part, in index order
-    const int s0 = warp * p.seg, s1 = min(n, s0 + p.seg);
-    uint32_t c = 0;
-    for (int i = s0 + lane; i < s1; i += 32) c += keys[i] == cut;
-    c = __reduce_add_sync(0xffffffffu, c);
-    if (lane == 0) sm.warp_c[warp] = c;
-    __syncthreads();
-    if (tid == 0) {
-        c = 0;
-        for (int w = 0; w < kSampleWarps; ++w) c += sm.warp_c[w];
-        sm.cta_c = c;
+    const uint64_t min_w =
+        min_p > 0.f ? max((uint64_t)1, (uint64_t)ceil(fmin((double)min_p, 1.0) * (double)(1ull << p.sh))) : 1ull;
+    uint32_t cut_key = kKeyNegInf, cut_idx = 0xFFFFFFFFu;           // keep keys above the cut, and its own up to an index
+    const bool by_k = top_k > 0 && top_k < p.V, by_p = top_p < 1.f;
+    if (by_k || by_p) {
+        // ---- the histogram, and the row's whole weight where top-p needs it
+        uint64_t w = 0, total, skip;
+        for (int i = tid; i < n; i += kSampleThreads) {
+            const uint32_t k = keys[i];
+            const float f = k == top ? 0.f : weigh.pos(k);
+            if (!(f < (float)(kSampleBins - 1))) continue;
+            const int b = (int)f;
+            atomicAdd(&sm.cnt[b], 1u);
+            if (by_p) {
+                float r;
+                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"((f - (float)b) * -0.03125f));
+                atomicAdd(&sm.low[b], (uint32_t)((1.f - r) * 2097152.f));
+                if (!by_k) w += weigh(k);
+            }
+        }
+        uint32_t c;
+        cluster_sums(x, w, 0, total, c, skip);
+        find_bin(x, by_k ? (uint32_t)top_k : 0u, fmax((double)top_p * (double)total, 1.0));
+        int b = sm.pick_bin;
+        uint32_t before = sm.pick_before, count = sm.pick_count;
+        const bool few = before + count <= (uint32_t)kSampleCap && b < kSampleBins - 1;
+        bool finish = false;
+        if (few) {
+            // ---- all that can be kept on one CTA
+            for (int i0 = 0; i0 < n; i0 += kSampleThreads) {
+                const int i = i0 + tid;
+                list_tokens(x, min(i, n - 1), i < n && weigh.bin(keys[i]) <= b);
+            }
+            cl.sync();
+            if (rank == 0) {
+                int n2;
+                const int m = gather_sorted(x, n2);
+                const int per = (n2 + kSampleThreads - 1) / kSampleThreads;
+                uint64_t mine[kSampleCap / kSampleThreads], s = 0;
+#pragma unroll
+                for (int q = 0; q < kSampleCap / kSampleThreads; ++q) {
+                    const int e = tid * per + q;
+                    const bool in = q < per && e < m && (!by_k || e < top_k);
+                    mine[q] = in ? weigh(~(uint32_t)(sm.all[e] >> 32)) : 0;
+                    s += mine[q];
+                }
+                const uint64_t upto = block_scan(sm, s);
+                if (tid == kSampleThreads - 1) sm.out_w = upto;
+                __syncthreads();
+                const uint64_t listed = sm.out_w;
+                const double target = fmax((double)top_p * (double)(by_k ? listed : total), 1.0);
+                // top-p alone: the histogram's estimate may have missed the cut
+                finish = !(by_p && !by_k && (double)listed < target);
+                if (finish) {
+                    uint64_t run = upto - s, kept = 0;
+#pragma unroll
+                    for (int q = 0; q < kSampleCap / kSampleThreads; ++q) {
+                        const int e = tid * per + q;
+                        if (q >= per || e >= n2) break;
+                        const uint64_t one = (by_p && (double)run >= target && e > 0) || mine[q] < min_w ? 0 : mine[q];
+                        run += mine[q];
+                        kept += one;
+                        sm.list[e] = one;
+                    }
+                    __syncthreads();
+                    for (int e = tid; e < n2; e += kSampleThreads)
+                        sm.all[e] = e < m && sm.list[e] ? sm.all[e] << 32 | (uint32_t)e : ~0ull;    // by index
+                    kept = block_scan(sm, kept);
+                    if (tid == kSampleThreads - 1) sm.out_w = kept;
+                    __syncthreads();
+                    const uint64_t sum = sm.out_w;
+                    block_sort(sm.all, n2);
+                    const double ut = fmax((double)u, 0.0) * (double)sum;
+                    const uint64_t goal = min(ut < (double)sum ? (uint64_t)ut : sum - 1, sum - 1);
+                    s = 0;
+#pragma unroll
+                    for (int q = 0; q < kSampleCap / kSampleThreads; ++q) {
+                        const int e = tid * per + q;
+                        mine[q] = q < per && e < n2 && sm.all[e] != ~0ull ? sm.list[(uint32_t)sm.all[e]] : 0;
+                        s += mine[q];
+                    }
+                    run = block_scan(sm, s) - s;
+#pragma unroll
+                    for (int q = 0; q < kSampleCap / kSampleThreads; ++q) {
+                        if (goal >= run && goal < run + mine[q])     // exactly one
+                            p.tokens[row] = (int64_t)(sm.all[tid * per + q] >> 32);
+                        run += mine[q];
+                    }
+                }
+                if (tid == 0) sm.out_move = finish ? 1 : 0;
+            }
+            cl.sync();
+            finish = cl.map_shared_rank(&sm, 0)->out_move == 1;
+            cl.sync();
+            if (finish) return;
+        }
+        uint64_t sum = total;
+        if (by_k && count > 0) {
+            resolve<true>(x, b, before, (uint32_t)top_k, 0.0, cut_key, cut_idx, sum);
+        } else if (by_k && by_p) {                                  // k reaches past every weight
+            uint64_t all = 0;
+            for (int i = tid; i < n; i += kSampleThreads) all += weigh(keys[i]);
+            cluster_sums(x, all, 0, sum, c, skip);
+        }
+        if (by_p) {
+            const double target = fmax((double)top_p * (double)sum, 1.0);
+            if (by_k) {
+                find_bin(x, 0u, target);
+                b = sm.pick_bin;
+                __syncthreads();
+            }
+            resolve<false>(x, b, 0, 0, target, cut_key, cut_idx, sum);
+        }
     }
-    cl.sync();
-    uint32_t tie0 = 0;
-    for (int r = 0; r < rank; ++r) tie0 += cl.map_shared_rank(&sm, r)->cta_c;
-    for (int w = 0; w < warp; ++w) tie0 += sm.warp_c[w];
     // ---- the kept weight of each warp's part
-    const auto kept = [&](int i, uint32_t &tie) -> uint64_t {       // whole warp; i may lie past the part's end
-        const uint32_t k = i < s1 ? keys[i] : 0u;
-        const uint32_t same = __ballot_sync(0xffffffffu, i < s1 && k == cut);
-        const uint32_t before = tie + __popc(same & ((1u << lane) - 1u));
-        tie += __popc(same);
-        if (i >= s1 || k < cut || (k == cut && before >= ties)) return 0;
+    const int s0 = warp * p.seg, s1 = min(n, s0 + p.seg);
+    const auto kept = [&](int i) -> uint64_t {
+        if (i >= s1) return 0;
+        const uint32_t k = keys[i];
+        if (k < cut_key || (k == cut_key && (uint32_t)base + (uint32_t)i > cut_idx)) return 0;
         const uint64_t w = weigh(k);
         return w >= min_w ? w : 0;
     };
-    uint64_t w = 0;
-    uint32_t tie = tie0;
-    if (!none)
-        for (int i = s0; i < s1; i += 32) w += kept(i + lane, tie);
+    uint64_t w = 0, total, before;
+    uint32_t c;
+    for (int i = s0; i < s1; i += 32) w += kept(i + lane);
+    cluster_sums(x, w, 0, total, c, before);
     for (int o = 16; o; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
-    if (lane == 0) sm.warp_w[warp] = w;
-    __syncthreads();
-    if (tid == 0) {
-        w = 0;
-        for (int i = 0; i < kSampleWarps; ++i) w += sm.warp_w[i];
-        sm.cta_w = w;
-    }
-    cl.sync();
-    uint64_t total = 0, before = 0;
-    for (int r = 0; r < C; ++r) {
-        const uint64_t x = cl.map_shared_rank(&sm, r)->cta_w;
-        if (r < rank) before += x;
-        total += x;
-    }
-    for (int i = 0; i < warp; ++i) before += sm.warp_w[i];
-    w = sm.warp_w[warp];
-    if (none) {
-        if (rank == 0 && tid == 0) p.tokens[row] = -1;
-    } else {
-        // ---- the first token whose running sum exceeds u * total
-        const double ut = fmax((double)p.u[row], 0.0) * (double)total;
-        uint64_t target = ut < (double)total ? (uint64_t)ut : total;
-        if (target >= total) target = total - 1;
-        if (target >= before && target < before + w) {              // exactly one warp of the cluster
-            uint64_t run = before;
-            tie = tie0;
-            for (int i = s0; i < s1; i += 32) {
-                uint64_t x = kept(i + lane, tie);
-                for (int o = 1; o < 32; o <<= 1) {
-                    const uint64_t y = __shfl_up_sync(0xffffffffu, x, o);
-                    if (lane >= o) x += y;
-                }
-                const uint32_t over = __ballot_sync(0xffffffffu, run + x > target);
-                if (over) {
-                    if (lane == 0) p.tokens[row] = base + i + (__ffs(over) - 1);
-                    break;
-                }
-                run += __shfl_sync(0xffffffffu, x, 31);
+    // ---- the first token whose running sum exceeds u * total
+    const double ut = fmax((double)u, 0.0) * (double)total;
+    const uint64_t goal = min(ut < (double)total ? (uint64_t)ut : total - 1, total - 1);
+    if (goal >= before && goal < before + w) {                      // exactly one warp of the cluster
+        uint64_t run = before;
+        for (int i = s0; i < s1; i += 32) {
+            uint64_t y = kept(i + lane);
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint64_t z = __shfl_up_sync(0xffffffffu, y, o);
+                if (lane >= o) y += z;
             }
+            const uint32_t over = __ballot_sync(0xffffffffu, run + y > goal);
+            if (over) {
+                if (lane == 0) p.tokens[row] = base + i + (__ffs(over) - 1);
+                break;
+            }
+            run += __shfl_sync(0xffffffffu, y, 31);
         }
     }
     cl.sync();                                        // no CTA leaves while another reads its shared memory
@@ -376,7 +745,7 @@ extern "C" int bf16x_sample(const void *logits, int dtype, int64_t ld, int64_t B
     if (B == 0) return BF16X_OK;
     if (!logits || !u || !tokens) return set_error(BF16X_ERR_INVALID, "bf16x_sample: null pointer");
     int C = 1;
-    while (C < kSampleMaxCluster && (B * C < 148 || V > (int64_t)C * kSampleMaxKeys)) C *= 2;
+    while (C < kSampleMaxCluster && (B * C < 2 * 148 || V > (int64_t)C * kSampleMaxKeys)) C *= 2;
     SampleParams p = {};
     p.logits = logits, p.ld = ld, p.V = V, p.bf16 = dtype == BF16X_DTYPE_BF16;
     p.seg = (int)((V + (int64_t)C * kSampleThreads - 1) / ((int64_t)C * kSampleThreads)) * 32;

@@ -149,3 +149,36 @@ def test_sample_distribution_and_graph():
     ud.copy_(u)
     g.replay()
     assert torch.equal(out, got)
+
+
+def _plain_fast(x, u, t, k, p, m):
+    """plain() for long rows with a temperature above 0."""
+    x = x.double()
+    s, idx = torch.sort(x, descending=True, stable=True)
+    w = torch.where(s == s[0], torch.ones_like(s), torch.exp((s - s[0]) / float(torch.tensor(t))))
+    if k:
+        w[k:] = 0
+    cum = torch.cumsum(w, 0)
+    if p < 1:
+        keep = cum - w < float(torch.tensor(p)) * cum[-1]
+        keep[0] = True
+        w = w * keep
+    w = w * (w >= float(torch.tensor(m)))
+    cum = torch.cumsum(torch.zeros_like(w).scatter_(0, idx, w), 0)
+    return int((cum <= float(u) * float(cum[-1])).sum())
+
+
+@pytest.mark.parametrize("V", [5000, 60001, 200000])
+@pytest.mark.parametrize("kind", ["equal", "two", "steps", "wide", "narrow", "flat-bf16"])
+def test_sample_many_ties_and_broad_rows(V, kind):
+    """Cuts inside bins of more tokens than one CTA sorts, and cuts after thousands of tokens."""
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn(4, V, generator=g)
+    x = {"equal": torch.full_like(x, 2.5), "two": (x > 1).float() * 0.5, "steps": (x * 2).round() / 2, "wide": x * 8,
+         "narrow": x * 1e-3, "flat-bf16": (x * 0.3).to(torch.bfloat16).float()}[kind]
+    # numbers away from the 64-bit form's own rounding where weights are equal and sums tie exactly
+    u = torch.tensor([0.0, 0.2871, 0.7313, 0.99993])
+    for t, k, p, m in ((1.0, 0, 0.9, 0.0), (0.7, 3001, 1.0, 0.0), (1.1, 4500, 0.65, 0.0), (1.0, 0, 0.9999999, 0.0),
+                       (1.0, 2, 0.5, 0.0), (1.0, 0, 0.0, 0.0), (1.0, V - 1, 0.999, 0.2), (3.0, 1025, 0.3, 0.0)):
+        got = sample(x.cuda(), u.cuda(), t, k, p, m).tolist()
+        assert got == [_plain_fast(x[i], u[i], t, k, p, m) for i in range(4)], (t, k, p, m)
