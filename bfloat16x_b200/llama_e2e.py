@@ -9,7 +9,10 @@ prefill, for the two decoder configurations of the benchmark (``CONFIGS``).
 Weights are random N(0, 0.02) (no checkpoints), drawn per weight from a
 seeded generator so that every tensor-parallel degree builds the same model;
 attention uses torch's scaled_dot_product_attention over a static KV cache,
-so one decode step has static shapes and is replayed as a CUDA graph.
+so one decode step has static shapes and is replayed as a CUDA graph.  With
+``kv_bits=4`` the cache is held in 4 bits (kv4.Kv4Cache) and attention is the
+framework's own, over what is in use of the cache, each sequence at its own
+position; ``generate`` takes the largest logit or draws (sampling.sample).
 
 Tensor parallelism (``tp`` ranks of a process group, Megatron pairing): each
 rank holds its query/key/value heads and its slice of the MLP's hidden units
@@ -28,6 +31,8 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import _lib
+from .kv4 import Kv4Cache, kv4_blocks
+from .sampling import SamplingParams, sample
 
 
 @dataclass
@@ -203,9 +208,12 @@ class Attention(nn.Module):
         w = _rand_weight(cfg.hidden, H * d, seed + 1000 * layer + 2, device)
         self.o_proj = ColumnShard(_linear_from(w[:, rank * self.h * d:(rank + 1) * self.h * d]), group, tp)
 
-    def forward(self, x, pos0, cache_k, cache_v, cos, sin, mask, tables=None):
+    def forward(self, x, pos0, cache_k, cache_v, cos, sin, mask, tables=None, kv4=None):
         B, T, _ = x.shape
         qkv = self.qkv_proj(x)
+        if kv4 is not None:
+            q = kv4.append(qkv, pos0, self.h, *tables)
+            return self.o_proj(kv4.attend(q, pos0).reshape(B, T, self.h * self.d))
         nq, nk = self.h * self.d, self.kvh * self.d
         if x.is_cuda and tables is not None:
             # rotary embedding of q and k and the cache write of k and v: one kernel
@@ -271,12 +279,17 @@ class Block(nn.Module):
 class LlamaModel(nn.Module):
     """Llama-style decoder with a static KV cache of ``max_seq`` positions for
     ``batch`` sequences; ``tp`` > 1 builds this rank's shard (``group``: the
-    tensor-parallel process group, default the world)."""
+    tensor-parallel process group, default the world).  ``kv_bits``: 16, or 4
+    for the 4-bit cache (GPU only)."""
 
     def __init__(self, cfg: LlamaConfig, max_seq: int, device, seed: int = 0, tp: int = 1, group=None,
-                 batch: int = 1):
+                 batch: int = 1, kv_bits: int = 16):
         super().__init__()
         device = torch.device(device)
+        if kv_bits not in (4, 16):
+            raise ValueError(f"kv_bits must be 4 or 16, got {kv_bits}")
+        if kv_bits == 4 and device.type != "cuda":
+            raise _lib.Bf16xError("the 4-bit cache runs on the GPU only")
         rank = dist.get_rank(group) if tp > 1 else 0
         if tp > 1 and dist.get_world_size(group) != tp:
             raise ValueError("tp must equal the size of the process group")
@@ -296,15 +309,36 @@ class LlamaModel(nn.Module):
             blk.post_attention_layernorm.to(device)
         self.cos, self.sin = _rope_tables(cfg.head_dim, max_seq, cfg.rope_theta, device)
         kvh = cfg.kv_heads // tp
-        self.cache_k = torch.zeros(cfg.layers, batch, max_seq, kvh, cfg.head_dim, dtype=torch.bfloat16, device=device)
-        self.cache_v = torch.zeros_like(self.cache_k)
+        self.kv_bits = kv_bits
+        self.cache_k = self.cache_v = self.cache_kv4 = None
+        if kv_bits == 4:
+            self.cache_kv4 = [Kv4Cache(kv4_blocks(batch, max_seq, kvh, cfg.head_dim, device), max_seq)
+                              for _ in range(cfg.layers)]
+        else:
+            self.cache_k = torch.zeros(cfg.layers, batch, max_seq, kvh, cfg.head_dim, dtype=torch.bfloat16,
+                                       device=device)
+            self.cache_v = torch.zeros_like(self.cache_k)
 
     @torch.no_grad()
     def forward(self, ids: torch.Tensor, pos0: torch.Tensor) -> torch.Tensor:
         """ids [batch, T] at positions pos0 .. pos0+T-1 (pos0: 0-d int64 device
-        tensor); returns logits of the last position [batch, vocab]."""
+        tensor; with the 4-bit cache also [batch], one per sequence, where a
+        negative position is padding); returns logits of the last position
+        [batch, vocab]."""
         T = ids.shape[1]
+        if self.cache_kv4 is None and pos0.dim() != 0:
+            raise ValueError("positions per sequence need the 4-bit cache (kv_bits=4)")
         x = self.embed_tokens(ids)
+        if self.cache_kv4 is not None:
+            tables = (self.cos, self.sin)
+            delta = None
+            for blk, kv4 in zip(self.layers, self.cache_kv4):
+                x, n1 = blk.input_layernorm.add_forward(x, delta)
+                a = blk.self_attn(n1, pos0, None, None, None, None, None, tables, kv4)
+                x, n2 = blk.post_attention_layernorm.add_forward(x, a)
+                delta = blk.mlp(n2)
+            _, h = self.norm.add_forward(x[:, -1:, :].contiguous(), delta[:, -1:, :].contiguous())
+            return self.lm_head(h).float().reshape(ids.shape[0], -1)
         pos = pos0 + torch.arange(T, device=ids.device)
         keys = torch.arange(self.max_seq, device=ids.device)
         mask = (keys[None, :] <= pos[:, None])[None, None]              # [1, 1, T, S]
@@ -384,19 +418,44 @@ def peer_heap_bytes(model: LlamaModel) -> int:
     return cfg.layers * per_layer + B * cfg.vocab * 8 + (1 << 20)
 
 
-class GraphDecoder:
-    """One decode step (a token in, the greedy next token out) captured as a
-    CUDA graph and replayed; the position lives in a device tensor."""
+class NextToken:
+    """The choice of the next token from logits: the largest, or drawn with
+    ``sampling`` from random numbers of ``generator`` (a device generator)."""
 
-    def __init__(self, model: LlamaModel, tok: torch.Tensor, pos: int):
-        """tok [batch, 1]: the first tokens to feed, at position ``pos``.  The
-        warm-up and capture write the cache row at ``pos`` only, which the
-        first replay writes again."""
+    def __init__(self, batch: int, device, sampling: SamplingParams | None = None, generator=None):
+        self.sampling, self.generator = sampling, generator
+        self.u = torch.zeros(batch, dtype=torch.float32, device=device)
+
+    def draw(self) -> None:
+        """New random numbers for the next choice (kept out of captured steps)."""
+        if self.sampling is not None:
+            torch.rand(self.u.shape, generator=self.generator, out=self.u)
+
+    def choose(self, logits: torch.Tensor) -> torch.Tensor:
+        """[batch, 1] tokens; calls between two draws use the same numbers."""
+        if self.sampling is None:
+            return logits.argmax(-1, keepdim=True)
+        s = self.sampling
+        return sample(logits, self.u, s.temperature, s.top_k, s.top_p, s.min_p).unsqueeze(1)
+
+
+class GraphDecoder:
+    """One decode step (a token in, the next token out: the largest logit, or
+    drawn with ``sampling``) captured as a CUDA graph and replayed; the
+    position lives in a device tensor."""
+
+    def __init__(self, model: LlamaModel, tok: torch.Tensor, pos, sampling: SamplingParams | None = None,
+                 generator=None):
+        """tok [batch, 1]: the first tokens to feed, at position ``pos`` (with
+        the 4-bit cache also one position per sequence).  The warm-up and
+        capture write the cache row at ``pos`` only, which the first replay
+        writes again."""
         self.model = model
-        dev = model.cache_k.device
+        dev = model.embed_tokens.weight.device
         self.tok = tok.reshape(-1, 1).clone()
-        self.pos = torch.tensor(pos, dtype=torch.long, device=dev)
+        self.pos = torch.as_tensor(pos, dtype=torch.long).to(dev, copy=True)
         self.next = torch.zeros_like(self.tok)
+        self.chooser = NextToken(self.tok.shape[0], dev, sampling, generator)
         s = torch.cuda.Stream(dev)
         s.wait_stream(torch.cuda.current_stream(dev))
         with torch.cuda.stream(s):
@@ -410,9 +469,10 @@ class GraphDecoder:
 
     def _step(self):
         logits = self.model(self.tok, self.pos)
-        self.next.copy_(logits.argmax(-1, keepdim=True))
+        self.next.copy_(self.chooser.choose(logits))
 
     def step(self):
+        self.chooser.draw()
         self.graph.replay()
         self.tok.copy_(self.next)
         self.pos += 1
@@ -463,34 +523,47 @@ def logits_rel_l2(a: torch.Tensor, b: torch.Tensor) -> tuple[float, float]:
 
 
 @torch.no_grad()
-def generate(model: LlamaModel, prompt: torch.Tensor, new_tokens: int, use_graph: bool = True):
-    """Greedy generation: prefill ``prompt`` [batch, P], then ``new_tokens``
-    decode steps.  Returns (tokens [new_tokens, batch], prefill ms, decode
+def generate(model: LlamaModel, prompt: torch.Tensor, new_tokens: int, use_graph: bool = True,
+             sampling: SamplingParams | None = None, generator=None, lengths=None):
+    """Generation: prefill ``prompt`` [batch, P], then ``new_tokens`` decode
+    steps, greedy or drawn with ``sampling`` (random numbers of ``generator``).
+    ``lengths`` (4-bit cache): the prompts' own lengths, each padded on the
+    left to P tokens.  Returns (tokens [new_tokens, batch], prefill ms, decode
     ms/token)."""
     dev = prompt.device
     P = prompt.shape[1]
     pos0 = torch.zeros((), dtype=torch.long, device=dev)
+    pos = torch.tensor(P, dtype=torch.long, device=dev)
+    if lengths is not None:
+        if model.cache_kv4 is None:
+            raise ValueError("prompts of different lengths need the 4-bit cache (kv_bits=4)")
+        pos = torch.as_tensor(lengths, dtype=torch.long).to(dev)
+        if pos.shape != (prompt.shape[0],) or int(pos.min()) < 1 or int(pos.max()) > P:
+            raise ValueError(f"lengths must be {prompt.shape[0]} numbers in 1..{P}")
+        pos0 = pos - P
+    chooser = NextToken(prompt.shape[0], dev, sampling, generator)
     a, b = torch.cuda.Event(True), torch.cuda.Event(True)
     a.record()
     logits = model(prompt, pos0)
     b.record()
     torch.cuda.synchronize(dev)
     prefill_ms = a.elapsed_time(b)
+    chooser.draw()
+    tok = chooser.choose(logits)
     out = []
     if use_graph:
-        dec = GraphDecoder(model, logits.argmax(-1, keepdim=True), P)
+        dec = GraphDecoder(model, tok, pos, sampling, generator)
         a.record()
         for _ in range(new_tokens):
             out.append(dec.tok.clone())
             dec.step()
         b.record()
     else:
-        tok = logits.argmax(-1, keepdim=True)
-        pos = torch.tensor(P, dtype=torch.long, device=dev)
         a.record()
         for _ in range(new_tokens):
             out.append(tok)
-            tok = model(tok, pos).argmax(-1, keepdim=True)
+            chooser.draw()
+            tok = chooser.choose(model(tok, pos))
             pos = pos + 1
         b.record()
     torch.cuda.synchronize(dev)
@@ -498,5 +571,5 @@ def generate(model: LlamaModel, prompt: torch.Tensor, new_tokens: int, use_graph
 
 
 __all__ = ["LlamaConfig", "CONFIGS", "LlamaModel", "ColumnShard", "VocabShard", "ResidentLinear", "pack_model",
-           "GraphDecoder", "generate", "use_peer_collectives", "peer_heap_bytes", "teacher_forced_logits",
+           "NextToken", "GraphDecoder", "generate", "SamplingParams", "use_peer_collectives", "peer_heap_bytes", "teacher_forced_logits",
            "logits_rel_l2", "fp32_linears"]

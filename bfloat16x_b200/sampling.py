@@ -3,12 +3,23 @@ given random numbers (the decoder's step after lm_head; the reference has no
 decoder of its own)."""
 from __future__ import annotations
 
+from dataclasses import dataclass
+
 import torch
 
 from . import _lib
 from ._lib import BF16X_DTYPE_BF16, BF16X_DTYPE_F32
 
 _DT = {torch.bfloat16: BF16X_DTYPE_BF16, torch.float32: BF16X_DTYPE_F32}
+
+
+@dataclass
+class SamplingParams:
+    """The settings of ``sample``, each a number or a tensor of one value per row."""
+    temperature: float | torch.Tensor = 1.0
+    top_k: int | torch.Tensor = 0
+    top_p: float | torch.Tensor = 1.0
+    min_p: float | torch.Tensor = 0.0
 
 
 def _setting(x, name: str, dtype: torch.dtype, logits: torch.Tensor):
@@ -69,4 +80,4 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     return out
 
 
-__all__ = ["sample"]
+__all__ = ["sample", "SamplingParams"]

@@ -1,0 +1,100 @@
+"""The decoder with the 4-bit cache and sampling: logits against the same model
+with torch's attention over the quantised values, prompts of different lengths
+against each alone, captured decode against eager decode, fixed random numbers."""
+import pytest
+import torch
+import torch.nn.functional as F
+
+from bfloat16x_b200 import _lib, llama_e2e
+from bfloat16x_b200.kv4 import Kv4Cache
+from bfloat16x_b200.llama_e2e import CONFIGS, LlamaModel, SamplingParams, generate, pack_model
+from tests.gpu_util import rel_l2
+
+pytestmark = pytest.mark.gpu
+TOL = 2e-2           # the decoder tests' tolerance: bf16 activations on both sides
+
+
+def _prompt(B, P, vocab, seed=1):
+    return torch.randint(0, vocab, (B, P), generator=torch.Generator().manual_seed(seed)).cuda()
+
+
+class _Quantised(Kv4Cache):
+    """The same cache, attended to by torch over the values read back."""
+    __slots__ = ()
+
+    def attend(self, q, pos0, scale=None, out=None):
+        B, T, H, D = q.shape
+        k, v = self.read(torch.zeros((), dtype=torch.long, device=q.device), self.max_seq)
+        pos = pos0.reshape(-1, 1) + torch.arange(T, device=q.device)
+        mask = (torch.arange(self.max_seq, device=q.device) <= pos.expand(B, T)[..., None])[:, None]
+        return F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), attn_mask=mask,
+                                              enable_gqa=True).transpose(1, 2)
+
+
+def test_model_with_4bit_cache_matches_torch_attention():
+    cfg = CONFIGS["tiny"]
+    prompt = _prompt(2, 40, cfg.vocab)
+    model = LlamaModel(cfg, 64, "cuda", seed=3, batch=2, kv_bits=4)
+    pack_model(model)
+    zero = torch.zeros((), dtype=torch.long, device="cuda")
+    step = torch.tensor(40, device="cuda")
+    tok = _prompt(2, 1, cfg.vocab, 9)
+    got = [model(prompt, zero), model(tok, step)]
+    model.cache_kv4 = [_Quantised(torch.zeros_like(c.blocks), 64) for c in model.cache_kv4]
+    ref = [model(prompt, zero), model(tok, step)]
+    for a, b in zip(got, ref):
+        assert rel_l2(a.cpu().numpy(), b.cpu().numpy()) < TOL
+    _lib.check_device_status()
+
+
+def test_prompts_of_different_lengths():
+    cfg = CONFIGS["tiny"]
+    lengths = [5, 33, 20]
+    P = max(lengths)
+    model = LlamaModel(cfg, 48, "cuda", seed=4, batch=3, kv_bits=4)
+    pack_model(model)
+    prompt = _prompt(3, P, cfg.vocab, 2)
+    pos0 = torch.tensor([n - P for n in lengths], device="cuda")
+    first = model(prompt, pos0)
+    nxt = model(prompt[:, :1], torch.tensor(lengths, device="cuda"))
+    one = LlamaModel(cfg, 48, "cuda", seed=4, batch=1, kv_bits=4)
+    pack_model(one)
+    for i, n in enumerate(lengths):
+        a = one(prompt[i:i + 1, P - n:], torch.zeros((), dtype=torch.long, device="cuda"))
+        b = one(prompt[i:i + 1, :1], torch.tensor(n, device="cuda"))
+        assert rel_l2(first[i].cpu().numpy(), a[0].cpu().numpy()) < TOL
+        assert rel_l2(nxt[i].cpu().numpy(), b[0].cpu().numpy()) < TOL
+    _lib.check_device_status()
+
+
+@pytest.mark.parametrize("sampling", [None, SamplingParams(temperature=0.8, top_k=20, top_p=0.9, min_p=0.01)])
+def test_graph_decode_matches_eager(sampling):
+    cfg = CONFIGS["tiny"]
+    lengths = [30, 12]
+    prompt = _prompt(2, 30, cfg.vocab, 5)
+    toks = []
+    for use_graph in (True, False):
+        model = LlamaModel(cfg, 64, "cuda", seed=6, batch=2, kv_bits=4)
+        pack_model(model)
+        gen = torch.Generator(device="cuda").manual_seed(77)
+        toks.append(generate(model, prompt, 12, use_graph, sampling, gen, lengths)[0])
+    assert torch.equal(*toks)
+    _lib.check_device_status()
+
+
+def test_sampling_with_the_bf16_cache_and_refusals():
+    cfg = CONFIGS["tiny"]
+    model = LlamaModel(cfg, 64, "cuda", seed=6)
+    prompt = _prompt(1, 20, cfg.vocab, 5)
+    greedy = generate(model, prompt, 8)[0]
+    cold = generate(model, prompt, 8, sampling=SamplingParams(temperature=0.0))[0]
+    assert torch.equal(greedy, cold)
+    gens = [torch.Generator(device="cuda").manual_seed(s) for s in (1, 1, 2)]
+    hot = [generate(model, prompt, 16, sampling=SamplingParams(temperature=3.0), generator=g)[0] for g in gens]
+    assert torch.equal(hot[0], hot[1]) and not torch.equal(hot[0], hot[2])
+    with pytest.raises(ValueError, match="4-bit"):
+        generate(model, prompt, 1, lengths=[20])
+    with pytest.raises(ValueError, match="4-bit"):
+        model(prompt, torch.zeros(1, dtype=torch.long, device="cuda"))
+    with pytest.raises(ValueError, match="kv_bits"):
+        llama_e2e.LlamaModel(cfg, 64, "cuda", kv_bits=8)
