@@ -1,6 +1,7 @@
 // bf16x_kv4.cu -- writing the 4-bit key/value cache, reading it back, and
 // attention of few query rows over it (decode steps, a few guessed tokens).
 #include <algorithm>
+#include <atomic>
 
 #include <cuda_runtime.h>
 
@@ -15,6 +16,8 @@ namespace bf16x {
 // d is rounded up so that no code exceeds 15, and m is a bf16 value already.
 // A group that holds an infinity or a NaN gets d = NaN, m = 0: it reads as NaN
 // and m stays finite, so a masked position cannot reach another row's sums.
+// A group of one value has codes 0, so its d is free: 2^-13 |m|, which gives
+// the attention the group's magnitude.
 // Every operation is rounded by itself (no fused multiply-add), so the codes
 // do not depend on how the compiler contracts.
 //
@@ -40,7 +43,9 @@ __device__ __forceinline__ void kv4_quantize8(const float (&y)[8], float &d, flo
     if (!(fabsf(span) < __int_as_float(0x7f800000))) {            // infinity or NaN in the group
         d = __int_as_float(0x7fc00000);
         m = 0.f;
-    } else if (d > 0.f) {
+    } else if (d == 0.f) {                                        // a constant group: m, with any d; one near m's
+        d = __uint_as_float(__float_as_uint(fabsf(lo) * 0x1p-13f) & 0xFFFF0000u);      // own scale suits the reader
+    } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float c = rintf(__fdiv_rn(__fsub_rn(y[i], lo), d));
@@ -201,10 +206,12 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
 // Rows r = t * G + h of one kv head's G query heads and T tokens, 8 per mma
 // column tile.  Per block of 16 positions a warp computes
 //   S^T [16 positions][8 rows] = K Q^T,  P = 2^(S' - M),  O^T [D][8 rows] += V^T P^T
-// with the codes as fp16 operands: per 32-channel group j
+// with the codes as operands: per 32-channel group j
 //   S  += dK_j (codes Q_j) + mK_j sum(Q_j),   O_j += codes (P dV_j),  O_j += mV_j P.
-// The minima go through one more mma each (bf16, exact on the m side, the
-// other side split into two or three bf16 parts).
+// Q, each row scaled by a power of two, is exact in fp16; P dV is rounded to
+// fp16.  The minima go through one more mma each (bf16, exact on the m side, the
+// other side split into three or two bf16 parts).  (fp8 operands for the K codes
+// would halve their mma's, but sm_100a's mma.sync widens e4m3 to fp16 first.)
 // P dV has to fit fp16 whatever the scale of V, so the running reference M of
 // a row is the maximum of S' + log2(max_j dV_j), not of S' alone; it is
 // raised only when a term exceeds it by more than 2^8.
@@ -212,14 +219,15 @@ struct Kv4AttendParams {
     const uint16_t *q;
     int64_t ldq_b, ldq_t, ldq_h;
     int B, T, H, KV, G, R;
-    int pos_stride, nsplit;
+    int pos_stride, tiles, warps;       // row tiles per head; warps of the grid
     const int64_t *pos0;
     float scale_log2;                   // softmax scale * log2(e)
     const uint8_t *blocks;
     int64_t max_seq, nblk;
     uint16_t *out;
-    float *part_o;                      // [item][row][split][D]
-    float2 *part_ml;                    // [item][row][split]
+    float *part_o;                      // [share][2][row of the tile][D]
+    float2 *part_ml;                    // [share][2][row of the tile]
+    int2 *held;                         // [unit]: the first and last share that hold blocks of it
 };
 
 constexpr float kRescale = 8.f;         // log2 of how far a term may exceed the reference
@@ -228,66 +236,62 @@ constexpr float kNoMax = -3.0e38f;
 template <int D, int NT>
 struct Kv4Rows {
     static constexpr int NG = D / 32;
-    uint32_t qb[NT][NG][4];             // B fragments: pairs (0,4) (1,5)/16 (2,6) (3,7)/16 of each 8 channels
+    uint32_t q;                         // shared address of this lane's B fragments [NT][NG][32 lanes] x 16 bytes:
+                                        // pairs (0,4) (1,5)/16 (2,6) (3,7)/16 of each 8 channels
     uint32_t qm[NT][2];                 // B fragment of the minima's mma: sums of Q per group, split in bf16 parts
     float c1[NT][2];                    // turns the sums of columns 2t, 2t+1 into log2 units
-    int64_t last[NT][2];                // last position that columns 2t, 2t+1 see, -1: none
+    int last[NT][2];                    // last position that columns 2t, 2t+1 see, from the origin of the walk
 };
 
-// This lane's row of the tile (row g of each column tile): its pointer, or null.
+// The rows of a tile: lane (g, t) takes channels 8 t .. 8 t + 7 of every group of row g.
 template <int D, int NT>
 __device__ __forceinline__ void kv4_load_rows(const Kv4AttendParams &p, int64_t b, int kvh, int row0, int64_t pos0,
-                                              Kv4Rows<D, NT> &rows) {
+                                              int64_t origin, uint4 (*frag)[D / 32][32], Kv4Rows<D, NT> &rows) {
     constexpr int NG = D / 32;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    rows.q = smem_u32(&frag[0][0][lane]);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const int r = row0 + 8 * nt + g;
         const bool have = r < p.R;
         const int tok = have ? r / p.G : 0, hh = have ? r - tok * p.G : 0;
         const uint16_t *src = p.q + b * p.ldq_b + (int64_t)tok * p.ldq_t + (int64_t)(kvh * p.G + hh) * p.ldq_h;
-        float x[NG][8];
+        uint4 raw[NG];
+#pragma unroll
+        for (int j = 0; j < NG; ++j)
+            raw[j] = have ? *reinterpret_cast<const uint4 *>(src + 32 * j + 8 * t) : make_uint4(0, 0, 0, 0);
         float top = 0.f;
 #pragma unroll
         for (int j = 0; j < NG; ++j) {
-            uint4 raw = make_uint4(0, 0, 0, 0);
-            if (have) raw = *reinterpret_cast<const uint4 *>(src + 32 * j + 8 * t);
-            const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+            const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                x[j][2 * i] = bf_lo(w[i]);
-                x[j][2 * i + 1] = bf_hi(w[i]);
-                top = fmaxf(top, fmaxf(fabsf(x[j][2 * i]), fabsf(x[j][2 * i + 1])));
-            }
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(fabsf(bf_lo(w[i])), fabsf(bf_hi(w[i]))));
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         // the row scaled by 2^e to a largest value in [2^13, 2^14): bf16 values are then exact in fp16
         const int ex = (int)(__float_as_uint(top) >> 23) - 127;
-        const int e = top > 0.f && ex < 128 ? min(max(13 - ex, -110), 110) : 0;
+        const int e = top > 0.f && ex < 128 ? min(max(13 - ex, -100), 110) : 0;
         const float up = __uint_as_float((uint32_t)(127 + e) << 23);
-        float sum[NG];
-#pragma unroll
-        for (int j = 0; j < NG; ++j) {
-            float s = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[j][i] *= up;
-                s += x[j][i];
-            }
-            s += __shfl_xor_sync(0xffffffffu, s, 1);
-            s += __shfl_xor_sync(0xffffffffu, s, 2);
-            sum[j] = s * 0x1p-24f;                                  // in the units of the codes' sums
-            rows.qb[nt][j][0] = pack_f16x2(x[j][0], x[j][4]);
-            rows.qb[nt][j][1] = pack_f16x2(x[j][1] * 0.0625f, x[j][5] * 0.0625f);
-            rows.qb[nt][j][2] = pack_f16x2(x[j][2], x[j][6]);
-            rows.qb[nt][j][3] = pack_f16x2(x[j][3] * 0.0625f, x[j][7] * 0.0625f);
-        }
-        // the group sums in three bf16 parts (24 bits): k index 4 part + j (NG = 4) or 2 part + j (NG = 2)
         float part[3][NG];
 #pragma unroll
         for (int j = 0; j < NG; ++j) {
-            float rest = sum[j];
+            const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+            float x[8], s = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[2 * i] = bf_lo(w[i]) * up;
+                x[2 * i + 1] = bf_hi(w[i]) * up;
+                s += x[2 * i] + x[2 * i + 1];
+            }
+            s += __shfl_xor_sync(0xffffffffu, s, 1);
+            s += __shfl_xor_sync(0xffffffffu, s, 2);
+            frag[nt][j][lane] =
+                make_uint4(pack_f16x2(x[0], x[4]), pack_f16x2(x[1] * 0.0625f, x[5] * 0.0625f), pack_f16x2(x[2], x[6]),
+                           pack_f16x2(x[3] * 0.0625f, x[7] * 0.0625f));
+            // the group sums, in the units of the codes' sums, in three bf16 parts (24 bits):
+            // k index 4 part + j (NG = 4) or 2 part + j (NG = 2)
+            float rest = s * 0x1p-24f;
 #pragma unroll
             for (int i = 0; i < 3; ++i) {
                 part[i][j] = bf_lo(pack_bf16x2(rest, 0.f) & 0xFFFFu);
@@ -307,14 +311,16 @@ __device__ __forceinline__ void kv4_load_rows(const Kv4AttendParams &p, int64_t 
             rows.qm[nt][1] = 0u;
         }
         const float c1 = p.scale_log2 * __uint_as_float((uint32_t)(127 + 24 - e) << 23);
-        int64_t last = have ? pos0 + tok : -1;
-        if (last >= p.max_seq) last = -1;
+        // negative: sees nothing (padding, past the cache, no row)
+        const int64_t at = have ? pos0 + tok : -1;
+        const int last = at < 0 || at >= p.max_seq ? -0x40000000 : (int)max(at - origin, (int64_t)-0x40000000);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             rows.c1[nt][i] = __shfl_sync(0xffffffffu, c1, 4 * (2 * t + i));
             rows.last[nt][i] = __shfl_sync(0xffffffffu, last, 4 * (2 * t + i));
         }
     }
+    __syncwarp();
 }
 
 template <int D, int NT>
@@ -340,119 +346,144 @@ __device__ __forceinline__ void kv4_acc_init(Kv4Acc<D, NT> &a) {
 }
 
 template <int NG>
-__device__ __forceinline__ void kv4_expand(const uint8_t *at, float (&d)[NG]) {     // NG bf16 values
+__device__ __forceinline__ void kv4_expand(uint32_t at, float (&d)[NG]) {           // NG bf16 values
     if constexpr (NG == 4) {
-        const uint2 w = *reinterpret_cast<const uint2 *>(at);
+        const uint2 w = lds64(at);
         d[0] = bf_lo(w.x);
         d[1] = bf_hi(w.x);
         d[2] = bf_lo(w.y);
         d[3] = bf_hi(w.y);
     } else {
-        const uint32_t w = *reinterpret_cast<const uint32_t *>(at);
+        const uint32_t w = lds32(at);
         d[0] = bf_lo(w);
         d[1] = bf_hi(w);
     }
 }
 
 template <int NG>
-__device__ __forceinline__ void kv4_words(const uint8_t *at, uint32_t (&w)[NG]) {   // NG words of codes
+__device__ __forceinline__ void kv4_words(uint32_t at, uint32_t (&w)[NG]) {         // NG words of codes
     if constexpr (NG == 4) {
-        const uint4 v = *reinterpret_cast<const uint4 *>(at);
+        const uint4 v = lds128(at);
         w[0] = v.x;
         w[1] = v.y;
         w[2] = v.z;
         w[3] = v.w;
     } else {
-        const uint2 v = *reinterpret_cast<const uint2 *>(at);
+        const uint2 v = lds64(at);
         w[0] = v.x;
         w[1] = v.y;
     }
 }
 
 // log2 of a position's largest V scale for the reference: not below -100, so
-// that P <= 2^108 and its sums stay finite; a position whose groups are all
-// constant has no code part, and -20 keeps m P finite too (where d is not 0, m
-// is at most 2^12 d: the values are bf16).
-__device__ __forceinline__ float kv4_ref_exp(float d) { return d > 0.f ? fmaxf(lg2(d), -100.f) : -20.f; }
+// that P <= 2^108 and its sums stay finite.
+__device__ __forceinline__ float kv4_ref_exp(float d) { return fmaxf(lg2(d), -100.f); }
 
-// One block at `blk`, whose first position is key0.  MASK: some row of the
-// tile does not see all of it; positions from n_keys on are not read as numbers.
-template <int D, int NT, bool MASK>
-__device__ __forceinline__ void kv4_block(const uint8_t *blk, int64_t key0, int64_t n_keys, const Kv4Rows<D, NT> &rows,
-                                          Kv4Acc<D, NT> &acc) {
+// Where this lane's parts of a block lie.
+template <int D>
+struct Kv4Lane {
+    uint32_t codes, row, kmin, vmin;    // byte offsets
+    int g, t;
+    __device__ __forceinline__ Kv4Lane() {
+        constexpr int NG = D / 32;
+        const int lane = threadIdx.x & 31;
+        g = lane >> 2, t = lane & 3;
+        codes = lane * NG * 4;
+        row = 16 * D + g * NG * 2;
+        kmin = 17 * D + g * NG * 2 + (NG == 4 ? (t & 1) * 4 : 0);
+        vmin = 19 * D + (t * NG + min(g, NG - 1)) * 4;
+        // kept in registers, not worked out again for every block
+        asm volatile("" : "+r"(codes), "+r"(row), "+r"(kmin), "+r"(vmin));
+    }
+};
+
+// NB consecutive blocks at shared address `blk`, the first position of the
+// first at key0 (relative to the tile's first row, like rows.last).  MASK: some
+// row of the tile does not see all of them; positions from n_keys on are not
+// read as numbers.
+template <int D, int NT, int NB, bool MASK>
+__device__ __forceinline__ void kv4_block(uint32_t blk, int key0, int n_keys, const Kv4Lane<D> &ln,
+                                          const Kv4Rows<D, NT> &rows, Kv4Acc<D, NT> &acc) {
     using L = KvLayout<D>;
     constexpr int NG = L::NG;
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const bool ok0 = !MASK || key0 + g < n_keys, ok1 = !MASK || key0 + g + 8 < n_keys;
+    constexpr float kInf = __builtin_huge_valf();
+    const int g = ln.g, t = ln.t;
+    float s[NB][NT][4];
+    bool ok[NB][2];
     // ---- scores
-    uint32_t k0[NG], k1[NG];
-    float d0[NG], d1[NG];
-    kv4_words<NG>(blk + (g * 4 + t) * NG * 4, k0);
-    kv4_words<NG>(blk + ((g + 8) * 4 + t) * NG * 4, k1);
-    kv4_expand<NG>(blk + L::kKd + g * NG * 2, d0);
-    kv4_expand<NG>(blk + L::kKd + (g + 8) * NG * 2, d1);
-    const int tm = NG == 4 ? (t & 1) * 4 : 0;
-    uint32_t m0 = *reinterpret_cast<const uint32_t *>(blk + L::kKm + g * NG * 2 + tm);
-    uint32_t m1 = *reinterpret_cast<const uint32_t *>(blk + L::kKm + (g + 8) * NG * 2 + tm);
-    if (MASK) {
-        m0 = ok0 ? m0 : 0u;
-        m1 = ok1 ? m1 : 0u;
-    }
-    float s[NT][4];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
-        mma_bf16(s[nt], m0, m1, m0, m1, rows.qm[nt][0], rows.qm[nt][1]);
-    }
+    for (int n = 0; n < NB; ++n) {
+        const uint32_t at = blk + n * L::kBytes;
+        ok[n][0] = !MASK || key0 + 16 * n + g < n_keys;
+        ok[n][1] = !MASK || key0 + 16 * n + g + 8 < n_keys;
+        uint32_t k0[NG], k1[NG];
+        float d0[NG], d1[NG];
+        kv4_words<NG>(at + ln.codes, k0);
+        kv4_words<NG>(at + ln.codes + 32 * NG * 4, k1);
+        kv4_expand<NG>(at + ln.row, d0);
+        kv4_expand<NG>(at + ln.row + 8 * NG * 2, d1);
+        uint32_t m0 = lds32(at + ln.kmin), m1 = lds32(at + ln.kmin + 8 * NG * 2);
+        if (MASK) {
+            m0 = ok[n][0] ? m0 : 0u;
+            m1 = ok[n][1] ? m1 : 0u;
+        }
 #pragma unroll
-    for (int j = 0; j < NG; ++j) {
-        const uint32_t h0 = k0[j] >> 8, h1 = k1[j] >> 8;
+        for (int nt = 0; nt < NT; ++nt)
+            mma_bf16(s[n][nt], m0, m1, m0, m1, rows.qm[nt][0], rows.qm[nt][1], 0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            float c[4] = {0.f, 0.f, 0.f, 0.f};
-            mma_f16(c, k0[j] & 0x000F000Fu, k1[j] & 0x000F000Fu, k0[j] & 0x00F000F0u, k1[j] & 0x00F000F0u,
-                    rows.qb[nt][j][0], rows.qb[nt][j][1]);
-            mma_f16(c, h0 & 0x000F000Fu, h1 & 0x000F000Fu, h0 & 0x00F000F0u, h1 & 0x00F000F0u, rows.qb[nt][j][2],
-                    rows.qb[nt][j][3]);
-            s[nt][0] = fmaf(d0[j], c[0], s[nt][0]);
-            s[nt][1] = fmaf(d0[j], c[1], s[nt][1]);
-            s[nt][2] = fmaf(d1[j], c[2], s[nt][2]);
-            s[nt][3] = fmaf(d1[j], c[3], s[nt][3]);
+        for (int j = 0; j < NG; ++j) {
+            const uint32_t h0 = k0[j] >> 8, h1 = k1[j] >> 8;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float c[4];
+                const uint4 q = lds128(rows.q + (nt * NG + j) * 512);
+                mma_f16(c, k0[j] & 0x000F000Fu, k1[j] & 0x000F000Fu, k0[j] & 0x00F000F0u, k1[j] & 0x00F000F0u, q.x,
+                        q.y, 0.f, 0.f, 0.f, 0.f);
+                mma_f16(c, h0 & 0x000F000Fu, h1 & 0x000F000Fu, h0 & 0x00F000F0u, h1 & 0x00F000F0u, q.z, q.w);
+                s[n][nt][0] = fmaf(d0[j], c[0], s[n][nt][0]);
+                s[n][nt][1] = fmaf(d0[j], c[1], s[n][nt][1]);
+                s[n][nt][2] = fmaf(d1[j], c[2], s[n][nt][2]);
+                s[n][nt][3] = fmaf(d1[j], c[3], s[n][nt][3]);
+            }
         }
     }
     // ---- V's scales, and the reference of each row
-    float v0[NG], v1[NG];
-    kv4_expand<NG>(blk + L::kVd + g * NG * 2, v0);
-    kv4_expand<NG>(blk + L::kVd + (g + 8) * NG * 2, v1);
-    if (MASK) {
+    float v[NB][2][NG], e[NB][2];
 #pragma unroll
-        for (int j = 0; j < NG; ++j) {
-            v0[j] = ok0 ? v0[j] : 0.f;
-            v1[j] = ok1 ? v1[j] : 0.f;
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            kv4_expand<NG>(blk + n * L::kBytes + ln.row + 2 * D + i * 8 * NG * 2, v[n][i]);
+            if (MASK) {
+#pragma unroll
+                for (int j = 0; j < NG; ++j) v[n][i][j] = ok[n][i] ? v[n][i][j] : 0.f;
+            }
+            e[n][i] = fmaxf(v[n][i][0], v[n][i][1]);
+            if constexpr (NG == 4) e[n][i] = fmaxf(e[n][i], fmaxf(v[n][i][2], v[n][i][3]));
+            e[n][i] = kv4_ref_exp(e[n][i]);
         }
-    }
-    float e0 = fmaxf(v0[0], v0[1]), e1 = fmaxf(v1[0], v1[1]);
-    if constexpr (NG == 4) {
-        e0 = fmaxf(e0, fmaxf(v0[2], v0[3]));
-        e1 = fmaxf(e1, fmaxf(v1[2], v1[3]));
-    }
-    e0 = kv4_ref_exp(e0);
-    e1 = kv4_ref_exp(e1);
     bool raise = false;
-    float top[NT][2];
+    float top[NT][2], unit[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+        if (MASK) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            s[nt][i] *= rows.c1[nt][i & 1];
-            if (MASK) {
-                const int64_t key = key0 + g + (i & 2 ? 8 : 0);
-                if (key > rows.last[nt][i & 1]) s[nt][i] = -__int_as_float(0x7f800000);
-            }
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[n][nt][i] *= rows.c1[nt][i & 1];
+                    if (key0 + 16 * n + g + (i & 2 ? 8 : 0) > rows.last[nt][i & 1]) s[n][nt][i] = -kInf;
+                }
         }
-        top[nt][0] = fmaxf(s[nt][0] + e0, s[nt][2] + e1);
-        top[nt][1] = fmaxf(s[nt][1] + e0, s[nt][3] + e1);
-        raise |= top[nt][0] > acc.M[nt][0] + kRescale || top[nt][1] > acc.M[nt][1] + kRescale;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            unit[nt][i] = MASK ? 1.f : rows.c1[nt][i];
+            top[nt][i] = fmaxf(fmaf(s[0][nt][i], unit[nt][i], e[0][0]), fmaf(s[0][nt][2 + i], unit[nt][i], e[0][1]));
+            if constexpr (NB == 2)
+                top[nt][i] = fmaxf(top[nt][i], fmaxf(fmaf(s[NB - 1][nt][i], unit[nt][i], e[NB - 1][0]),
+                                                     fmaf(s[NB - 1][nt][2 + i], unit[nt][i], e[NB - 1][1])));
+            raise |= top[nt][i] > acc.M[nt][i] + kRescale;
+        }
     }
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
@@ -477,197 +508,421 @@ __device__ __forceinline__ void kv4_block(const uint8_t *blk, int64_t key0, int6
         }
     }
     // ---- P, and O
-    uint32_t w0[NG], w1[NG];
-    kv4_words<NG>(blk + L::kV + (g * 4 + t) * NG * 4, w0);
-    kv4_words<NG>(blk + L::kV + ((8 + g) * 4 + t) * NG * 4, w1);
-    uint32_t vm0 = 0, vm1 = 0;
-    if (g < NG) {
-        vm0 = *reinterpret_cast<const uint32_t *>(blk + L::kVm + (t * NG + g) * 4);
-        vm1 = *reinterpret_cast<const uint32_t *>(blk + L::kVm + ((4 + t) * NG + g) * 4);
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+        const uint32_t at = blk + n * L::kBytes;
+        uint32_t w0[NG], w1[NG];
+        kv4_words<NG>(at + ln.codes + L::kV, w0);
+        kv4_words<NG>(at + ln.codes + L::kV + 32 * NG * 4, w1);
+        // rows g >= NG of this mma are not used: they may hold any finite numbers (the last group's minima)
+        uint32_t vm0 = lds32(at + ln.vmin), vm1 = lds32(at + ln.vmin + 16 * NG);
         if (MASK) {
-            const int64_t a = key0 + 2 * t, c = a + 8;
+            const int a = key0 + 16 * n + 2 * t, c = a + 8;
             vm0 = a + 1 < n_keys ? vm0 : a < n_keys ? vm0 & 0xFFFFu : 0u;
             vm1 = c + 1 < n_keys ? vm1 : c < n_keys ? vm1 & 0xFFFFu : 0u;
         }
-    }
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        float pr[4];
+        for (int nt = 0; nt < NT; ++nt) {
+            float pr[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pr[i] = ex2(s[nt][i] - acc.M[nt][i & 1]);
-        acc.l[nt][0] += pr[0] + pr[2];
-        acc.l[nt][1] += pr[1] + pr[3];
-        {
+            for (int i = 0; i < 4; ++i) pr[i] = ex2(fmaf(s[n][nt][i], unit[nt][i & 1], -acc.M[nt][i & 1]));
+            acc.l[nt][0] += pr[0] + pr[2];
+            acc.l[nt][1] += pr[1] + pr[3];
             const uint32_t a = pack_bf16x2(pr[0], pr[1]), c = pack_bf16x2(pr[2], pr[3]);
-            mma_bf16(acc.mt[nt], vm0, 0u, vm1, 0u, movmatrix(a), movmatrix(c));
             const uint32_t al = pack_bf16x2(pr[0] - bf_lo(a), pr[1] - bf_hi(a)),
                            cl = pack_bf16x2(pr[2] - bf_lo(c), pr[3] - bf_hi(c));
-            mma_bf16(acc.mt[nt], vm0, 0u, vm1, 0u, movmatrix(al), movmatrix(cl));
-        }
+            mma_bf16(acc.mt[nt], vm0, vm0, vm1, vm1, movmatrix(a), movmatrix(c));
+            mma_bf16(acc.mt[nt], vm0, vm0, vm1, vm1, movmatrix(al), movmatrix(cl));
 #pragma unroll
-        for (int j = 0; j < NG; ++j) {
-            float x[4] = {pr[0] * v0[j], pr[1] * v0[j], pr[2] * v1[j], pr[3] * v1[j]};
-            if (MASK) {                                             // 0 * NaN: a masked position stays out of its row
+            for (int j = 0; j < NG; ++j) {
+                float x[4] = {pr[0] * v[n][0][j], pr[1] * v[n][0][j], pr[2] * v[n][1][j], pr[3] * v[n][1][j]};
+                if (MASK) {                                         // 0 * NaN: a masked position stays out of its row
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = s[nt][i] == -__int_as_float(0x7f800000) ? 0.f : x[i];
+                    for (int i = 0; i < 4; ++i) x[i] = s[n][nt][i] == -kInf ? 0.f : x[i];
+                }
+                const uint32_t b0 = movmatrix(pack_f16x2(x[0], x[1])), b1 = movmatrix(pack_f16x2(x[2], x[3]));
+                const uint32_t h0 = w0[j] >> 8, h1 = w1[j] >> 8;
+                mma_f16(acc.o[nt][2 * j], w0[j] & 0x000F000Fu, w0[j] & 0x00F000F0u, w1[j] & 0x000F000Fu,
+                        w1[j] & 0x00F000F0u, b0, b1);
+                mma_f16(acc.o[nt][2 * j + 1], h0 & 0x000F000Fu, h0 & 0x00F000F0u, h1 & 0x000F000Fu, h1 & 0x00F000F0u,
+                        b0, b1);
             }
-            const uint32_t b0 = movmatrix(pack_f16x2(x[0], x[1])), b1 = movmatrix(pack_f16x2(x[2], x[3]));
-            const uint32_t h0 = w0[j] >> 8, h1 = w1[j] >> 8;
-            mma_f16(acc.o[nt][2 * j], w0[j] & 0x000F000Fu, w0[j] & 0x00F000F0u, w1[j] & 0x000F000Fu,
-                    w1[j] & 0x00F000F0u, b0, b1);
-            mma_f16(acc.o[nt][2 * j + 1], h0 & 0x000F000Fu, h0 & 0x00F000F0u, h1 & 0x000F000Fu, h1 & 0x00F000F0u, b0,
-                    b1);
         }
     }
 }
 
-constexpr int kAttendWarps = 8;
+// The schedule.  A unit is one row tile of one (sequence, kv head); its work is
+// the blocks that its sequence holds, plus kUnitCost blocks for starting and
+// ending a unit.  The units' work, one after the other, is cut into equal
+// shares, one for each warp of the grid: sequences of any lengths load the GPU
+// evenly, no warp waits for another, and lengths are read on the device, so a
+// captured call follows them.  A warp writes a unit that it has alone; of
+// others it writes its part, at most one that began before its share (slot 0)
+// and one that goes on after it (slot 1), and a second kernel joins the parts.
+template <int D, int NT>
+struct AttendCfg {
+    static constexpr int kWarps = NT == 1 ? 12 : 8;                 // per CTA and SM: what the registers allow
+    static constexpr int kNB = NT == 1 ? 2 : 1;                     // blocks per stage
+    static constexpr int kDepth = NT == 1 ? 3 : 5;                  // stages in flight per warp
+};
+constexpr int kUnitCost = 4;
+constexpr int kMinShare = 4;
 
 template <int D, int NT>
 struct AttendSmem {
-    float o[kAttendWarps][8 * NT][D + 4];
-    float M[kAttendWarps][8 * NT], l[kAttendWarps][8 * NT];
+    static constexpr int W = AttendCfg<D, NT>::kWarps;
+    uint8_t ring[W][AttendCfg<D, NT>::kDepth][AttendCfg<D, NT>::kNB * KvLayout<D>::kBytes];
+    uint4 frag[W][NT][D / 32][32];
+    uint64_t full[W][AttendCfg<D, NT>::kDepth];
+};
+
+__device__ __forceinline__ int64_t kv4_blocks_of(const Kv4AttendParams &p, int64_t pos0) {
+    const int64_t n = min(pos0 + p.T, p.max_seq);
+    return n > 0 ? (n + kKvBlock - 1) / kKvBlock : 0;
+}
+
+// a / b and its remainder, in 32 bits where that is enough (64-bit division takes some hundred instructions)
+__device__ __forceinline__ int64_t quot(int64_t a, int64_t b) {
+    return ((uint64_t)a | (uint64_t)b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
+
+struct Kv4Plan {                        // how the work is cut
+    int64_t total, shares, q, r;        // the first r shares have q + 1, the others q
+    __device__ __forceinline__ Kv4Plan(int64_t total_, int64_t warps) : total(total_) {
+        shares = max((int64_t)1, min(warps, quot(total, kMinShare)));
+        q = quot(total, shares);
+        r = total - q * shares;
+    }
+    __device__ __forceinline__ int64_t start(int64_t c) const { return q * c + min(c, r); }
+    __device__ __forceinline__ int64_t share_of(int64_t at) const {
+        const int64_t big = (q + 1) * r;
+        return at < big ? quot(at, q + 1) : r + quot(at - big, q);
+    }
+};
+
+// Work of all sequences, and of those before sequence `b` (one warp).
+__device__ __forceinline__ int64_t kv4_work(const Kv4AttendParams &p, int64_t per_seq, int64_t b, int64_t &before) {
+    int64_t x = 0, y = 0;
+    for (int64_t i = threadIdx.x & 31; i < p.B; i += 32) {
+        const int64_t k = kv4_blocks_of(p, p.pos0[i * p.pos_stride]);
+        const int64_t w = k ? k + kUnitCost : 0;
+        y += w;
+        if (i < b) x += w;
+    }
+    for (int o = 16; o; o >>= 1) {
+        x += __shfl_xor_sync(0xffffffffu, x, o);
+        y += __shfl_xor_sync(0xffffffffu, y, o);
+    }
+    before = x * per_seq;
+    return y * per_seq;
+}
+
+// Walks a share, unit by unit.
+struct Kv4Walk {
+    int64_t b, pos0, nb;                // the unit's sequence and its blocks
+    int kvh, tile;
+    int64_t blk, end;                   // blocks of the unit in this share: [blk, end)
+    int64_t left;                       // work of the share after this unit
+
+    // at: where in the unit's work the share begins; work: what the share still has
+    __device__ __forceinline__ void enter(int64_t at, int64_t work) {
+        const int64_t stop = min(at + work, nb + kUnitCost);
+        left = work - (stop - at);
+        blk = max(at - kUnitCost, (int64_t)0);
+        end = max(stop - kUnitCost, (int64_t)0);
+    }
+    __device__ __forceinline__ void next(const Kv4AttendParams &p) {       // left > 0
+        if (++tile == p.tiles) {
+            tile = 0;
+            if (++kvh == p.KV) {
+                kvh = 0;
+                do {
+                    ++b;
+                    pos0 = p.pos0[b * p.pos_stride];
+                    nb = kv4_blocks_of(p, pos0);
+                } while (nb == 0);
+            }
+        }
+        enter(0, left);
+    }
 };
 
 template <int D, int NT>
-__global__ void __launch_bounds__(kAttendWarps * 32) kv4_attend_kernel(const Kv4AttendParams p) {
+__global__ void __launch_bounds__(AttendCfg<D, NT>::kWarps * 32, 1)
+    kv4_attend_kernel(const __grid_constant__ Kv4AttendParams p) {
     using L = KvLayout<D>;
-    constexpr int NG = L::NG, W = kAttendWarps, C = 8 * NT;
-    extern __shared__ __align__(16) uint8_t smem_raw[];
+    using Cfg = AttendCfg<D, NT>;
+    constexpr int NG = L::NG, C = 8 * NT, DEPTH = Cfg::kDepth, NB = Cfg::kNB;
+    extern __shared__ __align__(128) uint8_t smem_raw[];
     AttendSmem<D, NT> &sm = *reinterpret_cast<AttendSmem<D, NT> *>(smem_raw);
-    griddep_launch_dependents();
-    griddep_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int split = blockIdx.x, row0 = blockIdx.y * C;
-    const int64_t item = blockIdx.z;
-    const int64_t b = item / p.KV;
-    const int kvh = (int)(item - b * p.KV);
-    const int64_t pos0 = p.pos0[b * p.pos_stride];
-    // positions that some row of the tile sees: rows are ordered by token
-    const int tok_last = min(row0 + C - 1, p.R - 1) / p.G;
-    int64_t n_keys = pos0 + tok_last + 1;
-    if (n_keys > p.max_seq) {                                       // tokens past the cache's end see nothing
-        if (threadIdx.x == 0) atomicOr(&g_status, kErrBadIndex);
-        n_keys = p.max_seq;
+    griddep_launch_dependents();
+    if (lane == 0)
+        for (int i = 0; i < DEPTH; ++i) mbar_init(&sm.full[warp][i], 1);
+    fence_mbar_init();
+    __syncwarp();
+    griddep_wait();
+    // ---- this warp's share: the CTAs in turn, so that few shares lie on many SMs
+    const int64_t share = (int64_t)warp * gridDim.x + blockIdx.x;
+    const int64_t per_seq = (int64_t)p.KV * p.tiles;
+    Kv4Walk con;
+    int64_t total, skip;
+    if (p.B == 1) {
+        con.b = 0;
+        con.pos0 = p.pos0[0];
+        con.nb = kv4_blocks_of(p, con.pos0);
+        total = con.nb ? (con.nb + kUnitCost) * per_seq : 0;
+    } else {
+        total = kv4_work(p, per_seq, 0, skip);
     }
-    n_keys = max(n_keys, (int64_t)0);
-    const int64_t first_last = pos0 + row0 / p.G;                   // last position that the tile's first row sees
-    const int64_t nb = (n_keys + kKvBlock - 1) / kKvBlock;
-    const int64_t b0 = nb * split / p.nsplit, b1 = nb * (split + 1) / p.nsplit;
-    Kv4Rows<D, NT> rows;
-    kv4_load_rows<D, NT>(p, b, kvh, row0, pos0, rows);
-    Kv4Acc<D, NT> acc;
-    kv4_acc_init(acc);
-    const uint8_t *base = p.blocks + (b * p.KV + kvh) * p.nblk * L::kBytes;
-    for (int64_t i = b0 + warp; i < b1; i += W) {
-        const int64_t key0 = i * kKvBlock;
-        if (key0 + kKvBlock - 1 <= first_last && key0 + kKvBlock <= n_keys)
-            kv4_block<D, NT, false>(base + i * L::kBytes, key0, n_keys, rows, acc);
-        else
-            kv4_block<D, NT, true>(base + i * L::kBytes, key0, n_keys, rows, acc);
+    if (total == 0) return;
+    const Kv4Plan plan(total, p.warps);
+    if (share >= plan.shares) return;
+    int64_t at = plan.start(share);
+    const int64_t next_at = plan.start(share + 1), work = next_at - at;     // in the cut order
+    if (p.B > 1) {
+        // the sequence in which the share begins
+        for (int64_t b0 = 0;; b0 += 32) {                           // ends: the share lies within the total
+            const int64_t b = b0 + lane;
+            const int64_t pos = b < p.B ? p.pos0[b * p.pos_stride] : -(int64_t)p.T;
+            const int64_t nb = kv4_blocks_of(p, pos), mine = nb ? (nb + kUnitCost) * per_seq : 0;
+            int64_t x = mine;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += y;
+            }
+            const uint32_t hit = __ballot_sync(0xffffffffu, at < x);
+            if (hit == 0 && b0 + 32 < p.B) {
+                at -= __shfl_sync(0xffffffffu, x, 31);
+                continue;
+            }
+            const int who = hit ? __ffs(hit) - 1 : 31;
+            con.b = b0 + who;
+            con.pos0 = __shfl_sync(0xffffffffu, pos, who);
+            con.nb = __shfl_sync(0xffffffffu, nb, who);
+            at -= __shfl_sync(0xffffffffu, x - mine, who);
+            break;
+        }
     }
-    // ---- the warps' sums joined: each scaled to the largest reference
+    {
+        const int64_t unit = quot(at, con.nb + kUnitCost);
+        con.kvh = (int)quot(unit, p.tiles);
+        con.tile = (int)(unit - (int64_t)con.kvh * p.tiles);
+        con.enter(at - unit * (con.nb + kUnitCost), work);
+    }
+    // ---- the ring: stages of NB blocks
+    const Kv4Lane<D> ln;
+    const uint32_t ring0 = smem_u32(sm.ring[warp][0]), bar0 = smem_u32(&sm.full[warp][0]);
+    uint32_t slot = 0, parity = 0;      // of the next stage to be read
+    const uint8_t *src = nullptr;       // the next stage to be asked for
+    int asked = 0, stages = 0, last_bytes = 0;
+    const auto issue = [&](uint32_t to) {
+        if (lane == 0) {
+            const uint32_t bytes = asked == stages - 1 ? last_bytes : NB * L::kBytes;
+            asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}"
+                         :: "r"(bar0 + 8 * to), "r"(bytes) : "memory");
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                         :: "r"(ring0 + to * NB * L::kBytes), "l"(src), "r"(bytes), "r"(bar0 + 8 * to) : "memory");
+        }
+        src += NB * L::kBytes;
+        ++asked;
+    };
+    const auto start = [&]() {          // the first stages of the unit's part; every slot is free
+        const int count = (int)(con.end - con.blk);
+        stages = (count + NB - 1) / NB;
+        last_bytes = (count - (stages - 1) * NB) * L::kBytes;
+        src = p.blocks + ((con.b * p.KV + con.kvh) * p.nblk + con.blk) * L::kBytes;
+        asked = 0;
+        uint32_t to = slot;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            float l = acc.l[nt][i];
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-            if (g == 0) {
-                sm.M[warp][8 * nt + 2 * t + i] = acc.M[nt][i];
-                sm.l[warp][8 * nt + 2 * t + i] = l;
+        for (int i = 0; i < DEPTH; ++i) {
+            if (asked < stages) issue(to);
+            if (++to == DEPTH) to = 0;
+        }
+    };
+    start();
+    bool alive = true;
+    for (;;) {
+        // ---- one unit's part; positions from here on relative to its first one
+        const int64_t b = con.b, pos0 = con.pos0, origin = con.blk * kKvBlock;
+        const int kvh = con.kvh, row0 = con.tile * C;
+        const bool began = con.blk == 0, ends = con.end == con.nb, any = con.end > con.blk;
+        if (began && any && lane == 0) {
+            // a unit that goes on after this share: its last block lies nb - end blocks past the share's end
+            p.held[(b * p.KV + kvh) * p.tiles + con.tile] =
+                make_int2((int)share, ends ? (int)share : (int)plan.share_of(next_at + (con.nb - con.end) - 1));
+        }
+        const int64_t lim = min(pos0 + min(row0 + C - 1, p.R - 1) / p.G + 1, p.max_seq);
+        const int part = (int)(con.end - con.blk) * kKvBlock;
+        const int n_keys = (int)max(min(lim - origin, (int64_t)part), (int64_t)0);
+        const int all_see = (int)max(min(pos0 + row0 / p.G + 1 - origin, (int64_t)n_keys), (int64_t)0);
+        Kv4Acc<D, NT> acc;
+        kv4_acc_init(acc);
+        if (any) {
+            Kv4Rows<D, NT> rows;
+            kv4_load_rows<D, NT>(p, b, kvh, row0, pos0, origin, sm.frag[warp], rows);
+            int key0 = 0;
+            for (int i = 0; i < stages; ++i) {
+                if (alive) alive = mbar_wait(&sm.full[warp][slot], parity, &g_status);
+                if (alive) {
+                    const uint32_t blk = ring0 + slot * NB * L::kBytes;
+                    if (key0 + NB * kKvBlock <= all_see) {
+                        kv4_block<D, NT, NB, false>(blk, key0, n_keys, ln, rows, acc);
+                    } else {
+                        for (int n = 0; n < NB; ++n)
+                            if (key0 + n * kKvBlock < n_keys)
+                                kv4_block<D, NT, 1, true>(blk + n * L::kBytes, key0 + n * kKvBlock, n_keys, ln, rows, acc);
+                    }
+                    __syncwarp();
+                    if (asked < stages) issue(slot);
+                }
+                key0 += NB * kKvBlock;
+                if (++slot == DEPTH) slot = 0, parity ^= 1;
             }
         }
-    __syncthreads();
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        float f[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            float top = kNoMax;
-            for (int w = 0; w < W; ++w) top = fmaxf(top, sm.M[w][8 * nt + 2 * t + i]);
-            f[i] = ex2(acc.M[nt][i] - top);
+        const bool more = con.left > 0;
+        if (more) {                     // the next unit's first stages come in while this one's rows are written
+            con.next(p);
+            if (alive) start();
         }
+        if (any) {
 #pragma unroll
-        for (int j = 0; j < NG; ++j) {
-            const float mt0 = __shfl_sync(0xffffffffu, acc.mt[nt][0], 4 * j + t),
-                        mt1 = __shfl_sync(0xffffffffu, acc.mt[nt][1], 4 * j + t);
+            for (int nt = 0; nt < NT; ++nt) {
+                float l[2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const float(&o)[4] = acc.o[nt][2 * j + i];
-                const int ch = 32 * j + 4 * g + 2 * i, c = 8 * nt + 2 * t;
-                *reinterpret_cast<float2 *>(&sm.o[warp][c][ch]) =
-                    make_float2((o[0] * 0x1p24f + mt0) * f[0], (o[2] * 0x1p20f + mt0) * f[0]);
-                *reinterpret_cast<float2 *>(&sm.o[warp][c + 1][ch]) =
-                    make_float2((o[1] * 0x1p24f + mt1) * f[1], (o[3] * 0x1p20f + mt1) * f[1]);
+                for (int i = 0; i < 2; ++i) {
+                    l[i] = acc.l[nt][i];
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o);
+                }
+                float mt[2][NG];
+#pragma unroll
+                for (int j = 0; j < NG; ++j)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) mt[i][j] = __shfl_sync(0xffffffffu, acc.mt[nt][i], 4 * j + t);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int c = 8 * nt + 2 * t + i, r = row0 + c;
+                    if (r >= p.R) continue;
+                    const bool whole = began && ends;
+                    const float f = !whole ? 1.f : l[i] != 0.f ? 1.f / l[i] : 0.f;
+                    const int tok = r / p.G, hh = r - tok * p.G;
+                    uint16_t *dst = p.out + ((b * p.T + tok) * p.H + kvh * p.G + hh) * D + 4 * g;
+                    const int64_t slot_at = (share * 2 + (began ? 1 : 0)) * C + c;
+#pragma unroll
+                    for (int j = 0; j < NG; ++j) {
+                        // a result that is 0 of nothing seen is 0, not what an empty sum left
+                        const float4 o = make_float4(fmaf(acc.o[nt][2 * j][i], 0x1p24f, mt[i][j]) * f,
+                                                     fmaf(acc.o[nt][2 * j][2 + i], 0x1p20f, mt[i][j]) * f,
+                                                     fmaf(acc.o[nt][2 * j + 1][i], 0x1p24f, mt[i][j]) * f,
+                                                     fmaf(acc.o[nt][2 * j + 1][2 + i], 0x1p20f, mt[i][j]) * f);
+                        if (whole)
+                            *reinterpret_cast<uint2 *>(dst + 32 * j) =
+                                make_uint2(pack_bf16x2(o.x, o.y), pack_bf16x2(o.z, o.w));
+                        else
+                            *reinterpret_cast<float4 *>(p.part_o + slot_at * D + 32 * j + 4 * g) = o;
+                    }
+                    if (!whole && g == 0) p.part_ml[slot_at] = make_float2(acc.M[nt][i], l[i]);
+                }
             }
         }
+        if (!more) break;
+        __syncwarp();
     }
-    __syncthreads();
-    for (int e = threadIdx.x; e < C * (D / 2); e += W * 32) {
-        const int c = e / (D / 2), ch = 2 * (e - c * (D / 2)), r = row0 + c;
-        if (r >= p.R) continue;
-        float top = kNoMax, l = 0.f;
-        for (int w = 0; w < W; ++w) top = fmaxf(top, sm.M[w][c]);
-        float2 o = make_float2(0.f, 0.f);
-        for (int w = 0; w < W; ++w) {
-            l += sm.l[w][c] * ex2(sm.M[w][c] - top);
-            const float2 a = *reinterpret_cast<const float2 *>(&sm.o[w][c][ch]);
-            o.x += a.x;
-            o.y += a.y;
-        }
-        if (p.nsplit == 1) {
-            const float inv = l != 0.f ? 1.f / l : 0.f;
-            const int tok = r / p.G, hh = r - tok * p.G;
-            *reinterpret_cast<uint32_t *>(p.out + ((b * p.T + tok) * p.H + kvh * p.G + hh) * D + ch) =
-                pack_bf16x2(o.x * inv, o.y * inv);
-        } else {
-            const int64_t at = (item * p.R + r) * p.nsplit + split;
-            *reinterpret_cast<float2 *>(p.part_o + at * D + ch) = o;
-            if (ch == 0) p.part_ml[at] = make_float2(top, l);
-        }
-    }
+    if (!alive)                         // a copy that was late: every slot's bounded once more before the memory goes
+        for (int i = 0; i < DEPTH; ++i) mbar_wait(&sm.full[warp][(slot + i) % DEPTH], parity ^ (slot + i >= DEPTH), &g_status);
 }
 
-// One warp per row: the splits' sums joined in order.
-template <int D>
-__global__ void __launch_bounds__(128) kv4_join_kernel(const Kv4AttendParams p) {
-    constexpr int V = D / 32;
+// Units of which several warps had a part, joined in order, and rows of
+// sequences that hold nothing.  WPR warps per row: a row of few units has many
+// parts, rows of many units have few.
+template <int D, int NT, int WPR>
+__global__ void __launch_bounds__(WPR > 8 ? WPR * 32 : 256) kv4_join_kernel(const __grid_constant__ Kv4AttendParams p) {
+    constexpr int V = D / 32, C = 8 * NT, W = WPR > 8 ? WPR : 8;
+    __shared__ float s_acc[WPR > 1 ? W : 1][D];
+    __shared__ float s_l[WPR > 1 ? W : 1];
     griddep_launch_dependents();
     griddep_wait();
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);      // item * R + r
-    const int lane = threadIdx.x & 31;
-    if (row >= (int64_t)p.B * p.KV * p.R) return;
-    const float2 *ml = p.part_ml + row * p.nsplit;
-    float top = kNoMax;
-    for (int s = lane; s < p.nsplit; s += 32) top = fmaxf(top, ml[s].x);
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float l = 0.f, acc[V];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % WPR;
+    const int64_t row = (int64_t)blockIdx.x * (W / WPR) + warp / WPR;       // (b * KV + kvh) * R + r
+    const bool live = row < (int64_t)p.B * p.KV * p.R;
+    const int64_t item = live ? quot(row, p.R) : 0;
+    const int r = live ? (int)(row - item * p.R) : 0;
+    const int64_t b = quot(item, p.KV);
+    const int kvh = (int)(item - b * p.KV), tile = r / C;
+    const int64_t pos0 = p.pos0[b * p.pos_stride];
+    const int2 held = p.held[item * p.tiles + tile];                // not written for a sequence that holds nothing
+    const int64_t nb = kv4_blocks_of(p, pos0);
+    const int tok = r / p.G, hh = r - tok * p.G;
+    if (live && sub == 0 && lane == 0 && pos0 + tok >= p.max_seq) atomicOr(&g_status, kErrBadIndex);
+    float acc[V], l = 0.f;
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[i] = 0.f;
-    for (int s = 0; s < p.nsplit; ++s) {
-        const float2 x = ml[s];
-        const float f = ex2(x.x - top);
-        l += x.y * f;
-        const float *src = p.part_o + (row * p.nsplit + s) * D + lane * V;
-#pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] = fmaf(src[i], f, acc[i]);
+    const bool parts = live && nb > 0 && held.x != held.y, write = live && (nb == 0 || parts);
+    if (parts) {
+        const int c0 = held.x, c1 = held.y;
+        const auto slot = [&](int c) { return ((int64_t)c * 2 + (c == c0 ? 1 : 0)) * C + (r - tile * C); };
+        float top = kNoMax;
+#pragma unroll 4
+        for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, p.part_ml[slot(c)].x);
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll 8
+        for (int c = c0 + sub; c <= c1; c += WPR) {
+            const int64_t at = slot(c);
+            const float2 x = p.part_ml[at];
+            const float f = ex2(x.x - top);
+            l += x.y * f;
+            const float *src = p.part_o + at * D + lane * V;
+            if constexpr (V == 4) {
+                const float4 y = *reinterpret_cast<const float4 *>(src);
+                acc[0] = fmaf(y.x, f, acc[0]);
+                acc[1] = fmaf(y.y, f, acc[1]);
+                acc[2] = fmaf(y.z, f, acc[2]);
+                acc[3] = fmaf(y.w, f, acc[3]);
+            } else {
+                const float2 y = *reinterpret_cast<const float2 *>(src);
+                acc[0] = fmaf(y.x, f, acc[0]);
+                acc[1] = fmaf(y.y, f, acc[1]);
+            }
+        }
     }
+    if constexpr (WPR > 1) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) s_acc[warp][lane * V + i] = acc[i];
+        if (lane == 0) s_l[warp] = l;
+        __syncthreads();
+        if (sub) return;
+#pragma unroll 4
+        for (int w = 1; w < WPR; ++w) {
+            l += s_l[warp + w];
+#pragma unroll
+            for (int i = 0; i < V; ++i) acc[i] += s_acc[warp + w][lane * V + i];
+        }
+    }
+    if (!write) return;
     const float inv = l != 0.f ? 1.f / l : 0.f;
-    const int64_t item = row / p.R;
-    const int r = (int)(row - item * p.R), tok = r / p.G, hh = r - tok * p.G;
-    const int64_t b = item / p.KV;
-    const int kvh = (int)(item - b * p.KV);
     uint16_t *dst = p.out + ((b * p.T + tok) * p.H + kvh * p.G + hh) * D + lane * V;
 #pragma unroll
     for (int i = 0; i < V; i += 2)
         *reinterpret_cast<uint32_t *>(dst + i) = pack_bf16x2(acc[i] * inv, acc[i + 1] * inv);
 }
 
-template <typename P>
-static int launch_kv4(void (*kern)(P), dim3 grid, unsigned block, size_t smem, cudaStream_t st, const char *what,
-                      const P &params) {
+// Launch as a programmatic dependent of the previous kernel of the stream.  The
+// shared-memory limit of a kernel is raised once per device.
+template <auto Kern, typename P>
+static int launch_kv4(dim3 grid, unsigned block, size_t smem, cudaStream_t st, const char *what, const P &params) {
+    cudaError_t e;
+    if (smem > 48 * 1024) {
+        static std::atomic<uint64_t> raised{0};
+        int dev = 0;
+        e = cudaGetDevice(&dev);
+        const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+        if (e == cudaSuccess && !(raised.load(std::memory_order_relaxed) & bit)) {
+            e = cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+            if (e == cudaSuccess) raised.fetch_or(bit, std::memory_order_relaxed);
+        }
+        if (e != cudaSuccess) return set_error(BF16X_ERR_CUDA, "%s: shared memory: %s", what, cudaGetErrorString(e));
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(block);
@@ -678,36 +933,36 @@ static int launch_kv4(void (*kern)(P), dim3 grid, unsigned block, size_t smem, c
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return set_error(BF16X_ERR_CUDA, "%s: shared memory: %s", what, cudaGetErrorString(e));
-    }
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, params);
+    e = cudaLaunchKernelEx(&cfg, Kern, params);
     if (e != cudaSuccess) return set_error(BF16X_ERR_CUDA, "%s: launch: %s", what, cudaGetErrorString(e));
     return check_launch(what);
 }
 
-// Column tiles of 8 rows that one CTA takes, and the splits of the positions.
-static int attend_tiles(int64_t R) { return R > 16 ? 4 : R > 8 ? 2 : 1; }
-static int attend_splits(int64_t items, int64_t row_tiles, int64_t nblk) {
-    const int64_t want = (2 * 148 + items * row_tiles - 1) / (items * row_tiles);
-    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, nblk / kAttendWarps), 148));
-}
+// Column tiles of 8 rows that one warp takes, and the grid.
+static int attend_tiles(int64_t R) { return R > 8 ? 2 : 1; }
+constexpr int kAttendGrid = 148;
+static int attend_warps(int nt) { return kAttendGrid * (nt == 1 ? AttendCfg<128, 1>::kWarps : AttendCfg<128, 2>::kWarps); }
 
 template <int D, int NT>
-static int attend_launch(const Kv4AttendParams &p, int64_t row_tiles, cudaStream_t st) {
-    const int64_t items = (int64_t)p.B * p.KV;
-    int rc = launch_kv4(kv4_attend_kernel<D, NT>, dim3((unsigned)p.nsplit, (unsigned)row_tiles, (unsigned)items),
-                        kAttendWarps * 32, sizeof(AttendSmem<D, NT>), st, "kv4_attend_kernel", p);
-    if (rc != BF16X_OK || p.nsplit == 1) return rc;
-    return launch_kv4(kv4_join_kernel<D>, dim3((unsigned)((items * p.R + 3) / 4)), 128, 0, st, "kv4_join_kernel", p);
+static int attend_launch(const Kv4AttendParams &p, cudaStream_t st) {
+    static_assert(AttendCfg<D, NT>::kWarps == AttendCfg<128, NT>::kWarps, "attend_warps");
+    const int64_t rows = (int64_t)p.B * p.KV * p.R, units = (int64_t)p.B * p.KV * p.tiles;
+    const int rc = launch_kv4<kv4_attend_kernel<D, NT>>(dim3(kAttendGrid), AttendCfg<D, NT>::kWarps * 32,
+                                                        sizeof(AttendSmem<D, NT>), st, "kv4_attend_kernel", p);
+    if (rc != BF16X_OK) return rc;
+    // a row has up to p.warps / units parts
+    if (units * 64 <= p.warps)
+        return launch_kv4<kv4_join_kernel<D, NT, 32>>(dim3((unsigned)rows), 1024, 0, st, "kv4_join_kernel", p);
+    if (units * 8 <= p.warps)
+        return launch_kv4<kv4_join_kernel<D, NT, 8>>(dim3((unsigned)rows), 256, 0, st, "kv4_join_kernel", p);
+    return launch_kv4<kv4_join_kernel<D, NT, 1>>(dim3((unsigned)((rows + 7) / 8)), 256, 0, st, "kv4_join_kernel", p);
 }
 
 static int check_shape(const char *what, int64_t B, int64_t T, int64_t KV, int64_t D, int64_t max_seq) {
     if (B < 0 || T < 0 || KV <= 0 || max_seq <= 0) return set_error(BF16X_ERR_INVALID, "%s: bad shape", what);
     if (D != 64 && D != 128) return set_error(BF16X_ERR_UNSUPPORTED, "%s: head_dim must be 64 or 128", what);
-    if (B > 65535 || KV > 4096 || T > (1 << 24) || max_seq > ((int64_t)1 << 40) || B * KV > 65535)
-        return set_error(BF16X_ERR_UNSUPPORTED, "%s: batch * kv_heads must be at most 65535", what);
+    if (B > 65535 || KV > 4096 || T > (1 << 24) || max_seq > ((int64_t)1 << 30) || B * KV > 65535)
+        return set_error(BF16X_ERR_UNSUPPORTED, "%s: at most 65535 heads in the batch and 2^30 positions", what);
     return BF16X_OK;
 }
 
@@ -733,9 +988,9 @@ extern "C" int bf16x_kv4_append(const uint16_t *qkv, int64_t ld_b, int64_t ld_t,
                          max_seq, (max_seq + kKvBlock - 1) / kKvBlock};
     const int64_t threads = B * T * (H + 2 * KV) * (D / 8), grid = (threads + 255) / 256;
     if (grid > 0x7fffffffLL) return set_error(BF16X_ERR_UNSUPPORTED, "bf16x_kv4_append: too many tokens");
-    return D == 64 ? launch_kv4(kv4_append_kernel<64>, dim3((unsigned)grid), 256, 0, (cudaStream_t)stream,
+    return D == 64 ? launch_kv4<kv4_append_kernel<64>>(dim3((unsigned)grid), 256, 0, (cudaStream_t)stream,
                                 "kv4_append_kernel", p)
-                   : launch_kv4(kv4_append_kernel<128>, dim3((unsigned)grid), 256, 0, (cudaStream_t)stream,
+                   : launch_kv4<kv4_append_kernel<128>>(dim3((unsigned)grid), 256, 0, (cudaStream_t)stream,
                                 "kv4_append_kernel", p);
 }
 
@@ -751,18 +1006,18 @@ extern "C" int bf16x_kv4_read(const uint8_t *blocks, int64_t max_seq, int64_t B,
                        k_out, v_out};
     const int64_t threads = B * T * 2 * KV * (D / 8), grid = (threads + 255) / 256;
     if (grid > 0x7fffffffLL) return set_error(BF16X_ERR_UNSUPPORTED, "bf16x_kv4_read: too many tokens");
-    return D == 64 ? launch_kv4(kv4_read_kernel<64>, dim3((unsigned)grid), 256, 0, (cudaStream_t)stream,
+    return D == 64 ? launch_kv4<kv4_read_kernel<64>>(dim3((unsigned)grid), 256, 0, (cudaStream_t)stream,
                                 "kv4_read_kernel", p)
-                   : launch_kv4(kv4_read_kernel<128>, dim3((unsigned)grid), 256, 0, (cudaStream_t)stream,
+                   : launch_kv4<kv4_read_kernel<128>>(dim3((unsigned)grid), 256, 0, (cudaStream_t)stream,
                                 "kv4_read_kernel", p);
 }
 
 extern "C" int64_t bf16x_kv4_attend_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t KV, int64_t D,
                                                     int64_t max_seq) {
     if (B <= 0 || T <= 0 || H <= 0 || KV <= 0 || H % KV || max_seq <= 0) return 0;
-    const int64_t R = T * (H / KV), C = 8 * attend_tiles(R), items = B * KV;
-    const int n = attend_splits(items, (R + C - 1) / C, (max_seq + kKvBlock - 1) / kKvBlock);
-    return n == 1 ? 0 : items * R * n * (D * 4 + 8);
+    const int nt = attend_tiles(T * (H / KV));
+    const int64_t units = B * KV * ((T * (H / KV) + 8 * nt - 1) / (8 * nt));
+    return (int64_t)attend_warps(nt) * 2 * 8 * nt * (D * 4 + 8) + units * 8;
 }
 
 extern "C" int bf16x_kv4_attend(const uint16_t *q, int64_t ldq_b, int64_t ldq_t, int64_t ldq_h, int64_t B, int64_t T,
@@ -781,22 +1036,19 @@ extern "C" int bf16x_kv4_attend(const uint16_t *q, int64_t ldq_b, int64_t ldq_t,
     const int64_t need = bf16x_kv4_attend_workspace_bytes(B, T, H, KV, D, max_seq);
     if (need && (!workspace || workspace_bytes < need))
         return set_error(BF16X_ERR_INVALID, "bf16x_kv4_attend: workspace too small (%lld bytes needed)", (long long)need);
-    const int64_t G = H / KV, R = T * G, nblk = (max_seq + kKvBlock - 1) / kKvBlock, items = B * KV;
+    const int64_t G = H / KV, R = T * G, nblk = (max_seq + kKvBlock - 1) / kKvBlock;
+    if (R > 0x7fffff00LL || B * KV * R > ((int64_t)1 << 32)) return set_error(BF16X_ERR_UNSUPPORTED, "bf16x_kv4_attend: too many query rows");
     const int nt = attend_tiles(R);
-    const int64_t row_tiles = (R + 8 * nt - 1) / (8 * nt);
-    if (row_tiles > 65535) return set_error(BF16X_ERR_UNSUPPORTED, "bf16x_kv4_attend: too many query rows");
     Kv4AttendParams p = {};
     p.q = q, p.ldq_b = ldq_b, p.ldq_t = ldq_t, p.ldq_h = ldq_h;
     p.B = (int)B, p.T = (int)T, p.H = (int)H, p.KV = (int)KV, p.G = (int)G, p.R = (int)R;
+    p.tiles = (int)((R + 8 * nt - 1) / (8 * nt)), p.warps = attend_warps(nt);
     p.pos_stride = pos_stride, p.pos0 = pos0, p.scale_log2 = scale * 1.44269504088896340736f;
     p.blocks = blocks, p.max_seq = max_seq, p.nblk = nblk, p.out = out;
-    p.nsplit = attend_splits(items, row_tiles, nblk);
     p.part_o = (float *)workspace;
-    p.part_ml = (float2 *)((uint8_t *)workspace + items * R * p.nsplit * D * 4);
+    p.part_ml = (float2 *)((uint8_t *)workspace + (int64_t)p.warps * 2 * 8 * nt * D * 4);
+    p.held = (int2 *)(p.part_ml + (int64_t)p.warps * 2 * 8 * nt);
     cudaStream_t st = (cudaStream_t)stream;
-    if (D == 64)
-        return nt == 1 ? attend_launch<64, 1>(p, row_tiles, st)
-                       : nt == 2 ? attend_launch<64, 2>(p, row_tiles, st) : attend_launch<64, 4>(p, row_tiles, st);
-    return nt == 1 ? attend_launch<128, 1>(p, row_tiles, st)
-                   : nt == 2 ? attend_launch<128, 2>(p, row_tiles, st) : attend_launch<128, 4>(p, row_tiles, st);
+    if (D == 64) return nt == 1 ? attend_launch<64, 1>(p, st) : attend_launch<64, 2>(p, st);
+    return nt == 1 ? attend_launch<128, 1>(p, st) : attend_launch<128, 2>(p, st);
 }

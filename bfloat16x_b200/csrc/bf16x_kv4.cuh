@@ -76,26 +76,44 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
     return r;
 }
 
-// D[16][8] += A[16][16] B[16][8], fp32 sums
-__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                        uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-                 "{%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-                 "{%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
+// D[16][8] = A[16][16] B[16][8] + C, fp32 sums
+#define BF16X_MMA(NAME, TYPE)                                                                                         \
+    __device__ __forceinline__ void NAME(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,           \
+                                         uint32_t b0, uint32_t b1, float c0, float c1, float c2, float c3) {          \
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32." TYPE "." TYPE ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "     \
+                     "{%8,%9}, {%10,%11,%12,%13};"                                                                    \
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])                                                 \
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));     \
+    }                                                                                                                 \
+    __device__ __forceinline__ void NAME(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,           \
+                                         uint32_t b0, uint32_t b1) {                                                  \
+        NAME(c, a0, a1, a2, a3, b0, b1, c[0], c[1], c[2], c[3]);                                                      \
+    }
+BF16X_MMA(mma_f16, "f16")
+BF16X_MMA(mma_bf16, "bf16")
+#undef BF16X_MMA
 
 // transposed 8x8 tile of 16-bit values: row g, columns 2t, 2t+1 -> row 2t.. as column
 __device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
     uint32_t r;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+    return r;
+}
+
+// shared-memory loads by 32-bit address
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+    uint32_t r;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(r) : "r"(a) : "memory");
+    return r;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+    uint2 r;
+    asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(a) : "memory");
+    return r;
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+    uint4 r;
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a) : "memory");
     return r;
 }
 
