@@ -39,6 +39,7 @@
 #include "bf16x_resident.cuh"
 #include "bf16x_status.cuh"
 #include "bf16x_tmap.h"
+#include "bf16x_umma.cuh"
 #include "bf16x_wait.cuh"
 
 namespace bf16x {
@@ -92,17 +93,6 @@ struct GemmParams {
 };
 
 // ------------------------------------------------------------- tcgen05 glue
-__device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t smem_addr) {
-    // K-major, 128-byte swizzle: rows of 128 bytes, 8-row atoms 1024 bytes apart
-    uint64_t d = 0;
-    d |= (uint64_t)((smem_addr >> 4) & 0x3FFFu);          // start address
-    d |= (uint64_t)1u << 16;                               // leading byte offset (unused for swizzled K-major)
-    d |= (uint64_t)(1024u >> 4) << 32;                     // stride byte offset
-    d |= (uint64_t)1u << 46;                               // descriptor version (sm100)
-    d |= (uint64_t)2u << 61;                               // layout: SWIZZLE_128B
-    return d;
-}
-
 template <int BN>
 __host__ __device__ constexpr uint32_t umma_idesc_bf16() {
     return (1u << 4)                       // D: f32
@@ -120,14 +110,6 @@ __device__ __forceinline__ void umma_bf16(uint32_t d_tmem, uint64_t adesc, uint6
         :: "r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
 }
 
-__device__ __forceinline__ void umma_commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
-                 :: "r"(smem_u32(bar)) : "memory");
-}
-
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
@@ -135,16 +117,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
           "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
         : "r"(taddr));
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-
-__device__ __forceinline__ void named_bar_sync(int id, int n) {
-    asm volatile("bar.sync %0, %1;" :: "r"(id), "r"(n) : "memory");
-}
-
-// Byte offset of element (row, col) inside a 128-row x 64-column K-major
-// 128-byte-swizzled tile (16-byte chunk index XOR row % 8).
-__device__ __forceinline__ uint32_t sw128_offset(uint32_t row, uint32_t col) {
-    return row * 128u + ((((col >> 3) ^ row) & 7u) << 4) + ((col & 7u) << 1);
 }
 
 template <int BN>

@@ -1,7 +1,6 @@
 // bf16x_kv4.cu -- writing the 4-bit key/value cache, reading it back, and
 // attention of few query rows over it (decode steps, a few guessed tokens).
 #include <algorithm>
-#include <atomic>
 
 #include <cuda_runtime.h>
 
@@ -215,24 +214,6 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
 // P dV has to fit fp16 whatever the scale of V, so the running reference M of
 // a row is the maximum of S' + log2(max_j dV_j), not of S' alone; it is
 // raised only when a term exceeds it by more than 2^8.
-struct Kv4AttendParams {
-    const uint16_t *q;
-    int64_t ldq_b, ldq_t, ldq_h;
-    int B, T, H, KV, G, R;
-    int pos_stride, tiles, warps;       // row tiles per head; warps of the grid
-    const int64_t *pos0;
-    float scale_log2;                   // softmax scale * log2(e)
-    const uint8_t *blocks;
-    int64_t max_seq, nblk;
-    uint16_t *out;
-    float *part_o;                      // [share][2][row of the tile][D]
-    float2 *part_ml;                    // [share][2][row of the tile]
-    int2 *held;                         // [unit]: the first and last share that hold blocks of it
-};
-
-constexpr float kRescale = 8.f;         // log2 of how far a term may exceed the reference
-constexpr float kNoMax = -3.0e38f;
-
 template <int D, int NT>
 struct Kv4Rows {
     static constexpr int NG = D / 32;
@@ -907,36 +888,8 @@ __global__ void __launch_bounds__(WPR > 8 ? WPR * 32 : 256) kv4_join_kernel(cons
         *reinterpret_cast<uint32_t *>(dst + i) = pack_bf16x2(acc[i] * inv, acc[i + 1] * inv);
 }
 
-// Launch as a programmatic dependent of the previous kernel of the stream.  The
-// shared-memory limit of a kernel is raised once per device.
-template <auto Kern, typename P>
-static int launch_kv4(dim3 grid, unsigned block, size_t smem, cudaStream_t st, const char *what, const P &params) {
-    cudaError_t e;
-    if (smem > 48 * 1024) {
-        static std::atomic<uint64_t> raised{0};
-        int dev = 0;
-        e = cudaGetDevice(&dev);
-        const uint64_t bit = dev < 64 ? 1ull << dev : 0;
-        if (e == cudaSuccess && !(raised.load(std::memory_order_relaxed) & bit)) {
-            e = cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-            if (e == cudaSuccess) raised.fetch_or(bit, std::memory_order_relaxed);
-        }
-        if (e != cudaSuccess) return set_error(BF16X_ERR_CUDA, "%s: shared memory: %s", what, cudaGetErrorString(e));
-    }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(block);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, Kern, params);
-    if (e != cudaSuccess) return set_error(BF16X_ERR_CUDA, "%s: launch: %s", what, cudaGetErrorString(e));
-    return check_launch(what);
-}
+// Rows per kv head up to which the kernel of this file takes a call; above, the prompt kernel.
+constexpr int64_t kFewRows = 16;
 
 // Column tiles of 8 rows that one warp takes, and the grid.
 static int attend_tiles(int64_t R) { return R > 8 ? 2 : 1; }
@@ -1015,6 +968,7 @@ extern "C" int bf16x_kv4_read(const uint8_t *blocks, int64_t max_seq, int64_t B,
 extern "C" int64_t bf16x_kv4_attend_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t KV, int64_t D,
                                                     int64_t max_seq) {
     if (B <= 0 || T <= 0 || H <= 0 || KV <= 0 || H % KV || max_seq <= 0) return 0;
+    if (T * (H / KV) > kFewRows) return kv4_prefill_workspace(B, KV, T * (H / KV), D, max_seq);
     const int nt = attend_tiles(T * (H / KV));
     const int64_t units = B * KV * ((T * (H / KV) + 8 * nt - 1) / (8 * nt));
     return (int64_t)attend_warps(nt) * 2 * 8 * nt * (D * 4 + 8) + units * 8;
@@ -1045,6 +999,7 @@ extern "C" int bf16x_kv4_attend(const uint16_t *q, int64_t ldq_b, int64_t ldq_t,
     p.tiles = (int)((R + 8 * nt - 1) / (8 * nt)), p.warps = attend_warps(nt);
     p.pos_stride = pos_stride, p.pos0 = pos0, p.scale_log2 = scale * 1.44269504088896340736f;
     p.blocks = blocks, p.max_seq = max_seq, p.nblk = nblk, p.out = out;
+    if (R > kFewRows) return kv4_prefill(p, D, workspace, (cudaStream_t)stream);
     p.part_o = (float *)workspace;
     p.part_ml = (float2 *)((uint8_t *)workspace + (int64_t)p.warps * 2 * 8 * nt * D * 4);
     p.held = (int2 *)(p.part_ml + (int64_t)p.warps * 2 * 8 * nt);

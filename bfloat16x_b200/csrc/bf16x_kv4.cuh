@@ -21,6 +21,8 @@
 // are taken out of the other operand (K) or of the sums (V).
 #pragma once
 
+#include <atomic>
+
 #include "bf16x_common.cuh"
 #include "bf16x_status.cuh"
 
@@ -116,5 +118,59 @@ __device__ __forceinline__ uint4 lds128(uint32_t a) {
     asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a) : "memory");
     return r;
 }
+
+// Arguments of the attention kernels.  Rows of one kv head: r = t * G + h.
+struct Kv4AttendParams {
+    const uint16_t *q;
+    int64_t ldq_b, ldq_t, ldq_h;
+    int B, T, H, KV, G, R;
+    int pos_stride, tiles, warps;       // row tiles per head; warps of the grid
+    const int64_t *pos0;
+    float scale_log2;                   // softmax scale * log2(e)
+    const uint8_t *blocks;
+    int64_t max_seq, nblk;
+    uint16_t *out;
+    float *part_o;                      // [share][2][row of the tile][D]
+    float2 *part_ml;                    // [share][2][row of the tile]
+    int2 *held;                         // [unit]: the first and last share that hold blocks of it
+};
+
+constexpr float kRescale = 8.f;         // log2 of how far a term may exceed the reference
+constexpr float kNoMax = -3.0e38f;
+
+// Launch as a programmatic dependent of the previous kernel of the stream.  The
+// shared-memory limit of a kernel is raised once per device.
+template <auto Kern, typename P>
+static int launch_kv4(dim3 grid, unsigned block, size_t smem, cudaStream_t st, const char *what, const P &params) {
+    cudaError_t e;
+    if (smem > 48 * 1024) {
+        static std::atomic<uint64_t> raised{0};
+        int dev = 0;
+        e = cudaGetDevice(&dev);
+        const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+        if (e == cudaSuccess && !(raised.load(std::memory_order_relaxed) & bit)) {
+            e = cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+            if (e == cudaSuccess) raised.fetch_or(bit, std::memory_order_relaxed);
+        }
+        if (e != cudaSuccess) return set_error(BF16X_ERR_CUDA, "%s: shared memory: %s", what, cudaGetErrorString(e));
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, Kern, params);
+    if (e != cudaSuccess) return set_error(BF16X_ERR_CUDA, "%s: launch: %s", what, cudaGetErrorString(e));
+    return check_launch(what);
+}
+
+// Attention of many rows per kv head (bf16x_kv4_prefill.cu): its workspace, and its launch.
+int64_t kv4_prefill_workspace(int64_t B, int64_t KV, int64_t R, int64_t D, int64_t max_seq);
+int kv4_prefill(Kv4AttendParams p, int64_t D, void *workspace, cudaStream_t st);
 
 }  // namespace bf16x

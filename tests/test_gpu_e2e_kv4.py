@@ -12,6 +12,14 @@ from tests.gpu_util import rel_l2
 
 pytestmark = pytest.mark.gpu
 TOL = 2e-2           # the decoder tests' tolerance: bf16 activations on both sides
+# Where the projections run at another number of rows, keys and values differ in
+# their last bf16 bit (up to 2^-8 of the value) before they are quantised, and a
+# value that crosses a border moves by a whole step d.  With 32 normal values
+# per group d is 4.1 sigma / 15 = 0.27 sigma; a value of 0.8 sigma crosses with
+# probability 2^-8 * 0.8 / 0.27 = 1.2 %, which is sqrt(0.012) * 0.27 = 3 % of the
+# keys' and values' norm if every value differs.  Two layers, keys and values:
+# 2 * 3 % on the attention's part of the stream at most, beside TOL.
+TOL_STEPS = 8e-2
 
 
 def _prompt(B, P, vocab, seed=1):
@@ -62,8 +70,8 @@ def test_prompts_of_different_lengths():
     for i, n in enumerate(lengths):
         a = one(prompt[i:i + 1, P - n:], torch.zeros((), dtype=torch.long, device="cuda"))
         b = one(prompt[i:i + 1, :1], torch.tensor(n, device="cuda"))
-        assert rel_l2(first[i].cpu().numpy(), a[0].cpu().numpy()) < TOL
-        assert rel_l2(nxt[i].cpu().numpy(), b[0].cpu().numpy()) < TOL
+        assert rel_l2(first[i].cpu().numpy(), a[0].cpu().numpy()) < TOL_STEPS
+        assert rel_l2(nxt[i].cpu().numpy(), b[0].cpu().numpy()) < TOL_STEPS
     _lib.check_device_status()
 
 
