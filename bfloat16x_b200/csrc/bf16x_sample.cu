@@ -12,7 +12,7 @@
 // so all of them together are one cut: a key and how many of its ties stay.
 //
 // Which token a number u falls on must not depend on the order of a sum: the
-// weights are computed in fp64 and held as 64-bit integers (2^-SH steps, SH
+// weights have some 31 correct bits and are held as 64-bit integers (2^-SH steps, SH
 // such that the sum of a row cannot overflow), so every sum is exact and the
 // same in any order.  With ~1e5 kept tokens, fp32 weights would move about
 // one draw in a hundred to a neighbour.
@@ -39,7 +39,7 @@ constexpr int kSampleWarps = 16;
 constexpr int kSampleThreads = kSampleWarps * 32;
 constexpr int kSampleBins = 1600;                     // 50 octaves: weights below 2^-49 are 0
 constexpr int kSampleCap = 1024;                      // tokens that one CTA sorts
-constexpr int kSampleMaxKeys = 40960;                 // keys per CTA (160 KB)
+constexpr int kSampleMaxKeys = 40960;                 // tokens per CTA (81 keys per thread: 162 KB)
 constexpr int kSampleMaxCluster = 8;
 constexpr uint32_t kKeyNegInf = 0x007FFFFFu;          // key of -infinity
 
@@ -54,24 +54,24 @@ struct SampleParams {
     int64_t *tokens;
 };
 
-// 2^(-i/64)
-__constant__ double c_exp2_tab[64] = {
-    1, 0.98922801319397546, 0.97857206208770009, 0.96803089674614717,
-    0.9576032806985737, 0.9472879907934828, 0.93708381705514998, 0.92698956254169274,
-    0.91700404320467122, 0.90712608775019943, 0.89735453750155358, 0.88768824626326059,
-    0.87812608018664973, 0.86866691763685311, 0.85930964906123897, 0.85005317685926174,
-    0.8408964152537145, 0.83183829016336819, 0.82287773907698247, 0.81401371092867392,
-    0.80524516597462714, 0.7965710756711335, 0.78799042255394325, 0.77950220011891846,
-    0.77110541270397037, 0.76279907537226921, 0.75458221379671142, 0.74645386414563242,
-    0.73841307296974967, 0.73045889709032352, 0.72259040348852333, 0.71480666919598501,
-    0.70710678118654757, 0.69948983626915562, 0.69195494098191601, 0.68450121148729526,
-    0.67712777346844633, 0.66983376202665146, 0.66261832157987066, 0.65548060576238221,
-    0.64841977732550482, 0.64143500803938913, 0.63452547859586661, 0.62769037851234555,
-    0.620928906036742, 0.61424026805343501, 0.60762367999023448, 0.60107836572635154,
-    0.59460355750136051, 0.58819849582514061, 0.58186242938878874, 0.57559461497649134,
-    0.56939431737834578, 0.56326080930412092, 0.55719337129794622, 0.55119129165392045,
-    0.54525386633262884, 0.53938039887855993, 0.53357020033841185, 0.52782258918027858,
-    0.52213689121370688, 0.51651243951061421, 0.51094857432705831, 0.50544464302585024};
+// 2^(62 - i/64)
+__constant__ uint64_t c_exp2_tab[64] = {
+    4611686018427387904ull, 4562008997483360349ull, 4512867096753504463ull, 4464254551929933550ull,
+    4416165660797809419ull, 4368594782566476878ull, 4321536337207803251ull, 4274984804801645281ull,
+    4228934724888366668ull, 4183380695828330266ull, 4138317374168289834ull, 4093739474014606996ull,
+    4049641766413219908ull, 4006019078736290889ull, 3962866294075461077ull, 3920178350641640941ull,
+    3877950241171266237ull, 3836177012338949768ull, 3794853764176460055ull, 3753975649497958757ull,
+    3713537873331429433ull, 3673535692356230935ull, 3633964414346709481ull, 3594819397621804119ull,
+    3556096050500581047ull, 3517789830763632898ull, 3479896245120279830ull, 3442410848681509921ull,
+    3405329244438597040ull, 3368647082747335039ull, 3332360060817827770ull, 3296463922209775076ull,
+    3260954456333195553ull, 3225827497954527522ull, 3191078926708050276ull, 3156704666612568285ull,
+    3122700685593301682ull, 3089062995008926926ull, 3055787649183712190ull, 3022870744944692570ull,
+    2990308421163830843ull, 2958096858305110056ull, 2926232277976504838ull, 2894710942486778865ull,
+    2863529154407056491ull, 2832683256137117140ull, 2802169629476361550ull, 2771984695199399577ull,
+    2742124912636209756ull, 2712586779256821376ull, 2683366830260470360ull, 2654461638169180747ull,
+    2625867812425724110ull, 2597581998995909751ull, 2569600879975159024ull, 2541921173199317625ull,
+    2514539631859660218ull, 2487453044122042215ull, 2460658232750154058ull, 2434152054732833796ull,
+    2407931400915394245ull, 2381993195634921490ull, 2356334396359501942ull, 2330951993331335645ull};
 
 // order-preserving key of a logit; NaN counts as -infinity, -0 as 0
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -83,39 +83,39 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
     return __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
 }
 
-// w = 2^-y in steps of 2^-sh: y = k/64 + g with |g| <= 1/128, so 2^-y =
-// 2^(-k/64) e^(-g ln 2), the last factor by its Taylor series to the 4th power
-// (|g ln 2| <= 0.0055: the rest is below 5e-14).  One call is a dozen fp64
-// operations, which is what a pass over many tokens costs.
+// w = 2^-y in steps of 2^-sh.  The difference top - l is kept exactly as a sum
+// of two fp32 numbers and multiplied by log2(e)/temperature in two parts, so y
+// = k/64 + g has some 40 correct bits; then 2^-y = 2^(-k/64) (1 - u) with the
+// first factor from a table of 62 bits and u = 1 - e^(-g ln 2) by its Taylor
+// series to the 4th power in fp32 (|g ln 2| <= 0.0055: the rest is below 5e-14),
+// which leaves a relative error of about 2^-31 without a sign of its own.  The
+// same in fp64 took some 250 cycles per 32 tokens and scheduler, which was most
+// of a call.
 struct Weigher {
-    double top, inv, scale;                           // maximum logit, log2(e) / temperature, 2^sh
-    float topf, invf;
+    float top, chi, clo;                              // maximum logit, log2(e) / temperature
+    float limit;                                      // weights below half a step are 0
     int sh;
     uint32_t top_key;
-    const double *tab;
+    const uint64_t *tab;
+    __device__ __forceinline__ float pos(uint32_t key) const { return __fmul_rn(__fsub_rn(top, logit_of(key)), chi); }
     __device__ __forceinline__ uint64_t operator()(uint32_t key) const {
         if (key == top_key) return 1ull << sh;
-        const double y = (top - (double)logit_of(key)) * inv;
-        if (!(y < (double)(sh + 2))) return 0;
-        const double magic = 6755399441055744.0 / 64.0;            // 1.5 * 2^52 / 64: rounds to a multiple of 1/64
-        const double yr = y + magic;
-        const int k = (int)(__double_as_longlong(yr) & 0xFFFFFFFFll);
-        const double g = (yr - magic) - y;
-        constexpr double L = 0.6931471805599453094;
-        double p = L * L * L * L / 24.0;
-        p = fma(p, g, L * L * L / 6.0);
-        p = fma(p, g, L * L / 2.0);
-        p = fma(p, g, L);
-        p = fma(p, g, 1.0);
-        const double m = fma(tab[k & 63] * scale, p, 4503599627370496.0);      // + 2^52: the sum's low bits are the integer
-        const uint64_t v = (uint64_t)__double_as_longlong(m) & 0xFFFFFFFFFFFFFull;
-        const int n = k >> 6;
-        return n == 0 ? v : (v + (1ull << (n - 1))) >> n;
+        const float l = logit_of(key), s = __fsub_rn(top, l), p = __fmul_rn(s, chi);
+        if (!(p < limit)) return 0;
+        const float bb = __fsub_rn(s, top), lo = __fsub_rn(__fsub_rn(top, __fsub_rn(s, bb)), __fadd_rn(l, bb));
+        const float e = __fmaf_rn(lo, chi, __fmaf_rn(s, clo, __fmaf_rn(s, chi, -p)));
+        const float m = __fmaf_rn(p, 64.f, 12582912.f);            // 1.5 * 2^23: rounds to a whole number
+        const int k = (int)__float_as_uint(m) - 0x4B400000;
+        const float x = 0.693147181f * __fadd_rn(__fmaf_rn(__fsub_rn(m, 12582912.f), -0.015625f, p), e);
+        const float u = x * (1.f - x * (0.5f - x * (0.166666667f - x * 0.0416666667f)));
+        const int64_t t = (int64_t)tab[k & 63];
+        const int64_t w = t - (((int64_t)__float2int_rn(u * 0x1p38f) * (int64_t)(t >> 31)) >> 7);
+        const int n = 62 - sh + (k >> 6);
+        return (uint64_t)(w + (1ll << (n - 1))) >> n;
     }
     // which 1/32 octave below the maximum a key lies in: rounded fp32 operations, so it never falls as the logit does
-    __device__ __forceinline__ float pos(uint32_t key) const { return (topf - logit_of(key)) * invf; }
     __device__ __forceinline__ int bin(uint32_t key) const {
-        return key == top_key ? 0 : (int)fminf(pos(key), (float)(kSampleBins - 1));
+        return key == top_key ? 0 : (int)fminf(pos(key) * 32.f, (float)(kSampleBins - 1));
     }
 };
 
@@ -138,7 +138,7 @@ struct alignas(16) SampleShared {
     int pick_bin;
     int last_bin;
     uint32_t pick_before, pick_count;
-    double tab[64];
+    uint64_t tab[64];
 };
 
 static_assert(sizeof(SampleShared) % 16 == 0, "the keys behind it are stored 16 bytes at a time");
@@ -147,6 +147,7 @@ struct SampleCtx {
     SampleShared &sm;
     const uint32_t *keys;
     int n, C, rank;
+    int l0, per;                                      // this lane's part of them: per keys from l0 on (per odd: no bank conflicts)
     uint32_t base;
     int turn;                                         // of the two exchange slots
     Weigher weigh;
@@ -179,15 +180,23 @@ __device__ __forceinline__ void cluster_sums(SampleCtx &x, uint64_t w, uint32_t 
         }
     }
     cl.sync();
-    tot_w = 0, tot_c = 0, before_w = 0;
-    for (int r = 0; r < x.C; ++r) {
-        const SampleShared *o = cl.map_shared_rank(&sm, r);
-        const uint64_t a = o->cta_w[s];
-        if (r < x.rank) before_w += a;
-        tot_w += a;
-        tot_c += o->cta_c[s];
+    // lane r reads rank r: one remote access deep, not C
+    uint64_t a = 0, f = 0;
+    uint32_t n = 0;
+    if (lane < x.C) {
+        const SampleShared *o = cl.map_shared_rank(&sm, lane);
+        a = o->cta_w[s];
+        n = o->cta_c[s];
+        f = lane < x.rank ? a : 0;
     }
-    for (int i = 0; i < warp; ++i) before_w += sm.red_w[s][i];
+    f += lane < warp ? sm.red_w[s][lane] : 0;
+    for (int o = 16; o; o >>= 1) {
+        a += __shfl_xor_sync(0xffffffffu, a, o);
+        f += __shfl_xor_sync(0xffffffffu, f, o);
+    }
+    tot_w = a;
+    tot_c = __reduce_add_sync(0xffffffffu, n);
+    before_w = f;
 }
 
 // Inclusive scan over the block (w in thread order).
@@ -231,12 +240,22 @@ __device__ void block_sort(uint64_t *a, int n2) {
 __device__ int gather_sorted(SampleCtx &x, int &n2) {
     SampleShared &sm = x.sm;
     cg::cluster_group cl = cg::this_cluster();
-    int m = 0;
-    for (int r = 0; r < x.C; ++r) {
-        const SampleShared *o = cl.map_shared_rank(&sm, r);
-        const int k = (int)o->n_list;
-        for (int i = threadIdx.x; i < k; i += kSampleThreads) sm.all[m + i] = o->list[i];
-        m += k;
+    const int lane = threadIdx.x & 31;
+    const uint32_t mine = lane < x.C ? cl.map_shared_rank(&sm, lane)->n_list : 0u;
+    uint32_t upto = mine;                                           // tokens of the ranks up to this lane's
+    for (int o = 1; o < kSampleMaxCluster; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
+    }
+    const int m = (int)__shfl_sync(0xffffffffu, upto, x.C - 1);
+    for (int i0 = 0; i0 < m; i0 += kSampleThreads) {
+        const uint32_t i = (uint32_t)(i0 + (int)threadIdx.x);
+        uint32_t r = 0, first = 0;
+        for (int q = 0; q < x.C - 1; ++q) {
+            const uint32_t end = __shfl_sync(0xffffffffu, upto, q);
+            if (i >= end) r = q + 1, first = end;
+        }
+        if (i < (uint32_t)m) sm.all[i] = cl.map_shared_rank(&sm, r)->list[i - first];
     }
     n2 = 64;
     while (n2 < m) n2 <<= 1;
@@ -272,16 +291,21 @@ __device__ void find_bin(SampleCtx &x, uint32_t k, double target) {
     __syncthreads();
     for (int b0 = 0; b0 < kSampleBins; b0 += kSampleThreads) {
         const int b = b0 + tid;
-        uint32_t c = 0, low = 0;
+        uint32_t c = 0;
         uint64_t lows = 0;
-        if (b < kSampleBins)
-            for (int r = 0; r < x.C; ++r) {
-                const SampleShared *o = cl.map_shared_rank(&sm, r);
-                c += o->cnt[b];
-                low = o->low[b];
-                lows += low;
+        if (b < kSampleBins) {
+            uint32_t rc[kSampleMaxCluster], rl[kSampleMaxCluster];
+#pragma unroll
+            for (int r = 0; r < kSampleMaxCluster; ++r) {           // all asked for before the first is used
+                const SampleShared *o = cl.map_shared_rank(&sm, r < x.C ? r : 0);
+                rc[r] = o->cnt[b];
+                rl[r] = o->low[b];
             }
-        const double start = x.weigh.tab[(2 * b) & 63] * x.weigh.scale;
+#pragma unroll
+            for (int r = 0; r < kSampleMaxCluster; ++r)
+                if (r < x.C) c += rc[r], lows += rl[r];
+        }
+        const double start = (double)(x.weigh.tab[(2 * b) & 63] >> (62 - x.weigh.sh));
         uint64_t w = c ? (uint64_t)(start * ((double)c - (double)lows * 0x1p-21)) >> (b >> 5) : 0;
         // inclusive scans of c and w
         uint32_t sc = c;
@@ -382,10 +406,11 @@ __device__ int next_bin(SampleCtx &x, int b, int d) {
 
 // The exact cut at or near bin b: K: the first `k` tokens of the order (`count`
 // of them lie before the bin); else the shortest prefix that weighs `target`.
-// `sum`: the weight of the prefix.
+// `sum`: the weight of the prefix; `at_bin`, `below`: the bin, and this lane's
+// weight in the bins before it (of its warp's part of the row).
 template <bool K>
 __device__ void resolve(SampleCtx &x, int b, uint32_t count, uint32_t k, double target,
-                        uint32_t &cut_key, uint32_t &cut_idx, uint64_t &sum) {
+                        uint32_t &cut_key, uint32_t &cut_idx, uint64_t &sum, int &at_bin, uint64_t &below) {
     SampleShared &sm = x.sm;
     cg::cluster_group cl = cg::this_cluster();
     const int tid = threadIdx.x;
@@ -394,14 +419,16 @@ __device__ void resolve(SampleCtx &x, int b, uint32_t count, uint32_t k, double 
         __syncthreads();
         uint64_t w = 0;
         uint32_t c = 0;
-        for (int i0 = 0; i0 < x.n; i0 += kSampleThreads) {
-            const int i = i0 + tid;
+        for (int q = 0; q < x.per; ++q) {
+            const int i = x.l0 + q;
             const uint32_t key = i < x.n ? x.keys[i] : 0u;
             const int kb = i < x.n ? x.weigh.bin(key) : kSampleBins;
             if (kb < b) w += x.weigh(key);
             if (kb == b) ++c;
             list_tokens(x, min(i, x.n - 1), kb == b);
         }
+        at_bin = b;
+        below = w;
         uint64_t before, skip;
         uint32_t m;
         cluster_sums(x, w, c, before, m, skip);
@@ -537,19 +564,19 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const SampleP
         if (lane == 0) sm.cta_c[0] = top;
     }
     cl.sync();
-    top = 0;
-    for (int r = 0; r < C; ++r) top = max(top, cl.map_shared_rank(&sm, r)->cta_c[0]);
+    top = __reduce_max_sync(0xffffffffu, lane < C ? cl.map_shared_rank(&sm, lane)->cta_c[0] : 0u);
     const float temp = p.temperature ? p.temperature[row] : p.temperature0;
     const float top_p = p.top_p ? p.top_p[row] : p.top_p0, min_p = p.min_p ? p.min_p[row] : p.min_p0;
     const int32_t top_k = p.top_k ? p.top_k[row] : p.top_k0;
     const float u = p.u[row];
-    SampleCtx x = {sm, keys, n, C, rank, (uint32_t)base, 1, {}};
+    const int per = p.seg / 32, l0 = warp * p.seg + lane * per;
+    SampleCtx x = {sm, keys, n, C, rank, l0, per, (uint32_t)base, 1, {}};
     Weigher &weigh = x.weigh;
-    weigh.top = (double)logit_of(top);
-    weigh.inv = 1.4426950408889634074 / (double)temp;
-    weigh.scale = (double)(1ull << p.sh);
-    weigh.topf = logit_of(top);
-    weigh.invf = 32.f * (1.44269504f / temp);
+    const double inv = 1.4426950408889634074 / (double)temp;
+    weigh.top = logit_of(top);
+    weigh.chi = (float)inv;
+    weigh.clo = (float)(inv - (double)weigh.chi);
+    weigh.limit = (float)p.sh + 1.5f;
     weigh.sh = p.sh;
     weigh.top_key = top;
     weigh.tab = sm.tab;
@@ -571,15 +598,17 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const SampleP
             sm.cta_c[1] = at;
         }
         cl.sync();
-        if (rank == 0 && tid == 0) {
-            for (int r = 0; r < C; ++r) at = min(at, cl.map_shared_rank(&sm, r)->cta_c[1]);
-            p.tokens[row] = none ? -1 : (int64_t)at;
+        if (rank == 0 && warp == 0) {
+            at = __reduce_min_sync(0xffffffffu, lane < C ? cl.map_shared_rank(&sm, lane)->cta_c[1] : 0xFFFFFFFFu);
+            if (lane == 0) p.tokens[row] = none ? -1 : (int64_t)at;
         }
         cl.sync();
         return;
     }
     const uint64_t min_w =
         min_p > 0.f ? max((uint64_t)1, (uint64_t)ceil(fmin((double)min_p, 1.0) * (double)(1ull << p.sh))) : 1ull;
+    int at_bin = -1;                                                // the cut's bin, where it was resolved
+    uint64_t below = 0;
     uint32_t cut_key = kKeyNegInf, cut_idx = 0xFFFFFFFFu;           // keep keys above the cut, and its own up to an index
     const bool by_k = top_k > 0 && top_k < p.V, by_p = top_p < 1.f;
     if (by_k || by_p) {
@@ -587,7 +616,7 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const SampleP
         uint64_t w = 0, total, skip;
         for (int i = tid; i < n; i += kSampleThreads) {
             const uint32_t k = keys[i];
-            const float f = k == top ? 0.f : weigh.pos(k);
+            const float f = k == top ? 0.f : weigh.pos(k) * 32.f;
             if (!(f < (float)(kSampleBins - 1))) continue;
             const int b = (int)f;
             atomicAdd(&sm.cnt[b], 1u);
@@ -676,7 +705,7 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const SampleP
         }
         uint64_t sum = total;
         if (by_k && count > 0) {
-            resolve<true>(x, b, before, (uint32_t)top_k, 0.0, cut_key, cut_idx, sum);
+            resolve<true>(x, b, before, (uint32_t)top_k, 0.0, cut_key, cut_idx, sum, at_bin, below);
         } else if (by_k && by_p) {                                  // k reaches past every weight
             uint64_t all = 0;
             for (int i = tid; i < n; i += kSampleThreads) all += weigh(keys[i]);
@@ -689,37 +718,52 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const SampleP
                 b = sm.pick_bin;
                 __syncthreads();
             }
-            resolve<false>(x, b, 0, 0, target, cut_key, cut_idx, sum);
+            resolve<false>(x, b, 0, 0, target, cut_key, cut_idx, sum, at_bin, below);
         }
     }
-    // ---- the kept weight of each warp's part
-    const int s0 = warp * p.seg, s1 = min(n, s0 + p.seg);
+    // ---- the kept weight of each lane's part
     const auto kept = [&](int i) -> uint64_t {
-        if (i >= s1) return 0;
         const uint32_t k = keys[i];
         if (k < cut_key || (k == cut_key && (uint32_t)base + (uint32_t)i > cut_idx)) return 0;
         const uint64_t w = weigh(k);
         return w >= min_w ? w : 0;
     };
+    const int l1 = min(n, l0 + per);
     uint64_t w = 0, total, before;
     uint32_t c;
-    for (int i = s0; i < s1; i += 32) w += kept(i + lane);
+    if (at_bin >= 0 && min_w == 1) {                                // only the cut's bin is left to look at
+        w = below;
+        for (int i = l0; i < l1; ++i)
+            if (weigh.bin(keys[i]) == at_bin) w += kept(i);
+    } else {
+#pragma unroll 2
+        for (int i = l0; i < l1; ++i) w += kept(i);
+    }
     cluster_sums(x, w, 0, total, c, before);
-    for (int o = 16; o; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
-    // ---- the first token whose running sum exceeds u * total
+    // ---- the first token whose running sum exceeds u * total: its lane's part, then the token
     const double ut = fmax((double)u, 0.0) * (double)total;
     const uint64_t goal = min(ut < (double)total ? (uint64_t)ut : total - 1, total - 1);
-    if (goal >= before && goal < before + w) {                      // exactly one warp of the cluster
-        uint64_t run = before;
-        for (int i = s0; i < s1; i += 32) {
-            uint64_t y = kept(i + lane);
+    uint64_t upto = w;
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t z = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += z;
+    }
+    upto += before;
+    const uint32_t over = __ballot_sync(0xffffffffu, upto > goal);
+    if (goal >= before && over) {                                   // exactly one warp of the cluster
+        const int who = __ffs(over) - 1;
+        uint64_t run = __shfl_sync(0xffffffffu, upto - w, who);
+        const int i0 = warp * p.seg + who * per;
+        for (int q = 0; q < per; q += 32) {
+            const int i = i0 + q + lane;
+            uint64_t y = q + lane < per && i < n ? kept(i) : 0;
             for (int o = 1; o < 32; o <<= 1) {
                 const uint64_t z = __shfl_up_sync(0xffffffffu, y, o);
                 if (lane >= o) y += z;
             }
-            const uint32_t over = __ballot_sync(0xffffffffu, run + y > goal);
-            if (over) {
-                if (lane == 0) p.tokens[row] = base + i + (__ffs(over) - 1);
+            const uint32_t hit = __ballot_sync(0xffffffffu, run + y > goal);
+            if (hit) {
+                if (lane == 0) p.tokens[row] = base + i0 + q + (__ffs(hit) - 1);
                 break;
             }
             run += __shfl_sync(0xffffffffu, y, 31);
@@ -748,7 +792,7 @@ extern "C" int bf16x_sample(const void *logits, int dtype, int64_t ld, int64_t B
     while (C < kSampleMaxCluster && (B * C < 2 * 148 || V > (int64_t)C * kSampleMaxKeys)) C *= 2;
     SampleParams p = {};
     p.logits = logits, p.ld = ld, p.V = V, p.bf16 = dtype == BF16X_DTYPE_BF16;
-    p.seg = (int)((V + (int64_t)C * kSampleThreads - 1) / ((int64_t)C * kSampleThreads)) * 32;
+    p.seg = (int)(((V + (int64_t)C * kSampleThreads - 1) / ((int64_t)C * kSampleThreads)) | 1) * 32;
     int lg = 0;
     while (((int64_t)1 << lg) < V) ++lg;
     p.sh = std::min(47, 62 - lg);                     // 16-bit limbs hold weights below 2^48
