@@ -19,11 +19,12 @@
 //
 // One cluster of C CTAs per row; each holds its part of the row as ordered
 // 32-bit keys in shared memory and the logits are read once.  A histogram of
-// (top - l) in 1/32 octaves of weight then says in which bin a cut lies.  If
+// (top - l) in 1/64 octaves of weight then says in which bin a cut lies.  If
 // all tokens down to that bin are few, one CTA sorts them and finishes alone
 // (the usual top-k, and top-p over a peaked row).  Otherwise the weight above
 // the bin is summed exactly and only the bin's own tokens are sorted.
 #include <algorithm>
+#include <atomic>
 
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
@@ -35,11 +36,8 @@ namespace cg = cooperative_groups;
 
 namespace bf16x {
 
-constexpr int kSampleWarps = 32;
-constexpr int kSampleThreads = kSampleWarps * 32;
-constexpr int kSampleBins = 1600;                     // 50 octaves: weights below 2^-49 are 0
-constexpr int kSampleCap = kSampleThreads;            // tokens that one CTA sorts: one per thread
-constexpr int kSampleMaxKeys = 40960;                 // tokens per CTA (41 keys per thread: 164 KB)
+constexpr int kSampleBins = 3200;                     // 50 octaves: weights below 2^-49 are 0
+constexpr int kSampleMaxKeys = 40960;                 // tokens per CTA (160 KB)
 constexpr int kSampleMaxCluster = 8;
 
 struct SampleParams {
@@ -53,7 +51,7 @@ struct SampleParams {
     int64_t *tokens;
 };
 
-// 2^(31 - i/64), and 2^(31 - (2 i - 1/2)/64): where a bin of two such steps begins
+// 2^(31 - i/64), and 2^(31 - (i - 1/2)/64): where the bin of that step begins
 __constant__ uint32_t c_step[64] = {
     2147483648u, 2124350982u, 2101467502u, 2078830522u, 2056437387u, 2034285470u, 2012372174u, 1990694927u,
     1969251188u, 1948038440u, 1927054196u, 1906295993u, 1885761398u, 1865448001u, 1845353420u, 1825475297u,
@@ -63,11 +61,15 @@ __constant__ uint32_t c_step[64] = {
     1392470869u, 1377471191u, 1362633090u, 1347954824u, 1333434672u, 1319070932u, 1304861917u, 1290805962u,
     1276901417u, 1263146652u, 1249540052u, 1236080024u, 1222764986u, 1209593378u, 1196563654u, 1183674286u,
     1170923762u, 1158310587u, 1145833280u, 1133490379u, 1121280436u, 1109202018u, 1097253708u, 1085434106u};
-__constant__ uint32_t c_bin[32] = {
-    2159144272u, 2112878262u, 2067603638u, 2023299156u, 1979944027u, 1937517909u, 1896000896u, 1855373507u,
-    1815616678u, 1776711757u, 1738640488u, 1701385007u, 1664927835u, 1629251865u, 1594340357u, 1560176931u,
-    1526745556u, 1494030547u, 1462016553u, 1430688553u, 1400031848u, 1370032052u, 1340675091u, 1311947188u,
-    1283834865u, 1256324931u, 1229404479u, 1203060876u, 1177281762u, 1152055042u, 1127368878u, 1103211687u};
+__constant__ uint32_t c_bin[64] = {
+    2159144272u, 2135885998u, 2112878262u, 2090118366u, 2067603638u, 2045331439u, 2023299156u, 2001504204u,
+    1979944027u, 1958616096u, 1937517909u, 1916646992u, 1896000896u, 1875577199u, 1855373507u, 1835387448u,
+    1815616678u, 1796058879u, 1776711757u, 1757573041u, 1738640488u, 1719911875u, 1701385007u, 1683057710u,
+    1664927835u, 1646993254u, 1629251865u, 1611701585u, 1594340357u, 1577166143u, 1560176931u, 1543370725u,
+    1526745556u, 1510299473u, 1494030547u, 1477936870u, 1462016553u, 1446267730u, 1430688553u, 1415277195u,
+    1400031848u, 1384950723u, 1370032052u, 1355274085u, 1340675091u, 1326233356u, 1311947188u, 1297814910u,
+    1283834865u, 1270005413u, 1256324931u, 1242791816u, 1229404479u, 1216161350u, 1203060876u, 1190101520u,
+    1177281762u, 1164600099u, 1152055042u, 1139645120u, 1127368878u, 1115224875u, 1103211687u, 1091327906u};
 
 // order-preserving key of a logit (no NaN, no -0)
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -95,27 +97,28 @@ struct Weigher {
     int sh;
     const uint32_t *step;
     // k = y in 1/64 octaves, rounded: fp32 operations each rounded by itself, so it never falls as the logit does
-    static __device__ __forceinline__ int steps(float p) { return (int)__float_as_uint(__fmaf_rn(p, 64.f, 12582912.f)) - 0x4B400000; }
-    // y and its steps; false for weights of 0
-    __device__ __forceinline__ bool place(float l, float &s, float &p, int &k) const {
+        // y, and k as a number and an integer; false for weights of 0
+    __device__ __forceinline__ bool place(float l, float &s, float &p, float &kf, int &k) const {
         s = l == top ? 0.f : __fsub_rn(top, l);                     // (infinity less infinity)
         p = __fmul_rn(s, chi);
         const bool ok = p < limit;
         p = ok ? p : 0.f;
-        k = steps(p);
+        const float m = __fmaf_rn(p, 64.f, 12582912.f);            // 1.5 * 2^23: rounds to a whole number
+        kf = __fsub_rn(m, 12582912.f);
+        k = (int)__float_as_uint(m) - 0x4B400000;
         return ok;
     }
-    // the bin of two such steps, the last one for weights of 0
+    // the bin of one step, the last one for weights of 0
     __device__ __forceinline__ int bin(float l) const {
-        float s, p;
+        float s, p, kf;
         int k;
-        return place(l, s, p, k) ? k >> 1 : kSampleBins - 1;
+        return place(l, s, p, kf, k) ? k : kSampleBins - 1;
     }
     // the weight of a logit that counts as mant * 2^(-31 - (k >> 6))
-    __device__ __forceinline__ uint32_t mantissa(float l, float s, float p, int k) const {
+    __device__ __forceinline__ uint32_t mantissa(float l, float s, float p, float kf, int k) const {
         const float bb = __fsub_rn(s, top), lo = __fsub_rn(__fsub_rn(top, __fsub_rn(s, bb)), __fadd_rn(l, bb));
         const float e = __fmaf_rn(lo, chi, __fmaf_rn(s, clo, __fmaf_rn(s, chi, -p)));
-        const float x = 0.693147181f * __fadd_rn(__fmaf_rn((float)k, -0.015625f, p), e);
+        const float x = 0.693147181f * __fadd_rn(__fmaf_rn(kf, -0.015625f, p), e);
         const float u = x * (1.f - x * (0.5f - x * (0.166666667f - x * 0.0416666667f)));
         const int q = (int)__float_as_uint(__fmaf_rn(u, 0x1p29f, 12582912.f)) - 0x4B400000;       // u 2^29, below 2^22
         const uint32_t t = step[k & 63];
@@ -128,27 +131,30 @@ struct Weigher {
         return acc + (uint64_t)m * (1u << max(e, 0));
     }
     __device__ __forceinline__ uint64_t add(uint64_t acc, float l, bool take = true) const {
-        float s, p;
+        float s, p, kf;
         int k;
-        const bool ok = place(l, s, p, k) && take;                  // no branch: four of these overlap
-        const uint32_t m = mantissa(l, s, p, k);
+        const bool ok = place(l, s, p, kf, k) && take;              // no branch: four of these overlap
+        const uint32_t m = mantissa(l, s, p, kf, k);
         return add(acc, ok ? m : 0u, k);
     }
     __device__ __forceinline__ uint64_t operator()(float l) const { return add(0, l); }
 };
 
+// W warps per CTA, a listed token per thread.
+template <int W>
 struct alignas(16) SampleShared {
+    static constexpr int kThreads = W * 32;
     uint32_t cnt[kSampleBins];
     uint32_t low[kSampleBins];                        // sum over the bin of (weight at its start - weight), 2^-21 of the octave's
-    uint64_t list[kSampleCap];                        // this CTA's tokens of a bin; later the weights of `all`
-    uint64_t all[kSampleCap];                         // the cluster's (first CTA)
-    uint64_t red_w[2][kSampleWarps];
-    uint32_t red_c[2][kSampleWarps];
+    uint64_t list[W * 32];                        // this CTA's tokens of a bin; later the weights of `all`
+    uint64_t all[W * 32];                         // the cluster's (first CTA)
+    uint64_t red_w[2][W];
+    uint32_t red_c[2][W];
     uint64_t cta_w[2];
     uint32_t cta_c[2];
     uint32_t n_list;
-    uint64_t scan[kSampleWarps];
-    uint32_t scan_c[kSampleWarps];
+    uint64_t scan[W];
+    uint32_t scan_c[W];
     // results of the first CTA, read by all
     uint64_t out_w;
     uint32_t out_key, out_idx;
@@ -156,12 +162,14 @@ struct alignas(16) SampleShared {
     int pick_bin;
     int last_bin;
     uint32_t pick_before, pick_count;
-    uint32_t step[64], start[32];
+    uint32_t step[64], start[64];
 };
-static_assert(sizeof(SampleShared) % 16 == 0, "the keys behind it are stored 16 bytes at a time");
+static_assert(sizeof(SampleShared<16>) % 16 == 0 && sizeof(SampleShared<32>) % 16 == 0,
+              "the logits behind it are stored 16 bytes at a time");
 
+template <int W>
 struct SampleCtx {
-    SampleShared &sm;
+    SampleShared<W> &sm;
     const float *logits;                              // this lane's: `per` of them (odd: no bank conflicts), padded
     int per, C, rank;                                 // with -infinity behind the row
     uint32_t first;                                   // index in the row of this lane's first one
@@ -170,8 +178,8 @@ struct SampleCtx {
 };
 
 // f(logit, q) for this lane's logits, four at a time: the weights' chains overlap.
-template <typename F>
-__device__ __forceinline__ void for_logits(const SampleCtx &x, F f) {
+template <int W, typename F>
+__device__ __forceinline__ void for_logits(const SampleCtx<W> &x, F f) {
     int q = 0;
     for (; q + 4 <= x.per; q += 4) {
         float l[4];
@@ -201,9 +209,10 @@ __device__ __forceinline__ uint64_t warp_scan(uint64_t w) {         // inclusive
 // Sums of w and c over the cluster; before_*: those of the CTAs and warps in
 // front of this warp.  Two slots in turn: a slot is written again only after
 // another cluster barrier, when everyone has read it.
-__device__ __forceinline__ void cluster_sums(SampleCtx &x, uint64_t w, uint32_t c, uint64_t &tot_w, uint32_t &tot_c,
+template <int W>
+__device__ __forceinline__ void cluster_sums(SampleCtx<W> &x, uint64_t w, uint32_t c, uint64_t &tot_w, uint32_t &tot_c,
                                              uint64_t &before_w) {
-    SampleShared &sm = x.sm;
+    SampleShared<W> &sm = x.sm;
     cg::cluster_group cl = cg::this_cluster();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, s = x.turn;
     x.turn ^= 1;
@@ -215,8 +224,8 @@ __device__ __forceinline__ void cluster_sums(SampleCtx &x, uint64_t w, uint32_t 
     }
     __syncthreads();
     if (warp == 0) {
-        const uint64_t a = warp_sum(sm.red_w[s][lane]);
-        const uint32_t b = __reduce_add_sync(0xffffffffu, sm.red_c[s][lane]);
+        const uint64_t a = warp_sum(lane < W ? sm.red_w[s][lane] : 0);
+        const uint32_t b = __reduce_add_sync(0xffffffffu, lane < W ? sm.red_c[s][lane] : 0u);
         if (lane == 0) {
             sm.cta_w[s] = a;
             sm.cta_c[s] = b;
@@ -227,7 +236,7 @@ __device__ __forceinline__ void cluster_sums(SampleCtx &x, uint64_t w, uint32_t 
     uint64_t a = 0, f = lane < warp ? sm.red_w[s][lane] : 0;
     uint32_t n = 0;
     if (lane < x.C) {
-        const SampleShared *o = cl.map_shared_rank(&sm, lane);
+        const SampleShared<W> *o = cl.map_shared_rank(&sm, lane);
         a = o->cta_w[s];
         n = o->cta_c[s];
         if (lane < x.rank) f += a;
@@ -238,12 +247,13 @@ __device__ __forceinline__ void cluster_sums(SampleCtx &x, uint64_t w, uint32_t 
 }
 
 // Inclusive scan over the block (in thread order), and the block's total.
-__device__ __forceinline__ uint64_t block_scan(SampleShared &sm, uint64_t w, uint64_t &total) {
+template <int W>
+__device__ __forceinline__ uint64_t block_scan(SampleShared<W> &sm, uint64_t w, uint64_t &total) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     w = warp_scan(w);
     if (lane == 31) sm.scan[warp] = w;
     __syncthreads();
-    const uint64_t all = sm.scan[lane];
+    const uint64_t all = lane < W ? sm.scan[lane] : 0;
     w += warp_sum(lane < warp ? all : 0);
     total = warp_sum(all);
     __syncthreads();
@@ -252,7 +262,8 @@ __device__ __forceinline__ uint64_t block_scan(SampleShared &sm, uint64_t w, uin
 
 // Ascending sort of one number per thread of the first n2 threads (a power of
 // two >= 64): shuffles within warps, shared memory (`all`) between them.
-__device__ uint64_t block_sort(SampleShared &sm, uint64_t a, int n2) {
+template <int W>
+__device__ uint64_t block_sort(SampleShared<W> &sm, uint64_t a, int n2) {
     const int tid = threadIdx.x;
     for (int size = 2; size <= n2; size <<= 1)
         for (int j = size >> 1; j; j >>= 1) {
@@ -275,7 +286,8 @@ __device__ uint64_t block_sort(SampleShared &sm, uint64_t a, int n2) {
 // The cluster's listed tokens in the first CTA, one per thread: ~key << 32 |
 // index, so that they ascend in the order (logit down, index up), all ones
 // behind the last.  Returns their number.
-__device__ __forceinline__ int gather(SampleCtx &x, uint64_t &token) {
+template <int W>
+__device__ __forceinline__ int gather(SampleCtx<W> &x, uint64_t &token) {
     cg::cluster_group cl = cg::this_cluster();
     const int lane = threadIdx.x & 31;
     const uint32_t mine = lane < x.C ? cl.map_shared_rank(&x.sm, lane)->n_list : 0u;
@@ -299,7 +311,6 @@ __device__ __forceinline__ int sort_size(int m) { return m <= 64 ? 64 : 1 << (32
 
 // Where few tokens are listed, eight threads count for each what a sort would
 // find: `before`: how many of `tok` are smaller, and what those weigh.
-constexpr int kCountCap = kSampleThreads / 8;
 __device__ __forceinline__ void count_before(const uint64_t *tok, const uint64_t *weight, int m, uint64_t mine, int &before,
                                              uint64_t &before_w) {
     before = 0, before_w = 0;
@@ -317,29 +328,31 @@ __device__ __forceinline__ void count_before(const uint64_t *tok, const uint64_t
 }
 
 // This lane's logit q into the CTA's list, if `take` (called by whole warps).
-__device__ __forceinline__ void list_token(SampleCtx &x, float l, int q, bool take) {
-    SampleShared &sm = x.sm;
+template <int W>
+__device__ __forceinline__ void list_token(SampleCtx<W> &x, float l, int q, bool take) {
+    SampleShared<W> &sm = x.sm;
     const uint32_t mask = __ballot_sync(0xffffffffu, take);
     if (mask == 0) return;
     const int lane = threadIdx.x & 31, lead = __ffs(mask) - 1;
     uint32_t at = 0;
     if (lane == lead) at = atomicAdd(&sm.n_list, (uint32_t)__popc(mask));
     at = __shfl_sync(0xffffffffu, at, lead) + __popc(mask & ((1u << lane) - 1u));
-    if (take && at < kSampleCap) sm.list[at] = (uint64_t)(~key_of(l)) << 32 | (x.first + (uint32_t)q);
+    if (take && at < (W * 32)) sm.list[at] = (uint64_t)(~key_of(l)) << 32 | (x.first + (uint32_t)q);
 }
 
 // The first bin at which the running count reaches k (k > 0) or the running
 // weight, as far as the histogram knows it, reaches target; the last occupied
 // bin if none does.  Sets pick_bin, pick_before (tokens before the bin),
 // pick_count (in it, 0 where none reaches it).
-__device__ void find_bin(SampleCtx &x, uint32_t k, double target) {
-    SampleShared &sm = x.sm;
+template <int W>
+__device__ void find_bin(SampleCtx<W> &x, uint32_t k, double target) {
+    SampleShared<W> &sm = x.sm;
     cg::cluster_group cl = cg::this_cluster();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     uint32_t run_c = 0;
     uint64_t run_w = 0;
     if (tid == 0) sm.pick_bin = -1, sm.pick_before = 0, sm.pick_count = 0, sm.last_bin = 0;
-    for (int b0 = 0; b0 < kSampleBins; b0 += kSampleThreads) {
+    for (int b0 = 0; b0 < kSampleBins; b0 += (W * 32)) {
         const int b = b0 + tid;
         uint32_t c = 0;
         uint64_t lows = 0;
@@ -347,7 +360,7 @@ __device__ void find_bin(SampleCtx &x, uint32_t k, double target) {
             uint32_t rc[kSampleMaxCluster], rl[kSampleMaxCluster];
 #pragma unroll
             for (int r = 0; r < kSampleMaxCluster; ++r) {           // all asked for before the first is used
-                const SampleShared *o = cl.map_shared_rank(&sm, r < x.C ? r : 0);
+                const SampleShared<W> *o = cl.map_shared_rank(&sm, r < x.C ? r : 0);
                 rc[r] = o->cnt[b];
                 rl[r] = k ? 0u : o->low[b];
             }
@@ -358,8 +371,8 @@ __device__ void find_bin(SampleCtx &x, uint32_t k, double target) {
         uint64_t w = 0;
         if (!k && c) {
             // 2^-31 of the octave's weight -> 2^-sh of the maximum's
-            const uint64_t v = (uint64_t)c * sm.start[b & 31] - (lows << 10);
-            const int e = x.weigh.sh - 31 - (b >> 5);
+            const uint64_t v = (uint64_t)c * sm.start[b & 63] - (lows << 10);
+            const int e = x.weigh.sh - 31 - (b >> 6);
             w = e >= 0 ? v << e : v >> -e;
         }
         uint32_t sc = c;
@@ -370,8 +383,8 @@ __device__ void find_bin(SampleCtx &x, uint32_t k, double target) {
         uint64_t sw = k ? 0 : warp_scan(w);
         if (lane == 31) sm.scan[warp] = sw, sm.scan_c[warp] = sc;
         __syncthreads();
-        const uint64_t aw = sm.scan[lane];
-        const uint32_t ac = sm.scan_c[lane];
+        const uint64_t aw = lane < W ? sm.scan[lane] : 0;
+        const uint32_t ac = lane < W ? sm.scan_c[lane] : 0u;
         sc += run_c + __reduce_add_sync(0xffffffffu, lane < warp ? ac : 0u);
         run_c += __reduce_add_sync(0xffffffffu, ac);
         if (!k) {
@@ -400,8 +413,8 @@ __device__ void find_bin(SampleCtx &x, uint32_t k, double target) {
 // CTA sorts (rows of a few distinct values): one exact sum over the cluster per
 // step.  K: by count (target = tokens still to take from the bin), else by
 // weight.  The cut and the weight of the bin's part before and with it.
-template <bool K>
-__device__ void bisect(SampleCtx &x, int b, double target, float &cut, uint32_t &cut_idx, uint64_t &part) {
+template <bool K, int W>
+__device__ void bisect(SampleCtx<W> &x, int b, double target, float &cut, uint32_t &cut_idx, uint64_t &part) {
     uint32_t lo = 0, hi = key_of(x.weigh.top);
     uint64_t tw, bw;
     uint32_t tc;
@@ -445,7 +458,8 @@ __device__ void bisect(SampleCtx &x, int b, double target, float &cut, uint32_t 
 }
 
 // The occupied bin next to b in direction d (b where there is none).
-__device__ int next_bin(SampleCtx &x, int b, int d) {
+template <int W>
+__device__ int next_bin(SampleCtx<W> &x, int b, int d) {
     cg::cluster_group cl = cg::this_cluster();
     for (int i = b + d; i >= 0 && i < kSampleBins; i += d)
         for (int r = 0; r < x.C; ++r)
@@ -457,10 +471,10 @@ __device__ int next_bin(SampleCtx &x, int b, int d) {
 // of them lie before the bin); else the shortest prefix that weighs `target`.
 // `sum`: the weight of the prefix; `at_bin`, `below`: the bin, and the weight
 // of this lane's tokens in the bins before it.
-template <bool K>
-__device__ void resolve(SampleCtx &x, int b, uint32_t count, uint32_t k, double target, float &cut,
+template <bool K, int W>
+__device__ void resolve(SampleCtx<W> &x, int b, uint32_t count, uint32_t k, double target, float &cut,
                         uint32_t &cut_idx, uint64_t &sum, int &at_bin, uint64_t &below) {
-    SampleShared &sm = x.sm;
+    SampleShared<W> &sm = x.sm;
     cg::cluster_group cl = cg::this_cluster();
     const int tid = threadIdx.x;
     for (;;) {
@@ -479,7 +493,7 @@ __device__ void resolve(SampleCtx &x, int b, uint32_t count, uint32_t k, double 
         uint64_t before, skip;
         uint32_t m;
         cluster_sums(x, w, c, before, m, skip);
-        if (m > (uint32_t)kSampleCap) {
+        if (m > (uint32_t)(W * 32)) {
             uint64_t part;
             double need = K ? (double)(k - count) : target - (double)before;
             if (!K) {                                               // whether the cut lies in this bin at all
@@ -520,7 +534,7 @@ __device__ void resolve(SampleCtx &x, int b, uint32_t count, uint32_t k, double 
             }
         }
         cl.sync();
-        const SampleShared *o = cl.map_shared_rank(&sm, 0);
+        const SampleShared<W> *o = cl.map_shared_rank(&sm, 0);
         const int move = o->out_move;
         cut = logit_of(o->out_key), cut_idx = o->out_idx, sum = o->out_w;
         cl.sync();
@@ -535,22 +549,22 @@ __device__ void resolve(SampleCtx &x, int b, uint32_t count, uint32_t k, double 
     }
 }
 
-__global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const SampleParams p) {
+template <int W>
+__global__ void __launch_bounds__(W * 32, W == 16 ? 2 : 1) sample_kernel(const SampleParams p) {
     extern __shared__ __align__(16) uint8_t smem_raw[];
-    SampleShared &sm = *reinterpret_cast<SampleShared *>(smem_raw);
-    float *logits = reinterpret_cast<float *>(smem_raw + sizeof(SampleShared));
+    SampleShared<W> &sm = *reinterpret_cast<SampleShared<W> *>(smem_raw);
+    float *logits = reinterpret_cast<float *>(smem_raw + sizeof(SampleShared<W>));
     cg::cluster_group cl = cg::this_cluster();
     const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     griddep_launch_dependents();
-    if (tid < 64) sm.step[tid] = c_step[tid];
-    if (tid < 32) sm.start[tid] = c_bin[tid];
-    for (int i = tid; i < kSampleBins; i += kSampleThreads) sm.cnt[i] = sm.low[i] = 0;
+    if (tid < 64) sm.step[tid] = c_step[tid], sm.start[tid] = c_bin[tid];
+    for (int i = tid; i < kSampleBins; i += (W * 32)) sm.cnt[i] = sm.low[i] = 0;
     if (tid == 0) sm.n_list = 0;
     const int64_t row = blockIdx.x / C;
-    const int64_t chunk = (int64_t)p.per * kSampleThreads, base = rank * chunk;
+    const int64_t chunk = (int64_t)p.per * (W * 32), base = rank * chunk;
     const int n = (int)max((int64_t)0, min(chunk, p.V - base));
-    for (int i = n + tid; i < (int)chunk; i += kSampleThreads) logits[i] = kNegInf;
+    for (int i = n + tid; i < (int)chunk; i += (W * 32)) logits[i] = kNegInf;
     griddep_wait();
     // ---- the row's part, and the maximum
     float top = kNegInf;
@@ -561,7 +575,7 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const SampleP
         if (vec && p.bf16) {
             done = n & ~7;
 #pragma unroll 4
-            for (int i = 8 * tid; i < done; i += 8 * kSampleThreads) {
+            for (int i = 8 * tid; i < done; i += 8 * (W * 32)) {
                 const uint4 v = __ldcs(reinterpret_cast<const uint4 *>(src + 2 * i));
                 const uint32_t w[4] = {v.x, v.y, v.z, v.w};
                 float l[8];
@@ -577,14 +591,14 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const SampleP
         } else if (vec) {
             done = n & ~3;
 #pragma unroll 8
-            for (int i = 4 * tid; i < done; i += 4 * kSampleThreads) {
+            for (int i = 4 * tid; i < done; i += 4 * (W * 32)) {
                 const float4 v = __ldcs(reinterpret_cast<const float4 *>(src + 4 * i));
                 const float4 l = make_float4(plain_logit(v.x), plain_logit(v.y), plain_logit(v.z), plain_logit(v.w));
                 top = fmaxf(fmaxf(top, fmaxf(l.x, l.y)), fmaxf(l.z, l.w));
                 *reinterpret_cast<float4 *>(logits + i) = l;
             }
         }
-        for (int i = done + tid; i < n; i += kSampleThreads) {
+        for (int i = done + tid; i < n; i += (W * 32)) {
             const float l = plain_logit(p.bf16 ? bf16_bits_to_f32(reinterpret_cast<const uint16_t *>(src)[i])
                                                : reinterpret_cast<const float *>(src)[i]);
             logits[i] = l;
@@ -599,12 +613,12 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const SampleP
     if (lane == 0) sm.red_c[0][warp] = high;
     __syncthreads();
     if (warp == 0) {
-        high = __reduce_max_sync(0xffffffffu, sm.red_c[0][lane]);
+        high = __reduce_max_sync(0xffffffffu, lane < W ? sm.red_c[0][lane] : 0u);
         if (lane == 0) sm.cta_c[0] = high;
     }
     cl.sync();
     top = logit_of(__reduce_max_sync(0xffffffffu, lane < C ? cl.map_shared_rank(&sm, lane)->cta_c[0] : 0u));
-    SampleCtx x = {sm, logits + tid * p.per, p.per, C, rank, (uint32_t)(base + tid * p.per), 1, {}};
+    SampleCtx<W> x = {sm, logits + tid * p.per, p.per, C, rank, (uint32_t)(base + tid * p.per), 1, {}};
     Weigher &weigh = x.weigh;
     const double inv = 1.4426950408889634074 / (double)temp;
     weigh.top = top;
@@ -624,7 +638,7 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const SampleP
         if (lane == 0) sm.red_c[1][warp] = at;
         __syncthreads();
         if (warp == 0) {
-            at = __reduce_min_sync(0xffffffffu, sm.red_c[1][lane]);
+            at = __reduce_min_sync(0xffffffffu, lane < W ? sm.red_c[1][lane] : 0xFFFFFFFFu);
             if (lane == 0) sm.cta_c[1] = at;
         }
         cl.sync();
@@ -646,19 +660,18 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const SampleP
         // ---- the histogram, and the row's whole weight where top-p needs it
         uint64_t w = 0, total, skip;
         for_logits(x, [&](float l, int) {
-            float d, y;
+            float d, y, kf;
             int k;
-            const bool ok = weigh.place(l, d, y, k);
-            const int b = k >> 1;
+            const bool ok = weigh.place(l, d, y, kf, k);
             if (!by_p) {
-                if (ok) atomicAdd(&sm.cnt[b], 1u);
+                if (ok) atomicAdd(&sm.cnt[k], 1u);
                 return;
             }
-            const uint32_t m = weigh.mantissa(l, d, y, k);
+            const uint32_t m = weigh.mantissa(l, d, y, kf, k);
             if (!by_k) w = weigh.add(w, ok ? m : 0u, k);
             if (ok) {
-                atomicAdd(&sm.cnt[b], 1u);
-                atomicAdd(&sm.low[b], (uint32_t)max((int)(sm.start[b & 31] - m), 0) >> 10);
+                atomicAdd(&sm.cnt[k], 1u);
+                atomicAdd(&sm.low[k], (uint32_t)max((int)(sm.start[k & 63] - m), 0) >> 10);
             }
         });
         uint32_t c;
@@ -666,7 +679,7 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const SampleP
         find_bin(x, by_k ? (uint32_t)top_k : 0u, fmax((double)top_p * (double)total, 1.0));
         int b = sm.pick_bin;
         uint32_t before = sm.pick_before, count = sm.pick_count;
-        if (before + count <= (uint32_t)kSampleCap && b < kSampleBins - 1) {
+        if (before + count <= (uint32_t)(W * 32) && b < kSampleBins - 1) {
             // ---- all that can be kept on one CTA, one token per thread
             for_logits(x, [&](float l, int q) { list_token(x, l, q, weigh.bin(l) <= b); });
             cl.sync();
@@ -675,7 +688,7 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const SampleP
                 uint64_t token, listed, sum;
                 const int m = gather(x, token);
                 const int top_n = by_k ? min(top_k, m) : m;         // of the order
-                if (m <= kCountCap) {
+                if (m <= W * 4) {                                   // eight threads per token
                     if (tid < m) {
                         sm.all[tid] = token;
                         sm.list[tid] = weigh(logit_of(~(uint32_t)(token >> 32)));
@@ -788,6 +801,38 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const SampleP
     cl.sync();                                        // no CTA leaves while another reads its shared memory
 }
 
+template <int W>
+static int sample_launch(SampleParams p, int64_t B, int C, cudaStream_t st) {
+    p.per = (int)((p.V + (int64_t)C * W * 32 - 1) / ((int64_t)C * W * 32)) | 1;
+    const size_t smem = sizeof(SampleShared<W>) + (size_t)p.per * W * 32 * 4;
+    static std::atomic<uint64_t> raised{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (e == cudaSuccess && !(raised.load(std::memory_order_relaxed) & bit)) {
+        e = cudaFuncSetAttribute(sample_kernel<W>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+        if (e == cudaSuccess) raised.fetch_or(bit, std::memory_order_relaxed);
+    }
+    if (e != cudaSuccess) return set_error(BF16X_ERR_CUDA, "bf16x_sample: shared memory: %s", cudaGetErrorString(e));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(B * C));
+    cfg.blockDim = dim3(W * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)C;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    e = cudaLaunchKernelEx(&cfg, sample_kernel<W>, p);
+    if (e != cudaSuccess) return set_error(BF16X_ERR_CUDA, "bf16x_sample: launch: %s", cudaGetErrorString(e));
+    return check_launch("sample_kernel");
+}
+
 }  // namespace bf16x
 
 using namespace bf16x;
@@ -804,35 +849,17 @@ extern "C" int bf16x_sample(const void *logits, int dtype, int64_t ld, int64_t B
     if (B > (1 << 24)) return set_error(BF16X_ERR_UNSUPPORTED, "bf16x_sample: too many rows");
     if (B == 0) return BF16X_OK;
     if (!logits || !u || !tokens) return set_error(BF16X_ERR_INVALID, "bf16x_sample: null pointer");
+    // CTAs per row: as the row's size asks, and more while the GPU has room
     int C = 1;
     while (C < kSampleMaxCluster && (B * C < 2 * 148 || V > (int64_t)C * kSampleMaxKeys)) C *= 2;
     SampleParams p = {};
     p.logits = logits, p.ld = ld, p.V = V, p.bf16 = dtype == BF16X_DTYPE_BF16;
-    p.per = (int)((V + (int64_t)C * kSampleThreads - 1) / ((int64_t)C * kSampleThreads)) | 1;
     int lg = 0;
     while (((int64_t)1 << lg) < V) ++lg;
-    p.sh = std::min(47, 62 - lg);                     // 16-bit limbs hold weights below 2^48
+    p.sh = std::min(47, 62 - lg);                     // a row's sum fits 64 bits
     p.u = u, p.temperature = temperature, p.top_p = top_p, p.min_p = min_p, p.top_k = top_k;
     p.temperature0 = temperature0, p.top_p0 = top_p0, p.min_p0 = min_p0, p.top_k0 = top_k0;
     p.tokens = tokens;
-    const size_t smem = sizeof(SampleShared) + (size_t)p.per * kSampleThreads * 4;
-    cudaError_t e = cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return set_error(BF16X_ERR_CUDA, "bf16x_sample: shared memory: %s", cudaGetErrorString(e));
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(B * C));
-    cfg.blockDim = dim3(kSampleThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = (cudaStream_t)stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = (unsigned)C;
-    attr[1].val.clusterDim.y = 1;
-    attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    e = cudaLaunchKernelEx(&cfg, sample_kernel, p);
-    if (e != cudaSuccess) return set_error(BF16X_ERR_CUDA, "bf16x_sample: launch: %s", cudaGetErrorString(e));
-    return check_launch("sample_kernel");
+    // one CTA per SM: 32 warps; else two of 16, which fill each other's waits
+    return B * C <= 148 ? sample_launch<32>(p, B, C, (cudaStream_t)stream) : sample_launch<16>(p, B, C, (cudaStream_t)stream);
 }
