@@ -143,6 +143,20 @@ def stream_of(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
+def call_on(index: int, name: str, *args) -> None:
+    """An entry point on CUDA device ``index`` and that device's current
+    stream (appended to the arguments): the short way for calls of a few
+    microseconds, without stream and device objects."""
+    fn = getattr(_lib or lib(), name)
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc, name)
+
+
 def require_cuda(t: torch.Tensor, name: str) -> None:
     if not t.is_cuda:
         raise Bf16xError(f"{name} must be a CUDA tensor (bfloat16x_b200 runs on the GPU only)")

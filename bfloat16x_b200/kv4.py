@@ -20,6 +20,8 @@ and reported by ``_lib.check_device_status``.
 """
 from __future__ import annotations
 
+from functools import lru_cache
+
 import torch
 
 from . import _lib
@@ -38,13 +40,18 @@ def kv4_blocks(batch: int, max_seq: int, kv_heads: int, head_dim: int, device=No
                        device=device)
 
 
+@lru_cache(maxsize=4096)
+def _workspace_bytes(batch: int, tokens: int, heads: int, kv_heads: int, head_dim: int, max_seq: int) -> int:
+    return int(_lib.lib().bf16x_kv4_attend_workspace_bytes(batch, tokens, heads, kv_heads, head_dim, max_seq))
+
+
 class Kv4Cache:
     """The 4-bit cache of one layer over its ``blocks`` (``kv4_blocks``, or a slice of a larger tensor)."""
 
-    __slots__ = ("blocks", "batch", "kv_heads", "max_seq", "head_dim")
+    __slots__ = ("blocks", "batch", "kv_heads", "max_seq", "head_dim", "device", "_index")
 
     def __init__(self, blocks: torch.Tensor, max_seq: int | None = None):
-        if blocks.dtype != torch.uint8 or blocks.dim() != 4 or not blocks.is_contiguous():
+        if blocks.dtype is not torch.uint8 or blocks.dim() != 4 or not blocks.is_contiguous():
             raise ValueError("blocks must be a contiguous uint8 tensor [batch, kv_heads, blocks, 20 * head_dim]")
         self.blocks = blocks
         self.batch, self.kv_heads, n, size = blocks.shape
@@ -54,6 +61,8 @@ class Kv4Cache:
         self.max_seq = n * BLOCK if max_seq is None else int(max_seq)
         if not (n - 1) * BLOCK < self.max_seq <= n * BLOCK:
             raise ValueError(f"{n} blocks hold {(n - 1) * BLOCK + 1}..{n * BLOCK} positions, not {self.max_seq}")
+        self.device = blocks.device
+        self._index = self.device.index
 
     @classmethod
     def empty(cls, batch: int, max_seq: int, kv_heads: int, head_dim: int, device=None) -> "Kv4Cache":
@@ -64,30 +73,20 @@ class Kv4Cache:
 
     def _pos(self, pos0: torch.Tensor) -> int:
         """The stride of the positions of the sequences (0: one for all)."""
-        if pos0.dtype != torch.int64 or pos0.device != self.blocks.device:
+        if pos0.dtype is not torch.int64 or pos0.device != self.device:
             raise ValueError("pos0 must be an int64 tensor on the cache's device")
-        n = pos0.numel()
-        if n == 1:
+        if pos0.numel() == 1:
             return 0
-        if pos0.dim() != 1 or n != self.batch:
+        if pos0.dim() != 1 or pos0.shape[0] != self.batch:
             raise ValueError(f"pos0 must hold one position, or one for each of {self.batch} sequences")
         return pos0.stride(0)
 
     def _check(self, x: torch.Tensor, name: str) -> None:
-        _lib.require_cuda(x, name)
-        if x.device != self.blocks.device:
-            raise ValueError(f"{name} must be on the cache's device")
-        if x.dtype != torch.bfloat16:
+        if x.dtype is not torch.bfloat16:
             raise ValueError(f"{name} must be bf16")
-
-    def _call(self, name: str, *args) -> None:
-        """The entry point on the cache's device and its current stream."""
-        dev = self.blocks.device
-        if torch.cuda.current_device() == dev.index:
-            _lib.check(getattr(_lib.lib(), name)(*args, torch.cuda.current_stream().cuda_stream), name)
-        else:
-            with torch.cuda.device(dev):
-                _lib.check(getattr(_lib.lib(), name)(*args, torch.cuda.current_stream().cuda_stream), name)
+        if x.device != self.device or self._index is None:
+            _lib.require_cuda(x, name)
+            raise ValueError(f"{name} must be on the cache's device")
 
     def append(self, qkv: torch.Tensor, pos0: torch.Tensor, heads: int, cos: torch.Tensor | None = None,
                sin: torch.Tensor | None = None) -> torch.Tensor:
@@ -102,19 +101,22 @@ class Kv4Cache:
             raise ValueError(f"qkv must be [{B}, T, (heads + {2 * KV}) * {D}], got {tuple(qkv.shape)} for {heads} heads")
         if (cos is None) != (sin is None):
             raise ValueError("cos and sin go together")
+        c = s = None
         if cos is not None:
             for a in (cos, sin):
-                if (a.dtype != torch.float32 or a.dim() != 2 or a.shape[1] != D // 2 or a.shape[0] < self.max_seq
-                        or not a.is_contiguous() or a.device != qkv.device):
+                if (a.dtype is not torch.float32 or a.dim() != 2 or a.shape[1] != D // 2 or a.shape[0] < self.max_seq
+                        or not a.is_contiguous() or a.device != self.device):
                     raise ValueError(f"cos and sin must be contiguous fp32 [>= {self.max_seq}, {D // 2}] on the cache's device")
+            c, s = cos.data_ptr(), sin.data_ptr()
         stride = self._pos(pos0)
-        if qkv.stride(2) != 1 or qkv.stride(0) % 8 or qkv.stride(1) % 8 or qkv.data_ptr() % 16:
+        ld_b, ld_t, one = qkv.stride()
+        if one != 1 or (ld_b | ld_t) % 8 or qkv.data_ptr() % 16:
             qkv = qkv.clone(memory_format=torch.contiguous_format)
+            ld_b, ld_t, _ = qkv.stride()
         T = qkv.shape[1]
-        q = torch.empty((B, T, heads, D), dtype=torch.bfloat16, device=qkv.device)
-        self._call("bf16x_kv4_append", qkv.data_ptr(), qkv.stride(0), qkv.stride(1), B, T, heads, KV, D,
-                   pos0.data_ptr(), stride, _lib.ptr(cos), _lib.ptr(sin), q.data_ptr(), self.blocks.data_ptr(),
-                   self.max_seq)
+        q = torch.empty((B, T, heads, D), dtype=torch.bfloat16, device=self.device)
+        _lib.call_on(self._index, "bf16x_kv4_append", qkv.data_ptr(), ld_b, ld_t, B, T, heads, KV, D, pos0.data_ptr(),
+                     stride, c, s, q.data_ptr(), self.blocks.data_ptr(), self.max_seq)
         return q
 
     def read(self, pos0: torch.Tensor, count: int) -> tuple[torch.Tensor, torch.Tensor]:
@@ -125,10 +127,10 @@ class Kv4Cache:
             raise ValueError("count must not be negative")
         stride = self._pos(pos0)
         shape = (self.batch, count, self.kv_heads, self.head_dim)
-        k = torch.empty(shape, dtype=torch.bfloat16, device=self.blocks.device)
-        v = torch.empty_like(k)
-        self._call("bf16x_kv4_read", self.blocks.data_ptr(), self.max_seq, self.batch, count, self.kv_heads,
-                   self.head_dim, pos0.data_ptr(), stride, k.data_ptr(), v.data_ptr())
+        k = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
+        v = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
+        _lib.call_on(self._index, "bf16x_kv4_read", self.blocks.data_ptr(), self.max_seq, self.batch, count,
+                     self.kv_heads, self.head_dim, pos0.data_ptr(), stride, k.data_ptr(), v.data_ptr())
         return k, v
 
     def attend(self, q: torch.Tensor, pos0: torch.Tensor, scale: float | None = None,
@@ -138,26 +140,27 @@ class Kv4Cache:
         sees positions 0 .. pos0[b] + t.  scale: default head_dim ** -0.5.
         Returns bf16 like q (zeros for a row that sees nothing)."""
         self._check(q, "q")
-        B, KV, D = self.batch, self.kv_heads, self.head_dim
-        if q.dim() != 4 or q.shape[0] != B or q.shape[3] != D or q.shape[2] % KV or q.shape[2] == 0:
-            raise ValueError(f"q must be [{B}, T, a multiple of {KV}, {D}], got {tuple(q.shape)}")
+        KV, D = self.kv_heads, self.head_dim
+        shape = q.shape
+        if len(shape) != 4 or shape[0] != self.batch or shape[3] != D or shape[2] % KV or shape[2] == 0:
+            raise ValueError(f"q must be [{self.batch}, T, a multiple of {KV}, {D}], got {tuple(shape)}")
         stride = self._pos(pos0)
-        s = q.stride()
-        if s[3] != 1 or s[0] % 8 or s[1] % 8 or s[2] % 8 or q.data_ptr() % 16:
+        B, T, H, _ = shape
+        s0, s1, s2, one = q.stride()
+        if one != 1 or (s0 | s1 | s2) % 8 or q.data_ptr() % 16:
             q = q.clone(memory_format=torch.contiguous_format)
-            s = q.stride()
-        T, H = q.shape[1], q.shape[2]
+            s0, s1, s2, _ = q.stride()
         if out is None:
-            out = torch.empty((B, T, H, D), dtype=torch.bfloat16, device=q.device)
-        elif (out.shape != q.shape or out.dtype != torch.bfloat16 or not out.is_contiguous() or out.device != q.device
-              or out.data_ptr() % 16):
+            out = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
+        elif (out.shape != shape or out.dtype is not torch.bfloat16 or not out.is_contiguous()
+              or out.device != self.device or out.data_ptr() % 16):
             raise ValueError("out must be a contiguous, 16-byte aligned bf16 tensor of q's shape")
         # a workspace of its own for every call (and every captured graph): calls may overlap on several streams
-        need = _lib.lib().bf16x_kv4_attend_workspace_bytes(B, T, H, KV, D, self.max_seq)
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-        self._call("bf16x_kv4_attend", q.data_ptr(), s[0], s[1], s[2], B, T, H, KV, D, pos0.data_ptr(), stride,
-                   D ** -0.5 if scale is None else float(scale), self.blocks.data_ptr(), self.max_seq, out.data_ptr(),
-                   _lib.ptr(ws), need)
+        need = _workspace_bytes(B, T, H, KV, D, self.max_seq)
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        _lib.call_on(self._index, "bf16x_kv4_attend", q.data_ptr(), s0, s1, s2, B, T, H, KV, D, pos0.data_ptr(), stride,
+                     D ** -0.5 if scale is None else float(scale), self.blocks.data_ptr(), self.max_seq, out.data_ptr(),
+                     None if ws is None else ws.data_ptr(), need)
         return out
 
 

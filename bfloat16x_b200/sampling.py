@@ -70,13 +70,9 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     m, m0 = _setting(min_p, "min_p", torch.float32, logits)
     if B and (logits.stride(1) != 1 or logits.stride(0) < V):
         logits = logits.clone(memory_format=torch.contiguous_format)
-    args = (logits.data_ptr(), _DT[logits.dtype], max(logits.stride(0), V), B, V, u.data_ptr(), t, float(t0), k,
-            max(0, min(int(k0), 0x7FFFFFFF)), p, float(p0), m, float(m0), out.data_ptr())
-    if torch.cuda.current_device() == logits.device.index:
-        _lib.check(_lib.lib().bf16x_sample(*args, torch.cuda.current_stream().cuda_stream), "bf16x_sample")
-    else:
-        with torch.cuda.device(logits.device):
-            _lib.check(_lib.lib().bf16x_sample(*args, torch.cuda.current_stream().cuda_stream), "bf16x_sample")
+    _lib.call_on(logits.device.index, "bf16x_sample", logits.data_ptr(), _DT[logits.dtype], max(logits.stride(0), V), B, V,
+                 u.data_ptr(), t, float(t0), k, max(0, min(int(k0), 0x7FFFFFFF)), p, float(p0), m, float(m0),
+                 out.data_ptr())
     return out
 
 
