@@ -44,11 +44,23 @@ __device__ __forceinline__ void kv4_quantize8(const float (&y)[8], float &d, flo
         m = 0.f;
     } else if (d == 0.f) {                                        // a constant group: m, with any d; one near m's
         d = __uint_as_float(__float_as_uint(fabsf(lo) * 0x1p-13f) & 0xFFFF0000u);      // own scale suits the reader
-    } else {
+    } else if (d < 0x1p-100f || d > 0x1p100f) {                   // 1/d may leave fp32
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float c = rintf(__fdiv_rn(__fsub_rn(y[i], lo), d));
             codes |= (uint32_t)fminf(fmaxf(c, 0.f), 15.f) << (4 * i);
+        }
+    } else {
+        // the nearest whole number to a / d without a division: n from a * (1/d),
+        // which may miss by one, and a - n d, which is exact (n d has 12 bits),
+        // against d / 2; halves go to the even n.  a / d <= 15, so n is a code.
+        const float inv = __frcp_rn(d), half = 0.5f * d, more = __uint_as_float(__float_as_uint(half) + 1u);
+#pragma unroll
+        for (int i = 7; i >= 0; --i) {
+            const float a = __fsub_rn(y[i], lo), t = __fmaf_rn(a, inv, 12582912.f), rest = __fmaf_rn(-__fsub_rn(t, 12582912.f), d, a);
+            uint32_t n = __float_as_uint(t) & 0x1Fu;
+            if (fabsf(rest) >= (n & 1u ? half : more)) n += rest > 0.f ? 1u : ~0u;
+            codes = codes * 16u + n;
         }
     }
 }
@@ -56,7 +68,6 @@ __device__ __forceinline__ void kv4_quantize8(const float (&y)[8], float &d, flo
 struct Kv4AppendParams {
     const uint16_t *qkv;
     int64_t ld_b, ld_t;                 // elements
-    int64_t tokens;
     int T, H, KV, pos_stride;
     const int64_t *pos0;
     const float *cos_t, *sin_t;         // NULL: no rotation
@@ -71,75 +82,75 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4AppendParams p
     constexpr int LPH = D / 8;                                      // lanes per head
     griddep_launch_dependents();
     griddep_wait();
-    const int heads = p.H + 2 * p.KV;
-    const int64_t unit_raw = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPH;
-    const int64_t n_units = p.tokens * heads;
-    const bool live = unit_raw < n_units;                           // the warp stays whole for the shuffles
-    const int64_t unit = live ? unit_raw : n_units - 1;
-    const int l = threadIdx.x % LPH;
-    const int64_t tok = unit / heads;
-    const int head = (int)(unit - tok * heads);
-    const int64_t b = tok / p.T;
-    const int t = (int)(tok - b * p.T);
-    const int64_t pos = p.pos0[b * p.pos_stride] + t;
-    const bool inside = pos >= 0 && pos < p.max_seq;
-    if (live && pos >= p.max_seq && head == 0 && l == 0) atomicOr(&g_status, kErrBadIndex);
-    const uint4 raw = *reinterpret_cast<const uint4 *>(p.qkv + b * p.ld_b + t * p.ld_t + (int64_t)head * D + 8 * l);
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-    float y[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        y[2 * i] = bf_lo(w[i]);
-        y[2 * i + 1] = bf_hi(w[i]);
-    }
-    if (head < p.H + p.KV && p.cos_t != nullptr && inside) {
+    // a token per CTA: its threads keep their channels' angles and go over the heads
+    constexpr int STEP = 256 / LPH;
+    const int heads = p.H + 2 * p.KV, l = threadIdx.x % LPH;
+    const int64_t tok = blockIdx.x;
+    const uint32_t b = blockIdx.x / (uint32_t)p.T, t = blockIdx.x - b * (uint32_t)p.T;
+    const int64_t pos = p.pos0[(int64_t)b * p.pos_stride] + t;
+    const bool inside = pos >= 0 && pos < p.max_seq, turn = p.cos_t != nullptr && inside;
+    if (pos >= p.max_seq && threadIdx.x == 0) atomicOr(&g_status, kErrBadIndex);
+    const uint16_t *src = p.qkv + (int64_t)b * p.ld_b + (int64_t)t * p.ld_t + 8 * l;
+    int head = (int)threadIdx.x / LPH;
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    if (head < heads) raw = *reinterpret_cast<const uint4 *>(src + head * D);
+    float c[4] = {}, s[4] = {};
+    if (turn) {
         const float4 c4 = *reinterpret_cast<const float4 *>(p.cos_t + pos * (D / 2) + 4 * l);
         const float4 s4 = *reinterpret_cast<const float4 *>(p.sin_t + pos * (D / 2) + 4 * l);
-        const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
+        c[0] = c4.x, c[1] = c4.y, c[2] = c4.z, c[3] = c4.w;
+        s[0] = s4.x, s[1] = s4.y, s[2] = s4.z, s[3] = s4.w;
+    }
+    const int r = (int)pos & 15, grp = l / 4, t4 = l % 4;
+    uint8_t *blocks = p.blocks + ((int64_t)b * p.KV * p.nblk + (pos >> 4)) * L::kBytes;        // of kv head 0; used if inside
+    uint16_t *q_out = p.q_out + tok * p.H * D + 8 * l;
+    for (int base = 0; base < heads; base += STEP, head += STEP) {  // whole warps: the quantiser shuffles
+        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+        if (head + STEP < heads) raw = *reinterpret_cast<const uint4 *>(src + (head + STEP) * D);
+        const bool live = head < heads;
+        uint32_t o[4] = {w[0], w[1], w[2], w[3]};
+        if (turn && head < p.H + p.KV) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x = bf_lo(w[i]), y = bf_hi(w[i]);
+                o[i] = pack_bf16x2(__fsub_rn(__fmul_rn(x, c[i]), __fmul_rn(y, s[i])),
+                                   __fadd_rn(__fmul_rn(x, s[i]), __fmul_rn(y, c[i])));
+            }
+        }
+        if (live && head < p.H)                                     // a position outside the cache: zeros
+            *reinterpret_cast<uint4 *>(q_out + head * D) = inside ? make_uint4(o[0], o[1], o[2], o[3]) : make_uint4(0, 0, 0, 0);
+        if (!__any_sync(0xffffffffu, live && head >= p.H)) continue;
+        float y[8], d, m;
+        uint32_t codes;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float a = __fsub_rn(__fmul_rn(y[2 * i], c[i]), __fmul_rn(y[2 * i + 1], s[i]));
-            const float e = __fadd_rn(__fmul_rn(y[2 * i], s[i]), __fmul_rn(y[2 * i + 1], c[i]));
-            const uint32_t r = pack_bf16x2(a, e);
-            y[2 * i] = bf_lo(r);
-            y[2 * i + 1] = bf_hi(r);
+            y[2 * i] = bf_lo(o[i]);
+            y[2 * i + 1] = bf_hi(o[i]);
         }
-    }
-    float d, m;
-    uint32_t codes;
-    kv4_quantize8<D>(y, d, m, codes);                               // shuffles: every lane takes part
-    if (!live) return;
-    if (head < p.H) {
-        uint4 o = make_uint4(0, 0, 0, 0);                           // a position outside the cache: zeros
-        if (inside)
-            o = make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]),
-                           pack_bf16x2(y[6], y[7]));
-        *reinterpret_cast<uint4 *>(p.q_out + (tok * p.H + head) * D + 8 * l) = o;
-        return;
-    }
-    if (!inside) return;
-    const bool is_v = head >= p.H + p.KV;
-    const int kvh = head - p.H - (is_v ? p.KV : 0);
-    uint8_t *blk = p.blocks + ((b * p.KV + kvh) * p.nblk + pos / kKvBlock) * L::kBytes;
-    const int r = (int)(pos % kKvBlock), grp = l / 4, t4 = l % 4;
-    const uint16_t db = (uint16_t)(__float_as_uint(d) >> 16), mb = (uint16_t)(__float_as_uint(m) >> 16);
-    if (!is_v) {
-        *reinterpret_cast<uint32_t *>(blk + ((r * 4 + t4) * L::NG + grp) * 4) = codes;
-        if (t4 == 0) {
-            *reinterpret_cast<uint16_t *>(blk + L::kKd + (r * L::NG + grp) * 2) = db;
-            *reinterpret_cast<uint16_t *>(blk + L::kKm + (r * L::NG + grp) * 2) = mb;
-        }
-    } else {
-        const int pp = r / 8, tt = (r % 8) / 2, h = r % 2;
+        kv4_quantize8<D>(y, d, m, codes);
+        if (!live || head < p.H || !inside) continue;
+        const bool is_v = head >= p.H + p.KV;
+        const int kvh = head - p.H - (is_v ? p.KV : 0);
+        uint8_t *blk = blocks + (int64_t)kvh * p.nblk * L::kBytes;
+        const uint16_t db = (uint16_t)(__float_as_uint(d) >> 16), mb = (uint16_t)(__float_as_uint(m) >> 16);
+        if (!is_v) {
+            *reinterpret_cast<uint32_t *>(blk + ((r * 4 + t4) * L::NG + grp) * 4) = codes;
+            if (t4 == 0) {
+                *reinterpret_cast<uint16_t *>(blk + L::kKd + (r * L::NG + grp) * 2) = db;
+                *reinterpret_cast<uint16_t *>(blk + L::kKm + (r * L::NG + grp) * 2) = mb;
+            }
+        } else {
+            const int pp = r / 8, tt = (r % 8) / 2, h = r % 2;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int g = 2 * t4 + i;                               // channels 32 grp + 4 g ..
-            *reinterpret_cast<uint16_t *>(blk + L::kV + (((pp * 8 + g) * 4 + tt) * L::NG + grp) * 4 + 2 * h) =
-                (uint16_t)(codes >> (16 * i));
-        }
-        if (t4 == 0) {
-            *reinterpret_cast<uint16_t *>(blk + L::kVd + (r * L::NG + grp) * 2) = db;
-            *reinterpret_cast<uint16_t *>(blk + L::kVm + (((r / 2) * L::NG + grp) * 2 + h) * 2) = mb;
+            for (int i = 0; i < 2; ++i) {
+                const int g = 2 * t4 + i;                           // channels 32 grp + 4 g ..
+                *reinterpret_cast<uint16_t *>(blk + L::kV + (((pp * 8 + g) * 4 + tt) * L::NG + grp) * 4 + 2 * h) =
+                    (uint16_t)(codes >> (16 * i));
+            }
+            if (t4 == 0) {
+                *reinterpret_cast<uint16_t *>(blk + L::kVd + (r * L::NG + grp) * 2) = db;
+                *reinterpret_cast<uint16_t *>(blk + L::kVm + (((r / 2) * L::NG + grp) * 2 + h) * 2) = mb;
+            }
         }
     }
 }
@@ -149,7 +160,7 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4AppendParams p
 // fp32 rounded to bf16; a position outside the cache reads as zeros.
 struct Kv4ReadParams {
     const uint8_t *blocks;
-    int64_t max_seq, nblk, tokens;
+    int64_t max_seq, nblk;
     int T, KV, pos_stride;
     const int64_t *pos0;
     uint16_t *k_out, *v_out;
@@ -161,20 +172,17 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
     constexpr int LPH = D / 8;
     griddep_launch_dependents();
     griddep_wait();
-    const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPH;
-    const int l = threadIdx.x % LPH;
-    if (unit >= p.tokens * p.KV * 2) return;
-    const int64_t row = unit >> 1;                                  // token * KV + head
-    const bool is_v = unit & 1;
-    const int64_t tok = row / p.KV;
-    const int kvh = (int)(row - tok * p.KV);
-    const int64_t b = tok / p.T;
-    const int64_t pos = p.pos0[b * p.pos_stride] + (tok - b * p.T);
+    const int part = (int)(blockIdx.y * (256 / LPH) + threadIdx.x / LPH), l = threadIdx.x % LPH;        // head, K or V
+    if (part >= 2 * p.KV) return;
+    const int kvh = part >> 1;
+    const bool is_v = part & 1;
+    const uint32_t b = blockIdx.x / (uint32_t)p.T, t = blockIdx.x - b * (uint32_t)p.T;
+    const int64_t row = (int64_t)blockIdx.x * p.KV + kvh, pos = p.pos0[(int64_t)b * p.pos_stride] + t;
     uint4 o = make_uint4(0, 0, 0, 0);
     if (pos >= p.max_seq && l == 0) atomicOr(&g_status, kErrBadIndex);
     if (pos >= 0 && pos < p.max_seq) {
-        const uint8_t *blk = p.blocks + ((b * p.KV + kvh) * p.nblk + pos / kKvBlock) * L::kBytes;
-        const int r = (int)(pos % kKvBlock), grp = l / 4, t4 = l % 4;
+        const uint8_t *blk = p.blocks + (((int64_t)b * p.KV + kvh) * p.nblk + (pos >> 4)) * L::kBytes;
+        const int r = (int)pos & 15, grp = l / 4, t4 = l % 4;
         uint32_t codes;
         uint16_t db, mb;
         if (!is_v) {
@@ -937,13 +945,13 @@ extern "C" int bf16x_kv4_append(const uint16_t *qkv, int64_t ld_b, int64_t ld_t,
     if (((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)blocks | (uintptr_t)cos_t | (uintptr_t)sin_t) & 15 ||
         (ld_b | ld_t) % 8)
         return set_error(BF16X_ERR_INVALID, "bf16x_kv4_append: pointers must be 16-byte aligned, strides multiples of 8");
-    Kv4AppendParams p = {qkv, ld_b, ld_t, B * T, (int)T, (int)H, (int)KV, pos_stride, pos0, cos_t, sin_t, q_out, blocks,
+    Kv4AppendParams p = {qkv, ld_b, ld_t, (int)T, (int)H, (int)KV, pos_stride, pos0, cos_t, sin_t, q_out, blocks,
                          max_seq, (max_seq + kKvBlock - 1) / kKvBlock};
-    const int64_t threads = B * T * (H + 2 * KV) * (D / 8), grid = (threads + 255) / 256;
-    if (grid > 0x7fffffffLL) return set_error(BF16X_ERR_UNSUPPORTED, "bf16x_kv4_append: too many tokens");
-    return D == 64 ? launch_kv4<kv4_append_kernel<64>>(dim3((unsigned)grid), 256, 0, (cudaStream_t)stream,
+    if (B * T > 0x7fffffffLL) return set_error(BF16X_ERR_UNSUPPORTED, "bf16x_kv4_append: too many tokens");
+    const dim3 grid((unsigned)(B * T));
+    return D == 64 ? launch_kv4<kv4_append_kernel<64>>(grid, 256, 0, (cudaStream_t)stream,
                                 "kv4_append_kernel", p)
-                   : launch_kv4<kv4_append_kernel<128>>(dim3((unsigned)grid), 256, 0, (cudaStream_t)stream,
+                   : launch_kv4<kv4_append_kernel<128>>(grid, 256, 0, (cudaStream_t)stream,
                                 "kv4_append_kernel", p);
 }
 
@@ -955,13 +963,13 @@ extern "C" int bf16x_kv4_read(const uint8_t *blocks, int64_t max_seq, int64_t B,
     if (!blocks || !pos0 || !k_out || !v_out) return set_error(BF16X_ERR_INVALID, "bf16x_kv4_read: null pointer");
     if (((uintptr_t)blocks | (uintptr_t)k_out | (uintptr_t)v_out) & 15)
         return set_error(BF16X_ERR_INVALID, "bf16x_kv4_read: pointers must be 16-byte aligned");
-    Kv4ReadParams p = {blocks, max_seq, (max_seq + kKvBlock - 1) / kKvBlock, B * T, (int)T, (int)KV, pos_stride, pos0,
+    Kv4ReadParams p = {blocks, max_seq, (max_seq + kKvBlock - 1) / kKvBlock, (int)T, (int)KV, pos_stride, pos0,
                        k_out, v_out};
-    const int64_t threads = B * T * 2 * KV * (D / 8), grid = (threads + 255) / 256;
-    if (grid > 0x7fffffffLL) return set_error(BF16X_ERR_UNSUPPORTED, "bf16x_kv4_read: too many tokens");
-    return D == 64 ? launch_kv4<kv4_read_kernel<64>>(dim3((unsigned)grid), 256, 0, (cudaStream_t)stream,
+    if (B * T > 0x7fffffffLL) return set_error(BF16X_ERR_UNSUPPORTED, "bf16x_kv4_read: too many tokens");
+    const dim3 grid((unsigned)(B * T), (unsigned)((2 * KV * (D / 8) + 255) / 256));
+    return D == 64 ? launch_kv4<kv4_read_kernel<64>>(grid, 256, 0, (cudaStream_t)stream,
                                 "kv4_read_kernel", p)
-                   : launch_kv4<kv4_read_kernel<128>>(dim3((unsigned)grid), 256, 0, (cudaStream_t)stream,
+                   : launch_kv4<kv4_read_kernel<128>>(grid, 256, 0, (cudaStream_t)stream,
                                 "kv4_read_kernel", p);
 }
 
