@@ -1,17 +1,23 @@
 // bf16x_kv4_prefill.cu -- attention of many query rows over the 4-bit cache
 // (prompts, chunks of prompts) on the 5th-generation tensor cores.
 //
-// Rows r = t * G + h of one kv head, 256 per CTA (two groups of 128), walk
+// Rows r = t * G + h of one kv head, 256 per unit (two groups of 128), walk
 // over the cache in tiles of 128 positions:
 //   S[128][128] = Q K^T,  P = 2^(S c - M),  O[128][D] += P V
-// with S, P and O in tensor memory (P takes the place of S) and Q, K and V^T as
-// fp16 operands in shared memory.  17 warps:
+// with S, P and O in tensor memory (all 512 columns at D = 128: P takes the
+// place of S) and Q, K and V^T as fp16 operands in shared memory.  13 warps:
 //   0..3, 4..7  one softmax group per 128 rows, one thread per row: scores out
 //               of tensor memory, maximum, 2^x, P back as fp16
-//   8..15       K and V of the next tile from 4 bits to fp16 (loaded one tile
-//               ahead into registers), into two stages each
-//   16          issues the MMAs
+//   8..11       K and V from 4 bits to fp16 (loaded one tile ahead into
+//               registers), one thread per position, into two stages each
+//   12          issues the MMAs
 // While one group works on its scores, the tensor cores work for the other.
+// The softmax goes over tensor memory twice in short loops: holding a row's 128
+// scores in registers took 700 cycles more per tile, as its straight code does
+// not stay in an instruction cache that three roles share; steps of 64 with two
+// S per group took a third more, since an MMA of 64 columns takes as long as
+// one of 128.  A CTA goes over several units (the longest first), so that the
+// next one's K and V are ready when a unit ends.
 //
 // fp16 operands hold any scale: a row of Q is scaled by a power of two into
 // [2^13, 2^14), exact; the values of a tile by 2^-dk (K) and 2^-dv (V) to at
@@ -40,9 +46,9 @@
 
 namespace bf16x {
 
-constexpr int kPreRows = 256;                         // rows per CTA
+constexpr int kPreRows = 256;                         // rows per unit
 constexpr int kPreKeys = 128;                         // positions per tile
-constexpr int kPreThreads = 17 * 32;
+constexpr int kPreThreads = 13 * 32;
 
 template <int D>
 struct PreSmem {
@@ -53,18 +59,19 @@ struct PreSmem {
     static constexpr int kKStage = (D / 64) * kSubK;
     static constexpr int kV = kK + 2 * kKStage;
     static constexpr int kVStage = 2 * kSubV;
-    static constexpr int kScale = kV + 2 * kVStage;   // fp16: kd [128][NG], km [128][NG], vd [NG][128], vm [NG][128]
-    static constexpr int kScaleBytes = 4 * kPreKeys * NG * 2;
-    static constexpr int kMisc = kScale + kScaleBytes;
+    static constexpr int kScale = kV + 2 * kVStage;   // fp16, two buffers: V's d [NG][128], m [NG][128]
+    static constexpr int kScaleBytes = 2 * kPreKeys * NG * 2;
+    static constexpr int kMisc = kScale + 2 * kScaleBytes;
     static constexpr int kBytes = kMisc + 7424 + 1024;              // alignment slack
 };
 
 struct PreMisc {
-    uint64_t q_ready[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], pv_done[2], drain;
+    uint64_t q_ready[2], k_full[2], k_empty[2], v_full[2], v_empty[2], drain;
+    uint64_t s_full[2], p_full[2], pv_done[2];                      // per group
     uint64_t dq[2], m_full[4];                        // the converting warps among themselves; a tile's numbers below
     uint32_t tmem;
     int abort_flag;
-    int red[8][4];
+    int red[2][4][4];
     int uneven[4];                                    // of tile j at j % 4: each position has its own dk and dv
     float k_fac[4][kPreKeys], v_exp[4][kPreKeys], v_inv[4][kPreKeys];      // 2^dk, dv, 2^-dv; else the first only
     uint32_t any_bad[4];
@@ -75,21 +82,45 @@ static_assert(sizeof(PreMisc) <= 7424, "PreMisc");
 __device__ __forceinline__ void tmem_ld32(uint32_t a, uint32_t (&v)[32]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+          "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+          "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(a)
+        : "memory");
+}
+// Loads that are asked for now and waited for together; the waits name the
+// registers, so that nothing reads them before.
+__device__ __forceinline__ void tmem_ask32(uint32_t a, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
         "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
         : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
           "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
           "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
           "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-        : "r"(a));
+        : "r"(a)
+        : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t a, const uint32_t (&v)[32]) {
+__device__ __forceinline__ void tmem_got32(uint32_t (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                   "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]),
+                   "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23])
+                 :
+                 : "memory");
+    asm volatile("" : "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
+                 :: "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t a, uint32_t (&v)[16]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
-        :: "r"(a), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
-           "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]),
-           "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]),
-           "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(a)
         : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t a, const uint32_t (&v)[16]) {
@@ -99,7 +130,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t a, const uint32_t (&v)[16]) {
            "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
         : "memory");
 }
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st8(uint32_t a, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 :: "r"(a), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // fp16 operands, fp32 sums, M = 128: A and B from shared memory, or A from tensor memory.
@@ -151,67 +186,153 @@ __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint3
 }
 __device__ __forceinline__ bool finite_bits(uint32_t b) { return (b & 0x7F800000u) != 0x7F800000u; }
 
-// The maximum of a row's terms S c + dv over the `vis` positions that it sees.
-template <bool UNEVEN, bool MASK>
-__device__ __forceinline__ float pre_top(uint32_t t_s, const PreMisc &ms, int slot, float c_row, int vis) {
-    float mx = -__builtin_huge_valf();
+// A tile that every row of the warp sees whole, with one dk and dv: the maximum
+// of a row's scores.
+__device__ __forceinline__ float pre_top(uint32_t t_s) {
+    float mx[8];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        uint32_t v[32];
-        tmem_ld32(t_s + 32 * c, v);
-        tmem_wait_ld();
+    for (int q = 0; q < 8; ++q) mx[q] = -__builtin_huge_valf();
+#pragma unroll 1
+    for (int c = 0; c < 2; ++c) {
+        uint32_t v[2][32];
+        tmem_ask32(t_s + 64 * c, v[0]);
+        tmem_ask32(t_s + 64 * c + 32, v[1]);
+        tmem_got32(v[0]);
+        tmem_got32(v[1]);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            float x = __uint_as_float(v[i]);
-            if (UNEVEN) x = fmaf(x, c_row * ms.k_fac[slot][32 * c + i], ms.v_exp[slot][32 * c + i]);
-            if (!MASK || 32 * c + i < vis) mx = fmaxf(mx, x);
-        }
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int q = 0; q < 8; ++q) mx[q] = fmaxf(mx[q], __uint_as_float(v[q >> 2][8 * (q & 3) + i]));
     }
-    return UNEVEN ? mx : fmaf(mx, c_row * ms.k_fac[slot][0], ms.v_exp[slot][0]);
+    return fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
 }
 
-// P = 2^(S c + dv - M) as fp16 over S; returns the sum of 2^-dv P.
-template <bool UNEVEN, bool MASK>
-__device__ __forceinline__ float pre_weights(uint32_t t_s, const PreMisc &ms, int slot, float c_row, float M, int vis) {
-    const float fac = c_row * ms.k_fac[slot][0], off = ms.v_exp[slot][0] - M;
-    const uint64_t f2 = pack2(fac, fac), o2 = pack2(off, off);
-    uint64_t sum2 = 0;
+// Its weights P = 2^(S fac + off), as fp16 over S (a chunk's P lies over scores
+// that were read before); returns their sum.
+__device__ __forceinline__ void pre_chunk(const uint32_t (&v)[32], uint32_t t_p, uint64_t f2, uint64_t o2, uint64_t (&sum2)[4]) {
+    uint32_t o[16];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        uint32_t v[32], o[16];
-        tmem_ld32(t_s + 32 * c, v);
-        tmem_wait_ld();
+    for (int h = 0; h < 32; h += 8) {                               // eight at a time: enough to overlap, few registers
+        float x[8];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int k = 32 * c + 2 * i;
-            float x, y;
-            if (UNEVEN) {
-                x = fmaf(__uint_as_float(v[2 * i]), c_row * ms.k_fac[slot][k], ms.v_exp[slot][k] - M);
-                y = fmaf(__uint_as_float(v[2 * i + 1]), c_row * ms.k_fac[slot][k + 1], ms.v_exp[slot][k + 1] - M);
-            } else {
-                unpack2(fma2(pack2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), f2, o2), x, y);
-            }
-            x = ex2(x);
-            y = ex2(y);
-            if (MASK) {
-                x = k < vis ? x : 0.f;
-                y = k + 1 < vis ? y : 0.f;
-            }
-            sum2 = UNEVEN ? fma2(pack2(x, y), pack2(ms.v_inv[slot][k], ms.v_inv[slot][k + 1]), sum2)
-                          : add2(sum2, pack2(x, y));
-            o[i] = pack_f16x2(x, y);
+        for (int i = 0; i < 8; i += 2)
+            unpack2(fma2(pack2(__uint_as_float(v[h + i]), __uint_as_float(v[h + i + 1])), f2, o2), x[i], x[i + 1]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = ex2(x[i]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            sum2[i] = add2(sum2[i], pack2(x[2 * i], x[2 * i + 1]));
+            o[h / 2 + i] = pack_f16x2(x[2 * i], x[2 * i + 1]);
         }
-        tmem_st16(t_s + 16 * c, o);
+    }
+    tmem_st16(t_p, o);
+}
+__device__ __forceinline__ float pre_weights(uint32_t t_s, float fac, float off) {
+    const uint64_t f2 = pack2(fac, fac), o2 = pack2(off, off);
+    uint64_t sum2[4] = {};
+    uint32_t a[32], b[32];
+    tmem_ask32(t_s, a);
+    tmem_got32(a);
+#pragma unroll 1
+    for (int c = 0; c < 2; ++c) {                                   // the next chunk comes in while one is worked on
+        tmem_ask32(t_s + 64 * c + 32, b);
+        pre_chunk(a, t_s + 32 * c, f2, o2, sum2);
+        tmem_got32(b);
+        if (c == 0) tmem_ask32(t_s + 64, a);
+        pre_chunk(b, t_s + 32 * c + 16, f2, o2, sum2);
+        if (c == 0) tmem_got32(a);
     }
     float x, y;
-    unpack2(sum2, x, y);
-    return UNEVEN ? x + y : (x + y) * ms.v_inv[slot][0];
+    unpack2(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])), x, y);
+    return x + y;
+}
+
+// The scores that a row does not see become -inf in tensor memory.
+__device__ __forceinline__ void pre_mask(uint32_t t_s, int vis) {
+#pragma unroll 1
+    for (int c = 0; c < kPreKeys; c += 16) {
+        if (!__any_sync(0xffffffffu, vis < c + 16)) continue;
+        uint32_t v[16];
+        tmem_ld16(t_s + c, v);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = c + i < vis ? v[i] : 0xFF800000u;
+        tmem_st16(t_s + c, v);
+    }
+    tmem_wait_st();
+}
+
+// The same for any tile: rows that see only `vis` of its positions, a dk and dv
+// for each position.  (Slow: 12000 cycles for a tile, against 3200.)
+__device__ __forceinline__ float pre_top_any(uint32_t t_s, const PreMisc &ms, int slot, bool uneven, float c_row, int vis) {
+    float mx = -__builtin_huge_valf();
+#pragma unroll 1
+    for (int c = 0; c < 8; ++c) {
+        uint32_t v[16];
+        tmem_ld16(t_s + 16 * c, v);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int k = 16 * c + i, n = uneven ? k : 0;
+            const float x = fmaf(__uint_as_float(v[i]), c_row * ms.k_fac[slot][n], ms.v_exp[slot][n]);
+            if (k < vis) mx = fmaxf(mx, x);
+        }
+    }
+    return mx;
+}
+__device__ __forceinline__ float pre_weights_any(uint32_t t_s, const PreMisc &ms, int slot, bool uneven, float c_row,
+                                                 float M, int vis) {
+    float sum = 0.f;
+#pragma unroll 1
+    for (int c = 0; c < 8; ++c) {
+        uint32_t v[16], o[8];
+        tmem_ld16(t_s + 16 * c, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float x[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int k = 16 * c + 2 * i + h, n = uneven ? k : 0;
+                x[h] = ex2(fmaf(__uint_as_float(v[2 * i + h]), c_row * ms.k_fac[slot][n], ms.v_exp[slot][n] - M));
+                x[h] = k < vis ? x[h] : 0.f;
+                sum = fmaf(x[h], ms.v_inv[slot][n], sum);
+            }
+            o[i] = pack_f16x2(x[0], x[1]);
+        }
+        tmem_st8(t_s + 8 * c, o);
+    }
+    return sum;
 }
 
 struct PreParams {
     Kv4AttendParams a;
-    int items, nsplit, row_tiles;
+    int items, nsplit, row_tiles, units;
 };
+
+// Unit u: 256 rows of one kv head and a part of the positions that they see.
+// The row tiles that see most come first; CTA c of n takes units c, 2 n - 1 - c,
+// 2 n + c, ..., so that one of the longest goes with one of the shortest.
+struct PreUnit {
+    int item, b, kvh, row0, split, nt, groups;
+    int64_t pos0, n_keys, t0;           // positions that some row sees; first tile
+    __device__ __forceinline__ PreUnit(const PreParams &pp, int u) {
+        const Kv4AttendParams &p = pp.a;
+        const int per_tile = pp.items * pp.nsplit, rest = u % per_tile;
+        split = rest / pp.items;
+        item = rest - split * pp.items;
+        b = item / p.KV;
+        kvh = item - b * p.KV;
+        row0 = (pp.row_tiles - 1 - u / per_tile) * kPreRows;
+        pos0 = p.pos0[(int64_t)b * p.pos_stride];
+        n_keys = max(min(pos0 + min(row0 + kPreRows - 1, p.R - 1) / p.G + 1, p.max_seq), (int64_t)0);
+        const uint32_t all = (uint32_t)((n_keys + kPreKeys - 1) / kPreKeys);       // (times 148 splits: below 2^32)
+        t0 = all * (uint32_t)split / (uint32_t)pp.nsplit;
+        nt = (int)(all * (uint32_t)(split + 1) / (uint32_t)pp.nsplit - (uint32_t)t0);
+        groups = p.R - row0 > 128 ? 2 : 1;
+    }
+};
+__device__ __forceinline__ int pre_unit(int i) {                    // the i-th unit of this CTA
+    const int n = (int)gridDim.x, c = (int)blockIdx.x;
+    return i & 1 ? (i + 1) * n - 1 - c : i * n + c;
+}
 
 template <int D>
 __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const __grid_constant__ PreParams pp) {
@@ -225,64 +346,24 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const __gri
     volatile int *abort_flag = &ms.abort_flag;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     griddep_launch_dependents();
-    griddep_wait();
-    // ---- this CTA's rows and positions; the row tiles that see most come first
-    const int item = blockIdx.x % pp.items, tile = pp.row_tiles - 1 - blockIdx.x / pp.items, split = blockIdx.y;
-    const int b = item / p.KV, kvh = item - b * p.KV, row0 = tile * kPreRows;
-    const int64_t pos0 = p.pos0[(int64_t)b * p.pos_stride];
-    const int tok_last = min(row0 + kPreRows - 1, p.R - 1) / p.G;
-    if (tid == 0 && pos0 + tok_last >= p.max_seq) atomicOr(&g_status, kErrBadIndex);
-    const int64_t n_keys = max(min(pos0 + tok_last + 1, p.max_seq), (int64_t)0);
-    const int64_t all = (n_keys + kPreKeys - 1) / kPreKeys;
-    const int64_t t0 = all * split / pp.nsplit, t1 = all * (split + 1) / pp.nsplit;
-    const int nt = (int)(t1 - t0);
-    const int groups = p.R - row0 > 128 ? 2 : 1;
-    const int64_t part0 = ((int64_t)item * pp.nsplit + split) * p.R;          // first row of this part
-    // ---- a thread's row (softmax groups)
-    const int grp = warp >> 2, row = row0 + (grp & 1) * 128 + (warp & 3) * 32 + lane;
-    const bool have = warp < 8 && row < p.R;
-    const int tok = have ? row / p.G : 0, hh = have ? row - tok * p.G : 0;
-    const auto write_row = [&](int c0, const float (&o)[32], float M, float l) {       // channels c0 .. c0 + 31
-        if (!have) return;
-        if (pp.nsplit > 1) {
-            float *dst = p.part_o + (part0 + row) * D + c0;
-#pragma unroll
-            for (int i = 0; i < 32; i += 4)
-                *reinterpret_cast<float4 *>(dst + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-            if (c0 == 0) p.part_ml[part0 + row] = make_float2(M, l);
-        } else {
-            const float inv = l != 0.f ? 1.f / l : 0.f;
-            uint16_t *dst = p.out + (((int64_t)b * p.T + tok) * p.H + kvh * p.G + hh) * D + c0;
-#pragma unroll
-            for (int i = 0; i < 32; i += 8)
-                *reinterpret_cast<uint4 *>(dst + i) =
-                    make_uint4(pack_bf16x2(o[i] * inv, o[i + 1] * inv), pack_bf16x2(o[i + 2] * inv, o[i + 3] * inv),
-                               pack_bf16x2(o[i + 4] * inv, o[i + 5] * inv), pack_bf16x2(o[i + 6] * inv, o[i + 7] * inv));
-        }
-    };
-    if (nt == 0) {
-        const float zero[32] = {};
-        for (int c0 = 0; c0 < D; c0 += 32) write_row(c0, zero, kNoMax, 0.f);
-        return;
-    }
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&ms.q_ready[i], 4);
-            mbar_init(&ms.k_full[i], 8);
+            mbar_init(&ms.k_full[i], 4);
             mbar_init(&ms.k_empty[i], 1);
-            mbar_init(&ms.v_full[i], 8);
+            mbar_init(&ms.v_full[i], 4);
             mbar_init(&ms.v_empty[i], 1);
             mbar_init(&ms.s_full[i], 1);
             mbar_init(&ms.p_full[i], 4);
             mbar_init(&ms.pv_done[i], 1);
         }
         mbar_init(&ms.drain, 1);
-        for (int i = 0; i < 2; ++i) mbar_init(&ms.dq[i], 8);
-        for (int i = 0; i < 4; ++i) mbar_init(&ms.m_full[i], 8);
+        for (int i = 0; i < 2; ++i) mbar_init(&ms.dq[i], 4);
+        for (int i = 0; i < 4; ++i) mbar_init(&ms.m_full[i], 4);
         ms.abort_flag = 0;
         fence_mbar_init();
     }
-    if (warp == 16) {
+    if (warp == 12) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                      :: "r"(smem_u32(&ms.tmem)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -292,357 +373,466 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const __gri
     tc_fence_after();
     const uint32_t tmem = ms.tmem;
     const uint32_t base = smem_u32(smem);
+    griddep_wait();
 
     if (warp < 8) {
         // ------------------------------------------------------------ softmax
-        if (grp < groups) {
-            const uint32_t t_lane = (uint32_t)((warp & 3) * 32) << 16;
-            const uint32_t t_s = tmem + t_lane + grp * 128, t_o = tmem + t_lane + 256 + grp * D;
-            // ---- this row of Q, scaled by 2^e (and the softmax scale's sign), in the K codes' channel order
-            const uint16_t *src = p.q + (int64_t)b * p.ldq_b + (int64_t)tok * p.ldq_t + (int64_t)(kvh * p.G + hh) * p.ldq_h;
-            float top = 0.f;
-            for (int c = 0; c < D / 8; ++c) {
-                const uint4 raw = have ? *reinterpret_cast<const uint4 *>(src + 8 * c) : make_uint4(0, 0, 0, 0);
-                const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(fabsf(bf_lo(w[i])), fabsf(bf_hi(w[i]))));
+        const int grp = warp >> 2, rl = (warp & 3) * 32 + lane;
+        const uint32_t t_lane = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t t_s = tmem + t_lane + grp * 128, t_o = tmem + t_lane + 256 + grp * D;
+        bool ok = true;
+        int tiles = 0, mine = 0;                                    // tiles before this unit: of all, and of this group
+        for (int n = 0; ok && pre_unit(n) < pp.units; ++n) {
+            const PreUnit un(pp, pre_unit(n));
+            const int row = un.row0 + grp * 128 + rl;
+            const bool have = row < p.R;
+            const int tok = have ? row / p.G : 0, hh = have ? row - tok * p.G : 0;
+            if (grp == 0 && un.split == 0 && un.kvh == 0 && have && hh == 0 && un.pos0 + tok >= p.max_seq)
+                atomicOr(&g_status, kErrBadIndex);
+            if (grp >= un.groups) {
+                tiles += un.nt;
+                continue;
             }
-            const int ex = (int)(__float_as_uint(top) >> 23) - 127;
-            const int e = top > 0.f && ex < 128 ? min(max(13 - ex, -100), 110) : 0;
-            const float up = __uint_as_float((uint32_t)(127 + e) << 23) * (p.scale_log2 < 0.f ? -1.f : 1.f);
-            const int rl = (warp & 3) * 32 + lane;
-            const uint32_t q_row = base + grp * SUBS * SM::kSubK + rl * 128;
-            for (int c = 0; c < D / 8; ++c) {
-                const uint4 raw = have ? *reinterpret_cast<const uint4 *>(src + 8 * c) : make_uint4(0, 0, 0, 0);
-                const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-                float x[8];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    x[2 * i] = bf_lo(w[i]) * up;
-                    x[2 * i + 1] = bf_hi(w[i]) * up;
+            // ---- Q, scaled by 2^e (and the softmax scale's sign), in the K codes' channel order.  D / 8 lanes fetch a
+            // row together, into its place; then each lane changes its own row there.  Short loops: straight code that
+            // runs once per unit waits for its instructions (this took 5 us, and the way out another 5)
+            float c_row = 0.f;
+            if (un.nt > 0) {
+                constexpr int LPR = D / 8, RPL = 32 / LPR;          // lanes per row, rows at a time
+                const int64_t off = have ? (int64_t)un.b * p.ldq_b + (int64_t)tok * p.ldq_t + (int64_t)(un.kvh * p.G + hh) * p.ldq_h : -1;
+                const uint32_t q_at = base + grp * SUBS * SM::kSubK + (warp & 3) * 4096;
+                const int c = lane % LPR;
+#pragma unroll 4
+                for (int i = 0; i < LPR; ++i) {
+                    const int r = i * RPL + lane / LPR;
+                    const int64_t from = __shfl_sync(0xffffffffu, off, r);
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                                 :: "r"(q_at + (c >> 3) * SM::kSubK + r * 128 + (((c ^ r) & 7) << 4)),
+                                    "l"(p.q + (from >= 0 ? from : 0) + 8 * c), "r"(from >= 0 ? 16 : 0) : "memory");
                 }
-                sts128(q_row + (c >> 3) * SM::kSubK + (((c ^ rl) & 7) << 4), pack_f16x2(x[0], x[4]),
-                       pack_f16x2(x[1], x[5]), pack_f16x2(x[2], x[6]), pack_f16x2(x[3], x[7]));
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                __syncwarp();
+                const uint32_t q_row = q_at + lane * 128;
+                uint32_t m2 = 0;                                    // largest magnitudes of the row, as bf16 bits
+#pragma unroll 4
+                for (int i = 0; i < LPR; ++i) {
+                    const uint4 x = lds128(q_row + (i >> 3) * SM::kSubK + (((i ^ lane) & 7) << 4));
+                    m2 = __vmaxu2(m2, __vmaxu2(__vmaxu2(x.x & 0x7FFF7FFFu, x.y & 0x7FFF7FFFu),
+                                               __vmaxu2(x.z & 0x7FFF7FFFu, x.w & 0x7FFF7FFFu)));
+                }
+                const uint32_t top = max(m2 & 0xFFFFu, m2 >> 16);
+                const int ex = (int)(top >> 7) - 127;
+                const int e = top && ex < 128 ? min(max(13 - ex, -100), 110) : 0;
+                const float up = __uint_as_float((uint32_t)(127 + e) << 23) * (p.scale_log2 < 0.f ? -1.f : 1.f);
+#pragma unroll 2
+                for (int i = 0; i < LPR; ++i) {
+                    const uint32_t at = q_row + (i >> 3) * SM::kSubK + (((i ^ lane) & 7) << 4);
+                    const uint4 x = lds128(at);                     // channels (0 4) (1 5) (2 6) (3 7)
+                    sts128(at, pack_f16x2(bf_lo(x.x) * up, bf_lo(x.z) * up), pack_f16x2(bf_hi(x.x) * up, bf_hi(x.z) * up),
+                           pack_f16x2(bf_lo(x.y) * up, bf_lo(x.w) * up), pack_f16x2(bf_hi(x.y) * up, bf_hi(x.w) * up));
+                }
+                c_row = fabsf(p.scale_log2) * __uint_as_float((uint32_t)(127 - e) << 23);
+                fence_proxy_async_smem();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&ms.q_ready[grp]);
             }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&ms.q_ready[grp]);
-            const float c_row = fabsf(p.scale_log2) * __uint_as_float((uint32_t)(127 - e) << 23);
             // positions that this row sees, from the first tile on
-            const int64_t at = have ? pos0 + tok : -1;
-            const int64_t sees = at < 0 || at >= p.max_seq ? 0 : max(at + 1 - t0 * kPreKeys, (int64_t)0);
+            const int64_t at = have ? un.pos0 + tok : -1;
+            const int64_t sees = at < 0 || at >= p.max_seq ? 0 : max(at + 1 - un.t0 * kPreKeys, (int64_t)0);
+            // a row that sees nothing here (padding, no row) goes along as if it saw all, and is zeros at the end
             float M = kNoMax, l = 0.f;
             uint32_t bad = 0;
-            bool ok = true;
-            for (int j = 0; j < nt; ++j) {
-                if (!role_wait(&ms.m_full[j & 3], (j >> 2) & 1, abort_flag) ||
-                    !role_wait(&ms.s_full[grp], j & 1, abort_flag)) {
+            for (int j = 0; j < un.nt; ++j) {
+                const int g = tiles + j, slot = g & 3;
+                // (the scores first: a group that sat out a unit may be phases ahead of m_full)
+                if (!role_wait(&ms.s_full[grp], (mine + j) & 1, abort_flag) ||
+                    !role_wait(&ms.m_full[slot], (g >> 2) & 1, abort_flag)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
-                const int vis = (int)min(max(sees - (int64_t)j * kPreKeys, (int64_t)0), (int64_t)kPreKeys);
-                const bool masked = __any_sync(0xffffffffu, vis < kPreKeys), uneven = ms.uneven[j & 3];
-                const float x_top = uneven   ? pre_top<true, true>(t_s, ms, j & 3, c_row, vis)
-                                    : masked ? pre_top<false, true>(t_s, ms, j & 3, c_row, vis)
-                                             : pre_top<false, false>(t_s, ms, j & 3, c_row, vis);
+                const int vis = sees ? (int)min(max(sees - (int64_t)j * kPreKeys, (int64_t)0), (int64_t)kPreKeys) : kPreKeys;
+                const float fac = c_row * ms.k_fac[slot][0], dv = ms.v_exp[slot][0];
+                // (a factor of zero would make NaN of the scores that are masked by -inf)
+                const bool uneven = ms.uneven[slot], plain = !uneven && !__any_sync(0xffffffffu, !(fac > 0.f));
+                if (plain && __any_sync(0xffffffffu, vis < kPreKeys)) pre_mask(t_s, vis);
+                const float x_top = plain ? fmaf(pre_top(t_s), fac, dv) : pre_top_any(t_s, ms, slot, uneven, c_row, vis);
                 if (__any_sync(0xffffffffu, x_top > M + kRescale)) {
-                    const float to = x_top > M ? x_top : M;
-                    const float a = ex2(M - to);
+                    const float to = x_top > M ? x_top : M, a = ex2(M - to);
                     M = to;
                     l *= a;
                     if (j > 0) {                                    // O is complete up to the last tile: its PV is done
-                        if (!role_wait(&ms.pv_done[grp], (j - 1) & 1, abort_flag)) {
+                        if (!role_wait(&ms.pv_done[grp], (mine + j - 1) & 1, abort_flag)) {
                             ok = false;
                             break;
                         }
                         tc_fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < D / 16; ++c) {
+                            uint32_t o[16];
+                            tmem_ld16(t_o + 16 * c, o);
 #pragma unroll
-                        for (int c = 0; c < D / 32; ++c) {
-                            uint32_t v[32];
-                            tmem_ld32(t_o + 32 * c, v);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * a);
-                            tmem_st32(t_o + 32 * c, v);
+                            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * a);
+                            tmem_st16(t_o + 16 * c, o);
                         }
                     }
                 }
-                const float sum = uneven   ? pre_weights<true, true>(t_s, ms, j & 3, c_row, M, vis)
-                                  : masked ? pre_weights<false, true>(t_s, ms, j & 3, c_row, M, vis)
-                                           : pre_weights<false, false>(t_s, ms, j & 3, c_row, M, vis);
+                l += plain ? pre_weights(t_s, fac, dv - M) * ms.v_inv[slot][0]
+                           : pre_weights_any(t_s, ms, slot, uneven, c_row, M, vis);
+                // (read before P is handed over: the slot is used again after that)
+                if (ms.any_bad[slot])
+                    for (int k = 0; k < vis; ++k) bad |= (ms.bad[slot][k >> 2] >> (8 * (k & 3))) & 0xFFu;
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&ms.p_full[grp]);
-                l += sum;
-                if (ms.any_bad[j & 3])
-                    for (int i = 0; i < vis; ++i) bad |= (ms.bad[j & 3][i >> 2] >> (8 * (i & 3))) & 0xFFu;
             }
-            if (ok && role_wait(&ms.pv_done[grp], (nt - 1) & 1, abort_flag)) {
-                tc_fence_after();
+            tiles += un.nt;
+            mine += un.nt;
+            if (ok && un.nt > 0) ok = role_wait(&ms.pv_done[grp], (mine - 1) & 1, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            // ---- out, by way of Q's place (its products are done): 128 bytes of 4 rows per store
+            int64_t off = -1;                                       // bytes of this row from the start
+            if (have)
+                off = pp.nsplit > 1 ? (((int64_t)un.item * pp.nsplit + un.split) * p.R + row) * D * 4
+                                    : (((int64_t)un.b * p.T + tok) * p.H + un.kvh * p.G + hh) * D * 2;
+            if (have && pp.nsplit > 1) p.part_ml[off / (D * 4)] = make_float2(sees ? M : kNoMax, sees ? l : 0.f);
+            uint8_t *dst = pp.nsplit > 1 ? reinterpret_cast<uint8_t *>(p.part_o) : reinterpret_cast<uint8_t *>(p.out);
+            const float inv = pp.nsplit > 1 ? 1.f : l != 0.f ? 1.f / l : 0.f;
+            const int per = pp.nsplit > 1 ? 2 : 4;                  // 16 channels each: together 128 bytes, a piece
+#pragma unroll 1
+            for (int c = 0; c < D / 16; ++c) {
+                const int piece = c / per, part = c % per;
+                const float f = (bad >> (c >> 1)) & 1u ? __int_as_float(0x7fc00000) : inv;
+                uint32_t v[16];
+                tmem_ld16(t_o + 16 * c, v);
 #pragma unroll
-                for (int c = 0; c < D / 32; ++c) {
-                    uint32_t v[32];
-                    tmem_ld32(t_o + 32 * c, v);
-                    tmem_wait_ld();
-                    float o[32];
+                for (int k = 0; k < 16; ++k) v[k] = sees ? __float_as_uint(__uint_as_float(v[k]) * f) : 0u;
+                const uint32_t at = base + (grp * SUBS + piece % SUBS) * SM::kSubK + (warp & 3) * 4096;
+                if (pp.nsplit > 1) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        o[i] = (bad >> c) & 1u ? __int_as_float(0x7fc00000) : __uint_as_float(v[i]);
-                    write_row(32 * c, o, M, l);
-                }
-            }
-            tc_fence_before();
-        }
-    } else if (warp < 16) {
-        // ------------------------------------------------- K and V to fp16
-        const int dw = warp - 8, dt = tid - 256;
-        // K: 8 positions x 2 halves of the channels' words x 2; V: 8 half blocks x 2 halves of the groups x 2
-        const int part = (lane >> 3) & 1, key = dw * 16 + (lane >> 4) * 8 + (lane & 7);
-        const int vp = (dw >> 2) * 8 + (lane & 7), vg = (dw & 3) * 2 + (lane >> 4);
-        const uint8_t *cache = p.blocks + ((int64_t)b * p.KV + kvh) * p.nblk * L::kBytes;
-        struct Raw {
-            uint32_t k[2][NG], v[4][NH], kd, km, vd, vm;                    // codes; two groups' scales and minima
-        } raw;
-        const auto load = [&](int j) {                              // this thread's part of tile j; nothing past the cache
-            const int64_t blk0 = (t0 + j) * (kPreKeys / kKvBlock);
-            const int64_t kb = blk0 + dw, vb = blk0 + (vp >> 1);
-            raw = Raw{};
-            if (kb < p.nblk) {
-                const uint8_t *at = cache + kb * L::kBytes;
-                const int r = key & 15;
-#pragma unroll
-                for (int i = 0; i < NH; ++i)
-                    raw.vm |= (uint32_t)*reinterpret_cast<const uint16_t *>(
-                                  at + L::kVm + (((r >> 1) * NG + part * NH + i) * 2 + (r & 1)) * 2) << (16 * i);
-                if constexpr (NG == 4) {
-                    const uint4 x = *reinterpret_cast<const uint4 *>(at + (r * 4 + 2 * part) * 16);
-                    const uint4 y = *reinterpret_cast<const uint4 *>(at + (r * 4 + 2 * part + 1) * 16);
-                    raw.k[0][0] = x.x, raw.k[0][1] = x.y, raw.k[0][2] = x.z, raw.k[0][3] = x.w;
-                    raw.k[1][0] = y.x, raw.k[1][1] = y.y, raw.k[1][2] = y.z, raw.k[1][3] = y.w;
-                    raw.kd = *reinterpret_cast<const uint32_t *>(at + L::kKd + r * 8 + part * 4);
-                    raw.km = *reinterpret_cast<const uint32_t *>(at + L::kKm + r * 8 + part * 4);
-                    raw.vd = *reinterpret_cast<const uint32_t *>(at + L::kVd + r * 8 + part * 4);
+                    for (int i = 0; i < 4; ++i)
+                        sts128(at + lane * 128 + (((4 * part + i) ^ lane) & 7) * 16, v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
                 } else {
-                    const uint4 x = *reinterpret_cast<const uint4 *>(at + (r * 4 + 2 * part) * 8);
-                    raw.k[0][0] = x.x, raw.k[0][1] = x.y, raw.k[1][0] = x.z, raw.k[1][1] = x.w;
-                    raw.kd = *reinterpret_cast<const uint16_t *>(at + L::kKd + r * 4 + part * 2);
-                    raw.km = *reinterpret_cast<const uint16_t *>(at + L::kKm + r * 4 + part * 2);
-                    raw.vd = *reinterpret_cast<const uint16_t *>(at + L::kVd + r * 4 + part * 2);
-                }
-            }
-            if (vb < p.nblk) {
-                const uint8_t *at = cache + vb * L::kBytes + L::kV + (((vp & 1) * 8 + vg) * 4) * NG * 4 + part * NH * 4;
 #pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    if constexpr (NG == 4) {
-                        const uint2 x = *reinterpret_cast<const uint2 *>(at + t * 16);
-                        raw.v[t][0] = x.x, raw.v[t][1] = x.y;
-                    } else {
-                        raw.v[t][0] = *reinterpret_cast<const uint32_t *>(at + t * 8);
+                    for (int i = 0; i < 2; ++i) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            w[k] = pack_bf16x2(__uint_as_float(v[8 * i + 2 * k]), __uint_as_float(v[8 * i + 2 * k + 1]));
+                        sts128(at + lane * 128 + (((2 * part + i) ^ lane) & 7) * 16, w[0], w[1], w[2], w[3]);
                     }
                 }
+                if (part + 1 < per) continue;
+                __syncwarp();
+#pragma unroll 2
+                for (int i = 0; i < 8; ++i) {
+                    const int r = 4 * i + (lane >> 3);
+                    const int64_t to = __shfl_sync(0xffffffffu, off, r);
+                    const uint4 x = lds128(at + r * 128 + (((lane ^ r) & 7) << 4));
+                    if (to >= 0) *reinterpret_cast<uint4 *>(dst + to + piece * 128 + (lane & 7) * 16) = x;
+                }
+                __syncwarp();
+            }
+        }
+        tc_fence_before();
+    } else if (warp < 12) {
+        // ------------------------------------------------- K and V to fp16
+        // K: thread = position.  V: thread = 8 positions (vp) x 4 channels of
+        // each group (vg); the scales of all positions through shared memory.
+        // Scales are prepared one tile ahead of the codes, and the tile's
+        // largest exponents before that, so the warps meet once per tile, long
+        // after they have arrived.
+        // The tiles of all units follow one another; the loads look ahead.
+        const int dw = warp - 8, key = tid - 256, vp = (dw >> 1) * 8 + (lane & 7), vg = (dw & 1) * 4 + (lane >> 3);
+        struct Tile {                                               // where a tile lies
+            const uint8_t *cache;                                   // its head's blocks
+            int64_t blk;                                            // its first block
+            int live;                                               // positions that some row sees; 0: no more tiles
+        };
+        struct Feed {                                               // the tiles of this CTA's units, one after the other
+            int n, left;                                            // next unit; tiles left of this one
+            Tile tl;
+            int64_t keys;                                           // positions left of this unit
+        } feed = {0, 0, {p.blocks, 0, 0}, 0};
+        const auto next_tile = [&]() -> Tile {
+            while (feed.left == 0 && pre_unit(feed.n) < pp.units) {
+                const PreUnit un(pp, pre_unit(feed.n++));
+                feed.left = un.nt;
+                feed.tl.cache = p.blocks + ((int64_t)un.b * p.KV + un.kvh) * p.nblk * L::kBytes;
+                feed.tl.blk = un.t0 * (kPreKeys / kKvBlock);
+                feed.keys = un.n_keys - un.t0 * kPreKeys;
+            }
+            Tile t = feed.tl;
+            t.live = feed.left ? (int)min(feed.keys, (int64_t)kPreKeys) : 0;
+            if (feed.left) {
+                --feed.left;
+                feed.tl.blk += kPreKeys / kKvBlock;
+                feed.keys -= kPreKeys;
+            }
+            return t;
+        };
+        uint32_t kc[4][NG], vc[4][NG];                              // codes of a tile
+        uint32_t rk[NH], rkm[NH], rv[NH], rvm[NH];                  // raw scales and minima of this position, in pairs
+        const auto words = [](const uint8_t *at, uint32_t (&w)[NG]) {
+            if constexpr (NG == 4) {
+                const uint4 x = *reinterpret_cast<const uint4 *>(at);
+                w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+            } else {
+                const uint2 x = *reinterpret_cast<const uint2 *>(at);
+                w[0] = x.x, w[1] = x.y;
             }
         };
-        load(0);
-        const uint32_t s_kd = base + SM::kScale, s_km = s_kd + kPreKeys * NG * 2, s_vd = s_km + kPreKeys * NG * 2,
-                       s_vm = s_vd + kPreKeys * NG * 2;
-        for (int j = 0; j < nt; ++j) {
-            const int st = j & 1, slot = j & 3;
-            const uint32_t wait_parity = ((j >> 1) & 1) ^ 1;
-            // ---- scales and minima; positions from n_keys on are zeros
-            const int64_t key0 = (t0 + j) * kPreKeys;
-            const int live = (int)min(n_keys - key0, (int64_t)kPreKeys);
-            float kd[2], km[2], vd[2], vm[2];
-            kd[0] = bf_lo(raw.kd), kd[1] = bf_hi(raw.kd);
-            km[0] = bf_lo(raw.km), km[1] = bf_hi(raw.km);
-            vd[0] = bf_lo(raw.vd), vd[1] = bf_hi(raw.vd);
-            vm[0] = bf_lo(raw.vm), vm[1] = bf_hi(raw.vm);
-            uint32_t bad_k = 0, bad_v = 0;
-            float kmax = 0.f, vmax = 0.f;                           // no value of this position is larger
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if (key >= live) kd[i] = km[i] = vd[i] = vm[i] = 0.f;
-                if (!finite_bits(__float_as_uint(kd[i])) || !finite_bits(__float_as_uint(km[i]))) {
-                    bad_k |= 1u << i;
-                    kd[i] = km[i] = 0.f;
-                }
-                if (!finite_bits(__float_as_uint(vd[i])) || !finite_bits(__float_as_uint(vm[i]))) {
-                    bad_v |= 1u << i;
-                    vd[i] = vm[i] = 0.f;
-                }
-                kmax = fmaxf(kmax, fmaxf(fabsf(km[i]), fabsf(fmaf(15.f, kd[i], km[i]))));
-                vmax = fmaxf(vmax, fmaxf(fabsf(vm[i]), fabsf(fmaf(15.f, vd[i], vm[i]))));
+        const auto halves = [](const uint8_t *at, uint32_t (&w)[NH]) {
+            if constexpr (NH == 2) {
+                const uint2 x = *reinterpret_cast<const uint2 *>(at);
+                w[0] = x.x, w[1] = x.y;
+            } else {
+                w[0] = *reinterpret_cast<const uint32_t *>(at);
             }
-            kmax = fmaxf(kmax, __shfl_xor_sync(0xffffffffu, kmax, 8));          // the position's other groups
-            vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 8));
-            // exponents: 2^e is above the largest value; a position of zeros has none
-            constexpr int kNone = 1 << 20;
-            const int ke = kmax > 0.f ? min(max((int)(__float_as_uint(kmax) >> 23) - 126, -100), 110) : kNone,
-                      ve = vmax > 0.f ? min(max((int)(__float_as_uint(vmax) >> 23) - 126, -100), 110) : kNone;
-            int k_hi = __reduce_max_sync(0xffffffffu, ke == kNone ? -100 : ke), k_lo = __reduce_min_sync(0xffffffffu, ke),
-                v_hi = __reduce_max_sync(0xffffffffu, ve == kNone ? -100 : ve), v_lo = __reduce_min_sync(0xffffffffu, ve);
+        };
+        const auto load_k = [&](const Tile &tl) {                   // nothing past the cache is read
+            const uint8_t *cache = tl.cache;
+            const int64_t blk = tl.blk + (key >> 4);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+#pragma unroll
+                for (int g = 0; g < NG; ++g) kc[t][g] = 0;
+                if (blk < p.nblk) words(cache + blk * L::kBytes + ((key & 15) * 4 + t) * NG * 4, kc[t]);
+            }
+        };
+        const auto load_v = [&](const Tile &tl) {
+            const uint8_t *cache = tl.cache;
+            const int64_t blk = tl.blk + (vp >> 1);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+#pragma unroll
+                for (int g = 0; g < NG; ++g) vc[t][g] = 0;
+                if (blk < p.nblk) words(cache + blk * L::kBytes + L::kV + (((vp & 1) * 8 + vg) * 4 + t) * NG * 4, vc[t]);
+            }
+        };
+        const auto load_scales = [&](const Tile &tl) {
+            const uint8_t *cache = tl.cache;
+            const int64_t blk = tl.blk + (key >> 4);
+            const int r = key & 15;
+#pragma unroll
+            for (int i = 0; i < NH; ++i) rk[i] = rkm[i] = rv[i] = rvm[i] = 0;
+            if (tl.live > 0 && blk < p.nblk) {
+                const uint8_t *at = cache + blk * L::kBytes;
+                halves(at + L::kKd + r * NG * 2, rk);
+                halves(at + L::kKm + r * NG * 2, rkm);
+                halves(at + L::kVd + r * NG * 2, rv);
+                uint32_t m[NG];                                     // pairs of positions, one word per group
+                words(at + L::kVm + (r >> 1) * NG * 4, m);
+#pragma unroll
+                for (int i = 0; i < NH; ++i) rvm[i] = prmt(m[2 * i], m[2 * i + 1], r & 1 ? 0x7632u : 0x5410u);
+            }
+        };
+        // numbers of a tile's position, ready to be scaled
+        float kd[NG], km[NG], vd[NG], vm[NG];
+        uint32_t bad_k = 0, bad_v = 0;
+        constexpr int kNone = 1 << 20;
+        int ke = kNone, ve = kNone;                                 // 2^e is above the position's largest value
+        const auto survey = [&](int j, int live) {                  // the raw scales of tile j; writes the warp's exponents
+            float kmax = 0.f, vmax = 0.f;
+            bad_k = bad_v = 0;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                const auto pick = [&](const uint32_t (&w)[NH]) { return g & 1 ? bf_hi(w[g >> 1]) : bf_lo(w[g >> 1]); };
+                kd[g] = pick(rk), km[g] = pick(rkm), vd[g] = pick(rv), vm[g] = pick(rvm);
+                if (key >= live) kd[g] = km[g] = vd[g] = vm[g] = 0.f;           // behind the last position: zeros
+                if (!finite_bits(__float_as_uint(kd[g])) || !finite_bits(__float_as_uint(km[g]))) {
+                    bad_k |= 1u << g;
+                    kd[g] = km[g] = 0.f;
+                }
+                if (!finite_bits(__float_as_uint(vd[g])) || !finite_bits(__float_as_uint(vm[g]))) {
+                    bad_v |= 1u << g;
+                    vd[g] = vm[g] = 0.f;
+                }
+                kmax = fmaxf(kmax, fmaxf(fabsf(km[g]), fabsf(fmaf(15.f, kd[g], km[g]))));
+                vmax = fmaxf(vmax, fmaxf(fabsf(vm[g]), fabsf(fmaf(15.f, vd[g], vm[g]))));
+            }
+            ke = kmax > 0.f ? min(max((int)(__float_as_uint(kmax) >> 23) - 126, -100), 110) : kNone;
+            ve = vmax > 0.f ? min(max((int)(__float_as_uint(vmax) >> 23) - 126, -100), 110) : kNone;
+            const int a = __reduce_max_sync(0xffffffffu, ke == kNone ? -100 : ke), c = __reduce_min_sync(0xffffffffu, ke),
+                      d = __reduce_max_sync(0xffffffffu, ve == kNone ? -100 : ve), f = __reduce_min_sync(0xffffffffu, ve);
             if (lane == 0) {
-                ms.red[dw][0] = k_hi;
-                ms.red[dw][1] = k_lo;
-                ms.red[dw][2] = v_hi;
-                ms.red[dw][3] = v_lo;
+                int *red = ms.red[j & 1][dw];
+                red[0] = a, red[1] = c, red[2] = d, red[3] = f;
             }
-            if (dt < kPreKeys / 4) ms.bad[slot][dt] = 0;
-            if (dt == 0) ms.any_bad[slot] = 0;
+            ms.bad[j & 3][lane] = 0;                                // every warp the same
+            if (lane == 0) ms.any_bad[j & 3] = 0;
             __syncwarp();
-            if (lane == 0) mbar_arrive(&ms.dq[0]);
-            if (!role_wait(&ms.dq[0], j & 1, abort_flag)) break;
+        };
+        uint32_t kd24[NH], kmh[NH];                                 // K's scales * 2^24 and minima of this position, fp16 pairs
+        const auto scale = [&](int j) {                             // after all warps' exponents of tile j
+            const int slot = j & 3;
+            int k_hi = -100, k_lo = kNone, v_hi = -100, v_lo = kNone;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                k_hi = max(k_hi, ms.red[i][0]);
-                k_lo = min(k_lo, ms.red[i][1]);
-                v_hi = max(v_hi, ms.red[i][2]);
-                v_lo = min(v_lo, ms.red[i][3]);
+            for (int i = 0; i < 4; ++i) {
+                const int *red = ms.red[j & 1][i];
+                k_hi = max(k_hi, red[0]), k_lo = min(k_lo, red[1]), v_hi = max(v_hi, red[2]), v_lo = min(v_lo, red[3]);
             }
             const bool uneven = k_hi - k_lo > 6 || v_hi - v_lo > 6;
             // 2^-dk times the largest value is at most 2^-6
             const int dk = (uneven && ke != kNone ? ke : k_hi) + 6, dv = (uneven && ve != kNone ? ve : v_hi) + 6;
-            {
-                const float k24 = __uint_as_float((uint32_t)(127 + 24 - dk) << 23), v24 = __uint_as_float((uint32_t)(127 + 24 - dv) << 23);
-                const uint32_t kdh = pack_f16x2(kd[0] * k24, kd[1] * k24), kmh = pack_f16x2(km[0] * k24 * 0x1p-24f, km[1] * k24 * 0x1p-24f);
-                const uint32_t vdh = pack_f16x2(vd[0] * v24, vd[1] * v24), vmh = pack_f16x2(vm[0] * v24 * 0x1p-24f, vm[1] * v24 * 0x1p-24f);
-                const uint32_t nan_k = (bad_k & 1 ? 0x7FFFu : 0u) | (bad_k & 2 ? 0x7FFF0000u : 0u);
-                uint16_t *a = reinterpret_cast<uint16_t *>(smem + SM::kScale);
-                constexpr int PART = kPreKeys * NG;
-                const int g0 = part * NH;
+            const float k0 = __uint_as_float((uint32_t)(127 - dk) << 23), k24 = k0 * 0x1p24f,
+                        v0 = __uint_as_float((uint32_t)(127 - dv) << 23), v24 = v0 * 0x1p24f;
+            uint16_t *a = reinterpret_cast<uint16_t *>(smem + SM::kScale + (j & 1) * SM::kScaleBytes);
 #pragma unroll
-                for (int i = 0; i < NH; ++i) {
-                    a[key * NG + g0 + i] = (uint16_t)((kdh | nan_k) >> (16 * i));
-                    a[PART + key * NG + g0 + i] = (uint16_t)(kmh >> (16 * i));
-                    a[2 * PART + (g0 + i) * kPreKeys + key] = (uint16_t)(vdh >> (16 * i));
-                    a[3 * PART + (g0 + i) * kPreKeys + key] = (uint16_t)(vmh >> (16 * i));
-                    if (bad_v >> i & 1) {
-                        atomicOr(&ms.bad[slot][key >> 2], (1u << (g0 + i)) << (8 * (key & 3)));
-                        ms.any_bad[slot] = 1;
-                    }
-                }
-                if (dt == 0) ms.uneven[slot] = uneven;
-                if (part == 0 && (uneven || key == 0)) {
-                    ms.k_fac[slot][key] = __uint_as_float((uint32_t)(127 + dk) << 23);
-                    ms.v_exp[slot][key] = (float)dv;
-                    ms.v_inv[slot][key] = ex2((float)-dv);
-                }
+            for (int i = 0; i < NH; ++i) {
+                kd24[i] = pack_f16x2(kd[2 * i] * k24, kd[2 * i + 1] * k24) | (bad_k >> (2 * i) & 1 ? 0x7FFFu : 0u) |
+                          (bad_k >> (2 * i + 1) & 1 ? 0x7FFF0000u : 0u);
+                kmh[i] = pack_f16x2(km[2 * i] * k0, km[2 * i + 1] * k0);
+                const uint32_t d = pack_f16x2(vd[2 * i] * v24, vd[2 * i + 1] * v24), m = pack_f16x2(vm[2 * i] * v0, vm[2 * i + 1] * v0);
+                a[2 * i * kPreKeys + key] = (uint16_t)d;
+                a[(2 * i + 1) * kPreKeys + key] = (uint16_t)(d >> 16);
+                a[(NG + 2 * i) * kPreKeys + key] = (uint16_t)m;
+                a[(NG + 2 * i + 1) * kPreKeys + key] = (uint16_t)(m >> 16);
+            }
+            if (bad_v) {
+                atomicOr(&ms.bad[slot][key >> 2], bad_v << (8 * (key & 3)));
+                ms.any_bad[slot] = 1;
+            }
+            if (key == 0) ms.uneven[slot] = uneven;
+            if (uneven || key == 0) {
+                ms.k_fac[slot][key] = __uint_as_float((uint32_t)(127 + dk) << 23);
+                ms.v_exp[slot][key] = (float)dv;
+                ms.v_inv[slot][key] = ex2((float)-dv);
             }
             __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(&ms.dq[1]);
-                mbar_arrive(&ms.m_full[slot]);
-            }
-            if (!role_wait(&ms.dq[1], j & 1, abort_flag)) break;
-            const Raw now = raw;
-            if (j + 1 < nt) load(j + 1);
+            if (lane == 0) mbar_arrive(&ms.m_full[slot]);
+        };
+        Tile now = next_tile(), ahead = next_tile();               // tile j and tile j + 1
+        load_scales(now);
+        load_k(now);
+        load_v(now);
+        survey(0, now.live);
+        if (lane == 0) mbar_arrive(&ms.dq[1]);
+        load_scales(ahead);
+        bool ok = role_wait(&ms.dq[1], 0, abort_flag);
+        if (ok && now.live) scale(0);
+        for (int j = 0; now.live && ok; ++j) {
+            const int st = j & 1;
+            const uint32_t wait_parity = ((j >> 1) & 1) ^ 1;
+            // ---- arrive with the scales of this tile and the exponents of the next
+            survey(j + 1, ahead.live);
+            if (lane == 0) mbar_arrive(&ms.dq[0]);
+            const Tile later = next_tile();
+            load_scales(later);
             // ---- K: 16-byte chunks of 8 channels, [128 positions][64 channels] swizzled
             if (!role_wait(&ms.k_empty[st], wait_parity, abort_flag)) break;
-            {
-                const uint32_t k_row = base + SM::kK + st * SM::kKStage + key * 128;
-                uint32_t dw_[NH], mw[NH];                           // this position's groups, in pairs
+            const uint32_t k_row = base + SM::kK + st * SM::kKStage + key * 128;
 #pragma unroll
-                for (int i = 0; i < NH; ++i) {
-                    dw_[i] = lds32(s_kd + key * NG * 2 + 4 * i);
-                    mw[i] = lds32(s_km + key * NG * 2 + 4 * i);
-                }
+            for (int g = 0; g < NG; ++g) {
+                const uint32_t sel = g & 1 ? 0x3232u : 0x1010u;
+                const uint32_t d24 = prmt(kd24[g >> 1], 0u, sel), m = prmt(kmh[g >> 1], 0u, sel);
+                const uint32_t d20 = hmul2(d24, 0x2C002C00u);       // / 16
 #pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    const uint32_t sel = g & 1 ? 0x3232u : 0x1010u;
-                    const uint32_t d24 = prmt(dw_[g >> 1], 0u, sel), m = prmt(mw[g >> 1], 0u, sel);
-                    const uint32_t d20 = hmul2(d24, 0x2C002C00u);   // / 16
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint32_t w = now.k[i][g], h = w >> 8;
-                        const int c = g * 4 + 2 * part + i;         // chunk of the row
-                        sts128(k_row + (c >> 3) * SM::kSubK + (((c ^ key) & 7) << 4), hfma2(w & 0x000F000Fu, d24, m),
-                               hfma2(w & 0x00F000F0u, d20, m), hfma2(h & 0x000F000Fu, d24, m),
-                               hfma2(h & 0x00F000F0u, d20, m));
-                    }
+                for (int t = 0; t < 4; ++t) {
+                    const uint32_t w = kc[t][g], h = w >> 8;
+                    const int c = g * 4 + t;                        // chunk of the row
+                    sts128(k_row + (c >> 3) * SM::kSubK + (((c ^ key) & 7) << 4), hfma2(w & 0x000F000Fu, d24, m),
+                           hfma2(w & 0x00F000F0u, d20, m), hfma2(h & 0x000F000Fu, d24, m), hfma2(h & 0x00F000F0u, d20, m));
                 }
             }
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&ms.k_full[st]);
+            if (ahead.live) load_k(ahead);
             // ---- V^T: 16-byte chunks of 8 positions, [D channels][64 positions] swizzled
-            if (!role_wait(&ms.v_empty[st], wait_parity, abort_flag)) break;
-            {
-                const uint32_t v_tile = base + SM::kV + st * SM::kVStage + (vp >> 3) * SM::kSubV;
+            if (!role_wait(&ms.dq[0], j & 1, abort_flag) || !role_wait(&ms.v_empty[st], wait_parity, abort_flag)) break;
+            const uint32_t v_tile = base + SM::kV + st * SM::kVStage + (vp >> 3) * SM::kSubV;
+            const uint32_t v_scale = base + SM::kScale + (j & 1) * SM::kScaleBytes + vp * 16;
 #pragma unroll
-                for (int i = 0; i < NH; ++i) {
-                    const int g = part * NH + i;
-                    const uint4 d4 = lds128(s_vd + (g * kPreKeys + vp * 8) * 2), m4 = lds128(s_vm + (g * kPreKeys + vp * 8) * 2);
-                    const uint32_t d24[4] = {d4.x, d4.y, d4.z, d4.w}, m[4] = {m4.x, m4.y, m4.z, m4.w};
-                    uint32_t x[4][4];                               // [channel][position pair]
+            for (int g = 0; g < NG; ++g) {
+                const uint4 d4 = lds128(v_scale + g * kPreKeys * 2), m4 = lds128(v_scale + (NG + g) * kPreKeys * 2);
+                const uint32_t d24[4] = {d4.x, d4.y, d4.z, d4.w}, m[4] = {m4.x, m4.y, m4.z, m4.w};
+                uint32_t x[4][4];                                   // [channel][position pair]
 #pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        const uint32_t w = now.v[t][i], h = w >> 8, d20 = hmul2(d24[t], 0x2C002C00u);
-                        x[0][t] = hfma2(w & 0x000F000Fu, d24[t], m[t]);
-                        x[1][t] = hfma2(w & 0x00F000F0u, d20, m[t]);
-                        x[2][t] = hfma2(h & 0x000F000Fu, d24[t], m[t]);
-                        x[3][t] = hfma2(h & 0x00F000F0u, d20, m[t]);
-                    }
+                for (int t = 0; t < 4; ++t) {
+                    const uint32_t w = vc[t][g], h = w >> 8, d20 = hmul2(d24[t], 0x2C002C00u);
+                    x[0][t] = hfma2(w & 0x000F000Fu, d24[t], m[t]);
+                    x[1][t] = hfma2(w & 0x00F000F0u, d20, m[t]);
+                    x[2][t] = hfma2(h & 0x000F000Fu, d24[t], m[t]);
+                    x[3][t] = hfma2(h & 0x00F000F0u, d20, m[t]);
+                }
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        const int ch = 32 * g + 4 * vg + n;
-                        sts128(v_tile + ch * 128 + (((vp ^ ch) & 7) << 4), x[n][0], x[n][1], x[n][2], x[n][3]);
-                    }
+                for (int n = 0; n < 4; ++n) {
+                    const int ch = 32 * g + 4 * vg + n;
+                    sts128(v_tile + ch * 128 + (((vp ^ ch) & 7) << 4), x[n][0], x[n][1], x[n][2], x[n][3]);
                 }
             }
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&ms.v_full[st]);
+            if (ahead.live) {
+                load_v(ahead);
+                scale(j + 1);
+            }
+            now = ahead;
+            ahead = later;
         }
     } else if (lane == 0) {
         // ------------------------------------------------------------ MMAs
         constexpr uint32_t id_s = umma_idesc_f16<kPreKeys>(), id_o = umma_idesc_f16<D>();
-        bool ok = true;
-        const auto qk = [&](int g, int j) {
-            const uint32_t qa = base + g * SUBS * SM::kSubK, ka = base + SM::kK + (j & 1) * SM::kKStage;
-#pragma unroll
+        const auto qk = [&](int g, int st) {                        // the scores of the tile in stage st
+            uint64_t a = umma_desc_sw128(base + g * SUBS * SM::kSubK), bd = umma_desc_sw128(base + SM::kK + st * SM::kKStage);
+#pragma unroll 1
             for (int s = 0; s < SUBS; ++s) {
-                const uint64_t a = umma_desc_sw128(qa + s * SM::kSubK), bd = umma_desc_sw128(ka + s * SM::kSubK);
 #pragma unroll
                 for (int k = 0; k < 4; ++k)                         // 16 channels each: 32 bytes along the row
                     umma_f16_ss(tmem + g * 128, a + 2u * k, bd + 2u * k, id_s, (s | k) != 0);
+                a += SM::kSubK >> 4;
+                bd += SM::kSubK >> 4;
             }
             umma_commit(&ms.s_full[g]);
         };
-        for (int g = 0; g < groups && ok; ++g) ok = role_wait(&ms.q_ready[g], 0, abort_flag);
-        ok = ok && role_wait(&ms.k_full[0], 0, abort_flag);
-        if (ok) {
-            tc_fence_after();
-            for (int g = 0; g < groups; ++g) qk(g, 0);
-            umma_commit(&ms.k_empty[0]);
-        }
-        for (int j = 0; j < nt && ok; ++j) {
-            for (int g = 0; g < groups && ok; ++g) {
-                if (g == 0) ok = role_wait(&ms.v_full[j & 1], (j >> 1) & 1, abort_flag);
-                ok = ok && role_wait(&ms.p_full[g], j & 1, abort_flag);
-                if (!ok) break;
+        bool ok = true;
+        int tiles = 0, mine[2] = {0, 0}, units[2] = {0, 0};         // so far: tiles, and tiles and units of each group
+        for (int n = 0; ok && pre_unit(n) < pp.units; ++n) {
+            const PreUnit un(pp, pre_unit(n));
+            if (un.nt == 0) continue;
+            for (int g = 0; g < un.groups && ok; ++g) ok = role_wait(&ms.q_ready[g], units[g]++ & 1, abort_flag);
+            ok = ok && role_wait(&ms.k_full[tiles & 1], (tiles >> 1) & 1, abort_flag);
+            if (ok) {
                 tc_fence_after();
-                const uint32_t va = base + SM::kV + (j & 1) * SM::kVStage;
-#pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    const uint64_t bd = umma_desc_sw128(va + s * SM::kSubV);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)                     // 16 positions each: 8 columns of P
-                        umma_f16_ts(tmem + 256 + g * D, tmem + g * 128 + 32 * s + 8 * k, bd + 2u * k, id_o,
-                                    (j | s | k) != 0);
-                }
-                umma_commit(&ms.pv_done[g]);
-                if (g == groups - 1) umma_commit(&ms.v_empty[j & 1]);
-                if (j + 1 == nt) continue;
-                // the next scores take the place of P: after its product is done
-                if (g == 0) ok = role_wait(&ms.k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, abort_flag);
-                ok = ok && role_wait(&ms.pv_done[g], j & 1, abort_flag);
-                if (!ok) break;
-                tc_fence_after();
-                qk(g, j + 1);
-                if (g == groups - 1) umma_commit(&ms.k_empty[(j + 1) & 1]);
+                for (int g = 0; g < un.groups; ++g) qk(g, tiles & 1);
+                umma_commit(&ms.k_empty[tiles & 1]);
             }
+            for (int j = 0; j < un.nt && ok; ++j) {
+                const int t = tiles + j, st = t & 1;
+                for (int g = 0; g < un.groups && ok; ++g) {
+                    if (g == 0) ok = role_wait(&ms.v_full[st], (t >> 1) & 1, abort_flag);
+                    ok = ok && role_wait(&ms.p_full[g], (mine[g] + j) & 1, abort_flag);
+                    if (!ok) break;
+                    tc_fence_after();
+                    uint64_t bd = umma_desc_sw128(base + SM::kV + st * SM::kVStage);
+                    uint32_t pa = tmem + g * 128;
+#pragma unroll 1
+                    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)                 // 16 positions each: 8 columns of P
+                            umma_f16_ts(tmem + 256 + g * D, pa + 8 * k, bd + 2u * k, id_o, (j | s | k) != 0);
+                        pa += 32;
+                        bd += SM::kSubV >> 4;
+                    }
+                    umma_commit(&ms.pv_done[g]);
+                    if (g == un.groups - 1) umma_commit(&ms.v_empty[st]);
+                    if (j + 1 == un.nt) continue;
+                    // the next scores take the place of P: after its product is done
+                    if (g == 0) ok = role_wait(&ms.k_full[st ^ 1], ((t + 1) >> 1) & 1, abort_flag);
+                    ok = ok && role_wait(&ms.pv_done[g], (mine[g] + j) & 1, abort_flag);
+                    if (!ok) break;
+                    tc_fence_after();
+                    qk(g, st ^ 1);
+                    if (g == un.groups - 1) umma_commit(&ms.k_empty[st ^ 1]);
+                }
+            }
+            tiles += un.nt;
+            for (int g = 0; g < un.groups; ++g) mine[g] += un.nt;
         }
         // nothing in flight when tensor memory goes
         umma_commit(&ms.drain);
@@ -651,7 +841,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const __gri
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (warp == 16) {
+    if (warp == 12) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512) : "memory");
     }
@@ -720,12 +910,13 @@ int kv4_prefill(Kv4AttendParams p, int64_t D, void *workspace, cudaStream_t st) 
     pp.items = p.B * p.KV;
     pp.row_tiles = (p.R + kPreRows - 1) / kPreRows;
     const int64_t ctas = (int64_t)pp.items * pp.row_tiles;
-    if (ctas > 0x7fffffffLL) return set_error(BF16X_ERR_UNSUPPORTED, "bf16x_kv4_attend: too many query rows");
     pp.nsplit = prefill_splits(ctas, p.max_seq);
+    if (ctas * pp.nsplit > 0x3fffffffLL) return set_error(BF16X_ERR_UNSUPPORTED, "bf16x_kv4_attend: too many query rows");
+    pp.units = (int)(ctas * pp.nsplit);
     p.part_o = (float *)workspace;
     p.part_ml = (float2 *)((uint8_t *)workspace + (int64_t)pp.items * pp.nsplit * p.R * D * 4);
     pp.a = p;
-    const dim3 grid((unsigned)ctas, (unsigned)pp.nsplit);
+    const dim3 grid((unsigned)std::min(pp.units, 148));
     const int rc = D == 64 ? launch_kv4<kv4_prefill_kernel<64>>(grid, kPreThreads, PreSmem<64>::kBytes, st, "kv4_prefill_kernel", pp)
                            : launch_kv4<kv4_prefill_kernel<128>>(grid, kPreThreads, PreSmem<128>::kBytes, st, "kv4_prefill_kernel", pp);
     if (rc != BF16X_OK || pp.nsplit == 1) return rc;
