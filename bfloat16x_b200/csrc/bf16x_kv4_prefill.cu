@@ -186,12 +186,18 @@ __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint3
 }
 __device__ __forceinline__ bool finite_bits(uint32_t b) { return (b & 0x7F800000u) != 0x7F800000u; }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 // A tile that every row of the warp sees whole, with one dk and dv: the maximum
 // of a row's scores.
 __device__ __forceinline__ float pre_top(uint32_t t_s) {
-    float mx[8];
+    float mx[4];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) mx[q] = -__builtin_huge_valf();
+    for (int q = 0; q < 4; ++q) mx[q] = -__builtin_huge_valf();
 #pragma unroll 1
     for (int c = 0; c < 2; ++c) {
         uint32_t v[2][32];
@@ -200,11 +206,12 @@ __device__ __forceinline__ float pre_top(uint32_t t_s) {
         tmem_got32(v[0]);
         tmem_got32(v[1]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < 16; i += 2)
 #pragma unroll
-            for (int q = 0; q < 8; ++q) mx[q] = fmaxf(mx[q], __uint_as_float(v[q >> 2][8 * (q & 3) + i]));
+            for (int q = 0; q < 4; ++q)
+                mx[q] = max3(mx[q], __uint_as_float(v[q >> 1][16 * (q & 1) + i]), __uint_as_float(v[q >> 1][16 * (q & 1) + i + 1]));
     }
-    return fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
+    return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
 }
 
 // Its weights P = 2^(S fac + off), as fp16 over S (a chunk's P lies over scores
@@ -424,12 +431,18 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const __gri
                 const int ex = (int)(top >> 7) - 127;
                 const int e = top && ex < 128 ? min(max(13 - ex, -100), 110) : 0;
                 const float up = __uint_as_float((uint32_t)(127 + e) << 23) * (p.scale_log2 < 0.f ? -1.f : 1.f);
-#pragma unroll 2
-                for (int i = 0; i < LPR; ++i) {
-                    const uint32_t at = q_row + (i >> 3) * SM::kSubK + (((i ^ lane) & 7) << 4);
-                    const uint4 x = lds128(at);                     // channels (0 4) (1 5) (2 6) (3 7)
-                    sts128(at, pack_f16x2(bf_lo(x.x) * up, bf_lo(x.z) * up), pack_f16x2(bf_hi(x.x) * up, bf_hi(x.z) * up),
-                           pack_f16x2(bf_lo(x.y) * up, bf_lo(x.w) * up), pack_f16x2(bf_hi(x.y) * up, bf_hi(x.w) * up));
+#pragma unroll 1
+                for (int n = 0; n < LPR; n += 4) {
+                    uint4 w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[i] = lds128(q_row + (n >> 3) * SM::kSubK + ((((n + i) ^ lane) & 7) << 4));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint4 x = w[i];                       // channels (0 4) (1 5) (2 6) (3 7)
+                        sts128(q_row + (n >> 3) * SM::kSubK + ((((n + i) ^ lane) & 7) << 4),
+                               pack_f16x2(bf_lo(x.x) * up, bf_lo(x.z) * up), pack_f16x2(bf_hi(x.x) * up, bf_hi(x.z) * up),
+                               pack_f16x2(bf_lo(x.y) * up, bf_lo(x.w) * up), pack_f16x2(bf_hi(x.y) * up, bf_hi(x.w) * up));
+                    }
                 }
                 c_row = fabsf(p.scale_log2) * __uint_as_float((uint32_t)(127 - e) << 23);
                 fence_proxy_async_smem();
