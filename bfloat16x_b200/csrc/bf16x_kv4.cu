@@ -896,8 +896,11 @@ __global__ void __launch_bounds__(WPR > 8 ? WPR * 32 : 256) kv4_join_kernel(cons
         *reinterpret_cast<uint32_t *>(dst + i) = pack_bf16x2(acc[i] * inv, acc[i + 1] * inv);
 }
 
-// Rows per kv head up to which the kernel of this file takes a call; above, the prompt kernel.
-constexpr int64_t kFewRows = 16;
+// Rows per kv head up to which the kernel of this file takes a call; above, the
+// prompt kernel.  8B heads (4 per kv head): 8 tokens (32 rows) of 4 sequences of
+// 8192 positions take 39 us here and 55 us there, 12 tokens (48 rows) of one
+// sequence 22 and 27 us, 16 tokens (64 rows) of 4 sequences 66 and 55 us.
+constexpr int64_t kFewRows = 48;
 
 // Column tiles of 8 rows that one warp takes, and the grid.
 static int attend_tiles(int64_t R) { return R > 8 ? 2 : 1; }
@@ -976,7 +979,7 @@ extern "C" int bf16x_kv4_read(const uint8_t *blocks, int64_t max_seq, int64_t B,
 extern "C" int64_t bf16x_kv4_attend_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t KV, int64_t D,
                                                     int64_t max_seq) {
     if (B <= 0 || T <= 0 || H <= 0 || KV <= 0 || H % KV || max_seq <= 0) return 0;
-    if (T * (H / KV) > kFewRows) return kv4_prefill_workspace(B, KV, T * (H / KV), D, max_seq);
+    if (T * (H / KV) > kFewRows) return kv4_prefill_workspace(B, KV, T * (H / KV), T, D, max_seq);
     const int nt = attend_tiles(T * (H / KV));
     const int64_t units = B * KV * ((T * (H / KV) + 8 * nt - 1) / (8 * nt));
     return (int64_t)attend_warps(nt) * 2 * 8 * nt * (D * 4 + 8) + units * 8;

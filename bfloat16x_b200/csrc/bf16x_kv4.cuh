@@ -170,7 +170,7 @@ static int launch_kv4(dim3 grid, unsigned block, size_t smem, cudaStream_t st, c
 }
 
 // Attention of many rows per kv head (bf16x_kv4_prefill.cu): its workspace, and its launch.
-int64_t kv4_prefill_workspace(int64_t B, int64_t KV, int64_t R, int64_t D, int64_t max_seq);
+int64_t kv4_prefill_workspace(int64_t B, int64_t KV, int64_t R, int64_t T, int64_t D, int64_t max_seq);
 int kv4_prefill(Kv4AttendParams p, int64_t D, void *workspace, cudaStream_t st);
 
 }  // namespace bf16x

@@ -49,6 +49,8 @@ namespace bf16x {
 constexpr int kPreRows = 256;                         // rows per unit
 constexpr int kPreKeys = 128;                         // positions per tile
 constexpr int kPreThreads = 13 * 32;
+constexpr int kPreCut = 4 * 148;                      // units, up to which they may be cut
+constexpr int kPreUnitCost = 2;                       // of a unit's start and end, in tiles
 
 template <int D>
 struct PreSmem {
@@ -62,7 +64,8 @@ struct PreSmem {
     static constexpr int kScale = kV + 2 * kVStage;   // fp16, two buffers: V's d [NG][128], m [NG][128]
     static constexpr int kScaleBytes = 2 * kPreKeys * NG * 2;
     static constexpr int kMisc = kScale + 2 * kScaleBytes;
-    static constexpr int kBytes = kMisc + 7424 + 1024;              // alignment slack
+    static constexpr int kPlan = kMisc + 7424;        // PrePlan
+    static constexpr int kBytes = kPlan + 2560 + 1024;              // alignment slack
 };
 
 struct PreMisc {
@@ -78,6 +81,11 @@ struct PreMisc {
     uint32_t bad[4][kPreKeys / 4];                    // per position a byte: its V groups that are not finite
 };
 static_assert(sizeof(PreMisc) <= 7424, "PreMisc");
+struct PrePlan {
+    int start[kPreCut + 1];                           // of the units, each nt + kPreUnitCost long
+    int sum[kPreThreads / 32];
+};
+static_assert(sizeof(PrePlan) <= 2560, "PrePlan");
 
 __device__ __forceinline__ void tmem_ld32(uint32_t a, uint32_t (&v)[32]) {
     asm volatile(
@@ -311,34 +319,117 @@ __device__ __forceinline__ float pre_weights_any(uint32_t t_s, const PreMisc &ms
 
 struct PreParams {
     Kv4AttendParams a;
-    int items, nsplit, row_tiles, units;
+    int items, row_tiles, units;
+    int *held;                          // units that may be cut: whether units are cut, then first and last CTA of each
 };
 
-// Unit u: 256 rows of one kv head and a part of the positions that they see.
-// The row tiles that see most come first; CTA c of n takes units c, 2 n - 1 - c,
-// 2 n + c, ..., so that one of the longest goes with one of the shortest.
+// Unit u: 256 rows of one kv head; the row tiles that see most come first.  A
+// piece of it: nt tiles of positions from tile t0 on.
 struct PreUnit {
-    int item, b, kvh, row0, split, nt, groups;
-    int64_t pos0, n_keys, t0;           // positions that some row sees; first tile
-    __device__ __forceinline__ PreUnit(const PreParams &pp, int u) {
+    int b, kvh, row0, t0, nt, groups;
+    int slot;                           // where the piece's sums go; -1: it is the whole unit
+    int64_t pos0, n_keys;               // positions that some row sees
+    __device__ __forceinline__ void set(const PreParams &pp, int u) {
         const Kv4AttendParams &p = pp.a;
-        const int per_tile = pp.items * pp.nsplit, rest = u % per_tile;
-        split = rest / pp.items;
-        item = rest - split * pp.items;
+        const int tile = u / pp.items, item = u - tile * pp.items;
         b = item / p.KV;
-        kvh = item - b * p.KV;
-        row0 = (pp.row_tiles - 1 - u / per_tile) * kPreRows;
         pos0 = p.pos0[(int64_t)b * p.pos_stride];
+        kvh = item - b * p.KV;
+        row0 = (pp.row_tiles - 1 - tile) * kPreRows;
         n_keys = max(min(pos0 + min(row0 + kPreRows - 1, p.R - 1) / p.G + 1, p.max_seq), (int64_t)0);
-        const uint32_t all = (uint32_t)((n_keys + kPreKeys - 1) / kPreKeys);       // (times 148 splits: below 2^32)
-        t0 = all * (uint32_t)split / (uint32_t)pp.nsplit;
-        nt = (int)(all * (uint32_t)(split + 1) / (uint32_t)pp.nsplit - (uint32_t)t0);
         groups = p.R - row0 > 128 ? 2 : 1;
+        slot = -1;
+        t0 = 0;
+        nt = (int)((n_keys + kPreKeys - 1) / kPreKeys);
     }
 };
-__device__ __forceinline__ int pre_unit(int i) {                    // the i-th unit of this CTA
-    const int n = (int)gridDim.x, c = (int)blockIdx.x;
-    return i & 1 ? (i + 1) * n - 1 - c : i * n + c;
+
+// The pieces of a CTA.  Whole units: CTA c of n takes units c, 2 n - 1 - c,
+// 2 n + c, ..., so that one of the longest goes with one of the shortest.  Or
+// all units in a row, cut into equal shares, one per CTA.
+struct PreWalk {
+    int share;                          // 0: whole units
+    int i;
+    const int *start;
+    __device__ __forceinline__ PreWalk(const PreParams &pp, const PrePlan &plan, int share_) : share(share_), i(0), start(plan.start) {
+        if (share) {                    // the last unit that starts at or before the share
+            int hi = pp.units;
+            while (hi - i > 1) {
+                const int mid = (i + hi) >> 1;
+                if (start[mid] <= (int)blockIdx.x * share) i = mid;
+                else hi = mid;
+            }
+        }
+    }
+    __device__ __forceinline__ bool next(const PreParams &pp, PreUnit &un) {
+        if (!share) {
+            const int n = (int)gridDim.x, c = (int)blockIdx.x, u = i & 1 ? (i + 1) * n - 1 - c : i * n + c;
+            if (u >= pp.units) return false;
+            ++i;
+            un.set(pp, u);
+            return true;
+        }
+        for (; i < pp.units && start[i] < ((int)blockIdx.x + 1) * share; ++i) {
+            const int a = (int)blockIdx.x * share - start[i], all = start[i + 1] - start[i] - kPreUnitCost;
+            const int lo = max(a - kPreUnitCost, 0), hi = min(a + share - kPreUnitCost, all);
+            if (hi <= lo && (all > 0 || a > 0)) continue;           // (a unit without tiles is zeros, from where it starts)
+            un.set(pp, i++);
+            un.t0 = lo;
+            un.nt = max(hi - lo, 0);
+            if (un.nt < all) un.slot = 2 * (int)blockIdx.x + (lo == 0);
+            return true;
+        }
+        return false;
+    }
+};
+
+// How the units go over the CTAs: 0 for whole units, else a CTA's share.  Units
+// are cut when that ends earlier by more than what it costs to write the sums
+// of the pieces and to join them.
+__device__ __forceinline__ int pre_plan(const PreParams &pp, PrePlan &plan) {
+    constexpr int kJoinCost = 2;
+    const int tid = threadIdx.x, lane = tid & 31, n = (int)gridDim.x;
+    int before = 0;
+    for (int u0 = 0; u0 < pp.units; u0 += kPreThreads) {            // running sum of the units' costs
+        int cost = 0;
+        if (u0 + tid < pp.units) {
+            PreUnit un;
+            un.set(pp, u0 + tid);
+            cost = un.nt + kPreUnitCost;
+        }
+        int x = cost;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 31) plan.sum[tid >> 5] = x;
+        __syncthreads();
+        int all = before;
+        for (int w = 0; w < kPreThreads / 32; ++w) {
+            if (w < tid >> 5) x += plan.sum[w];
+            all += plan.sum[w];
+        }
+        if (u0 + tid < pp.units) plan.start[u0 + tid] = before + x - cost;
+        before = all;
+        __syncthreads();
+    }
+    if (tid == 0) plan.start[pp.units] = before;
+    __syncthreads();
+    const int share = max((before + n - 1) / n, 2 * kPreUnitCost);
+    int load = 0;
+    if (tid < n)
+        for (int i = 0, u = tid; u < pp.units; ++i, u = i & 1 ? (i + 1) * n - 1 - tid : i * n + tid)
+            load += plan.start[u + 1] - plan.start[u];
+    const bool cut = __syncthreads_or(load > share + kJoinCost);
+    if (blockIdx.x == 0) {
+        for (int u = tid; u < pp.units; u += kPreThreads) {
+            const int first = plan.start[u] + kPreUnitCost, last = max(plan.start[u + 1] - 1, first);
+            reinterpret_cast<int2 *>(pp.held)[1 + u] = make_int2(first / share, last / share);
+        }
+        if (tid == 0) pp.held[0] = cut;
+    }
+    return cut ? share : 0;
 }
 
 template <int D>
@@ -351,6 +442,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const __gri
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     PreMisc &ms = *reinterpret_cast<PreMisc *>(smem + SM::kMisc);
     volatile int *abort_flag = &ms.abort_flag;
+    PrePlan &plan = *reinterpret_cast<PrePlan *>(smem + SM::kPlan);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     griddep_launch_dependents();
     if (tid == 0) {
@@ -381,6 +473,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const __gri
     const uint32_t tmem = ms.tmem;
     const uint32_t base = smem_u32(smem);
     griddep_wait();
+    const int share = pp.held ? pre_plan(pp, plan) : 0;
 
     if (warp < 8) {
         // ------------------------------------------------------------ softmax
@@ -389,12 +482,12 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const __gri
         const uint32_t t_s = tmem + t_lane + grp * 128, t_o = tmem + t_lane + 256 + grp * D;
         bool ok = true;
         int tiles = 0, mine = 0;                                    // tiles before this unit: of all, and of this group
-        for (int n = 0; ok && pre_unit(n) < pp.units; ++n) {
-            const PreUnit un(pp, pre_unit(n));
+        PreWalk walk(pp, plan, share);
+        for (PreUnit un; ok && walk.next(pp, un);) {
             const int row = un.row0 + grp * 128 + rl;
             const bool have = row < p.R;
             const int tok = have ? row / p.G : 0, hh = have ? row - tok * p.G : 0;
-            if (grp == 0 && un.split == 0 && un.kvh == 0 && have && hh == 0 && un.pos0 + tok >= p.max_seq)
+            if (grp == 0 && un.t0 == 0 && un.kvh == 0 && have && hh == 0 && un.pos0 + tok >= p.max_seq)
                 atomicOr(&g_status, kErrBadIndex);
             if (grp >= un.groups) {
                 tiles += un.nt;
@@ -452,7 +545,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const __gri
             }
             // positions that this row sees, from the first tile on
             const int64_t at = have ? un.pos0 + tok : -1;
-            const int64_t sees = at < 0 || at >= p.max_seq ? 0 : max(at + 1 - un.t0 * kPreKeys, (int64_t)0);
+            const int64_t sees = at < 0 || at >= p.max_seq ? 0 : max(at + 1 - (int64_t)un.t0 * kPreKeys, (int64_t)0);
             // a row that sees nothing here (padding, no row) goes along as if it saw all, and is zeros at the end
             float M = kNoMax, l = 0.f;
             uint32_t bad = 0;
@@ -507,27 +600,27 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const __gri
             if (!ok) break;
             tc_fence_after();
             // ---- out, by way of Q's place (its products are done): 128 bytes of 4 rows per store
+            const bool part = un.slot >= 0;
+            const int64_t in_slot = (int64_t)un.slot * kPreRows + grp * 128 + rl;
             int64_t off = -1;                                       // bytes of this row from the start
-            if (have)
-                off = pp.nsplit > 1 ? (((int64_t)un.item * pp.nsplit + un.split) * p.R + row) * D * 4
-                                    : (((int64_t)un.b * p.T + tok) * p.H + un.kvh * p.G + hh) * D * 2;
-            if (have && pp.nsplit > 1) p.part_ml[off / (D * 4)] = make_float2(sees ? M : kNoMax, sees ? l : 0.f);
-            uint8_t *dst = pp.nsplit > 1 ? reinterpret_cast<uint8_t *>(p.part_o) : reinterpret_cast<uint8_t *>(p.out);
-            const float inv = pp.nsplit > 1 ? 1.f : l != 0.f ? 1.f / l : 0.f;
-            const int per = pp.nsplit > 1 ? 2 : 4;                  // 16 channels each: together 128 bytes, a piece
+            if (have) off = part ? in_slot * D * 4 : (((int64_t)un.b * p.T + tok) * p.H + un.kvh * p.G + hh) * D * 2;
+            if (have && part) p.part_ml[in_slot] = make_float2(sees ? M : kNoMax, sees ? l : 0.f);
+            uint8_t *dst = part ? reinterpret_cast<uint8_t *>(p.part_o) : reinterpret_cast<uint8_t *>(p.out);
+            const float inv = part ? 1.f : l != 0.f ? 1.f / l : 0.f;
+            const int per = part ? 2 : 4;                  // 16 channels each: together 128 bytes, a piece
 #pragma unroll 1
             for (int c = 0; c < D / 16; ++c) {
-                const int piece = c / per, part = c % per;
+                const int piece = c / per, nth = c % per;
                 const float f = (bad >> (c >> 1)) & 1u ? __int_as_float(0x7fc00000) : inv;
                 uint32_t v[16];
                 tmem_ld16(t_o + 16 * c, v);
 #pragma unroll
                 for (int k = 0; k < 16; ++k) v[k] = sees ? __float_as_uint(__uint_as_float(v[k]) * f) : 0u;
                 const uint32_t at = base + (grp * SUBS + piece % SUBS) * SM::kSubK + (warp & 3) * 4096;
-                if (pp.nsplit > 1) {
+                if (part) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        sts128(at + lane * 128 + (((4 * part + i) ^ lane) & 7) * 16, v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                        sts128(at + lane * 128 + (((4 * nth + i) ^ lane) & 7) * 16, v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
                 } else {
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
@@ -535,10 +628,10 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const __gri
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
                             w[k] = pack_bf16x2(__uint_as_float(v[8 * i + 2 * k]), __uint_as_float(v[8 * i + 2 * k + 1]));
-                        sts128(at + lane * 128 + (((2 * part + i) ^ lane) & 7) * 16, w[0], w[1], w[2], w[3]);
+                        sts128(at + lane * 128 + (((2 * nth + i) ^ lane) & 7) * 16, w[0], w[1], w[2], w[3]);
                     }
                 }
-                if (part + 1 < per) continue;
+                if (nth + 1 < per) continue;
                 __syncwarp();
 #pragma unroll 2
                 for (int i = 0; i < 8; ++i) {
@@ -558,25 +651,26 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const __gri
         // Scales are prepared one tile ahead of the codes, and the tile's
         // largest exponents before that, so the warps meet once per tile, long
         // after they have arrived.
-        // The tiles of all units follow one another; the loads look ahead.
+        // The tiles of all pieces follow one another; the loads look ahead.
         const int dw = warp - 8, key = tid - 256, vp = (dw >> 1) * 8 + (lane & 7), vg = (dw & 1) * 4 + (lane >> 3);
         struct Tile {                                               // where a tile lies
             const uint8_t *cache;                                   // its head's blocks
             int64_t blk;                                            // its first block
             int live;                                               // positions that some row sees; 0: no more tiles
         };
-        struct Feed {                                               // the tiles of this CTA's units, one after the other
-            int n, left;                                            // next unit; tiles left of this one
+        struct Feed {                                               // the tiles of this CTA's pieces, one after the other
+            PreWalk walk;
+            int left;                                               // tiles left of this piece
             Tile tl;
-            int64_t keys;                                           // positions left of this unit
-        } feed = {0, 0, {p.blocks, 0, 0}, 0};
+            int64_t keys;                                           // positions left of its unit
+        } feed = {PreWalk(pp, plan, share), 0, {p.blocks, 0, 0}, 0};
         const auto next_tile = [&]() -> Tile {
-            while (feed.left == 0 && pre_unit(feed.n) < pp.units) {
-                const PreUnit un(pp, pre_unit(feed.n++));
+            PreUnit un;
+            while (feed.left == 0 && feed.walk.next(pp, un)) {
                 feed.left = un.nt;
                 feed.tl.cache = p.blocks + ((int64_t)un.b * p.KV + un.kvh) * p.nblk * L::kBytes;
-                feed.tl.blk = un.t0 * (kPreKeys / kKvBlock);
-                feed.keys = un.n_keys - un.t0 * kPreKeys;
+                feed.tl.blk = (int64_t)un.t0 * (kPreKeys / kKvBlock);
+                feed.keys = un.n_keys - (int64_t)un.t0 * kPreKeys;
             }
             Tile t = feed.tl;
             t.live = feed.left ? (int)min(feed.keys, (int64_t)kPreKeys) : 0;
@@ -805,8 +899,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const __gri
         };
         bool ok = true;
         int tiles = 0, mine[2] = {0, 0}, units[2] = {0, 0};         // so far: tiles, and tiles and units of each group
-        for (int n = 0; ok && pre_unit(n) < pp.units; ++n) {
-            const PreUnit un(pp, pre_unit(n));
+        PreWalk walk(pp, plan, share);
+        for (PreUnit un; ok && walk.next(pp, un);) {
             if (un.nt == 0) continue;
             for (int g = 0; g < un.groups && ok; ++g) ok = role_wait(&ms.q_ready[g], units[g]++ & 1, abort_flag);
             ok = ok && role_wait(&ms.k_full[tiles & 1], (tiles >> 1) & 1, abort_flag);
@@ -860,80 +954,96 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const __gri
     }
 }
 
-// The splits of the positions joined, one warp per row.
+// The sums of the units that were cut, joined: one warp per row.
 template <int D>
 __global__ void __launch_bounds__(256) kv4_prefill_join_kernel(const __grid_constant__ PreParams pp) {
     constexpr int V = D / 32;
     const Kv4AttendParams &p = pp.a;
+    const int lane = threadIdx.x & 31;
     griddep_launch_dependents();
     griddep_wait();
-    const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);        // item * R + r
-    const int lane = threadIdx.x & 31;
-    if (at >= (int64_t)pp.items * p.R) return;
-    const int64_t item = at / p.R;
-    const int r = (int)(at - item * p.R);
-    const auto slot = [&](int s) { return (item * pp.nsplit + s) * p.R + r; };
-    float top = kNoMax;
-    for (int s = lane; s < pp.nsplit; s += 32) top = fmaxf(top, p.part_ml[slot(s)].x);
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float acc[V], l = 0.f;
+    if (!pp.held[0]) return;
+    for (int task = blockIdx.x; task < pp.units * (kPreRows / 8); task += gridDim.x) {
+        const int u = task / (kPreRows / 8), tile = u / pp.items, item = u - tile * pp.items;
+        const int in_unit = task % (kPreRows / 8) * 8 + (threadIdx.x >> 5), r = (pp.row_tiles - 1 - tile) * kPreRows + in_unit;
+        const int2 held = reinterpret_cast<const int2 *>(pp.held)[1 + u];
+        if (held.x == held.y || r >= p.R) continue;
+        const int n = held.y - held.x + 1;
+        const auto slot = [&](int s) { return (int64_t)(2 * (held.x + s) + (s == 0)) * kPreRows + in_unit; };
+        float top = kNoMax;
+        for (int s = lane; s < n; s += 32) top = fmaxf(top, p.part_ml[slot(s)].x);
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        float acc[V], l = 0.f;
 #pragma unroll
-    for (int i = 0; i < V; ++i) acc[i] = 0.f;
+        for (int i = 0; i < V; ++i) acc[i] = 0.f;
 #pragma unroll 8
-    for (int s = 0; s < pp.nsplit; ++s) {
-        const float2 x = p.part_ml[slot(s)];
-        const float f = ex2(x.x - top);
-        l += x.y * f;
-        const float *src = p.part_o + slot(s) * D + lane * V;
-        if constexpr (V == 4) {
-            const float4 y = *reinterpret_cast<const float4 *>(src);
-            acc[0] = fmaf(y.x, f, acc[0]);
-            acc[1] = fmaf(y.y, f, acc[1]);
-            acc[2] = fmaf(y.z, f, acc[2]);
-            acc[3] = fmaf(y.w, f, acc[3]);
-        } else {
-            const float2 y = *reinterpret_cast<const float2 *>(src);
-            acc[0] = fmaf(y.x, f, acc[0]);
-            acc[1] = fmaf(y.y, f, acc[1]);
+        for (int s = 0; s < n; ++s) {
+            const float2 x = p.part_ml[slot(s)];
+            const float f = ex2(x.x - top);
+            l += x.y * f;
+            const float *src = p.part_o + slot(s) * D + lane * V;
+            if constexpr (V == 4) {
+                const float4 y = *reinterpret_cast<const float4 *>(src);
+                acc[0] = fmaf(y.x, f, acc[0]);
+                acc[1] = fmaf(y.y, f, acc[1]);
+                acc[2] = fmaf(y.z, f, acc[2]);
+                acc[3] = fmaf(y.w, f, acc[3]);
+            } else {
+                const float2 y = *reinterpret_cast<const float2 *>(src);
+                acc[0] = fmaf(y.x, f, acc[0]);
+                acc[1] = fmaf(y.y, f, acc[1]);
+            }
         }
-    }
-    const float inv = l != 0.f ? 1.f / l : 0.f;
-    const int64_t b = item / p.KV;
-    const int kvh = (int)(item - b * p.KV), tok = r / p.G, hh = r - tok * p.G;
-    uint16_t *dst = p.out + ((b * p.T + tok) * p.H + kvh * p.G + hh) * D + lane * V;
+        const float inv = l != 0.f ? 1.f / l : 0.f;
+        const int64_t b = item / p.KV;
+        const int kvh = item - (int)b * p.KV, tok = r / p.G, hh = r - tok * p.G;
+        uint16_t *dst = p.out + ((b * p.T + tok) * p.H + kvh * p.G + hh) * D + lane * V;
 #pragma unroll
-    for (int i = 0; i < V; i += 2)
-        *reinterpret_cast<uint32_t *>(dst + i) = pack_bf16x2(acc[i] * inv, acc[i + 1] * inv);
+        for (int i = 0; i < V; i += 2)
+            *reinterpret_cast<uint32_t *>(dst + i) = pack_bf16x2(acc[i] * inv, acc[i + 1] * inv);
+    }
 }
 
-// Splits of the positions: where there are fewer row tiles than SMs, at least
-// two tiles of positions each.
-static int prefill_splits(int64_t ctas, int64_t max_seq) {
-    return (int)std::max<int64_t>(1, std::min<int64_t>(148 / ctas, max_seq / (2 * kPreKeys)));
+static int64_t prefill_units(int64_t B, int64_t KV, int64_t R) { return B * KV * ((R + kPreRows - 1) / kPreRows); }
+
+// Units may be cut where whole ones can leave CTAs idle: fewer units than CTAs,
+// or up to four per CTA over a long cache.  A prompt from its first token on (a
+// cache of at most twice its tokens) with more units than CTAs goes well in whole
+// units, of which the longest go with the shortest: planning and a second kernel
+// made 2048 tokens of the 8B heads 4 us slower (60 -> 64); 3 x 511 tokens of 8
+// heads of 64 channels behind 333 to 7003 positions, 48 units, went from 63 us
+// with equal cuts of each unit to 47.  (The costs' sum has to fit 31 bits.)
+static bool prefill_may_cut(int64_t B, int64_t KV, int64_t R, int64_t T, int64_t max_seq) {
+    const int64_t units = prefill_units(B, KV, R);
+    return units <= kPreCut && (units < 148 || max_seq > 2 * T) &&
+           units * (max_seq / kPreKeys + 1 + kPreUnitCost) <= (1 << 30);
 }
 
-int64_t kv4_prefill_workspace(int64_t B, int64_t KV, int64_t R, int64_t D, int64_t max_seq) {
-    const int64_t items = B * KV;
-    const int n = prefill_splits(items * ((R + kPreRows - 1) / kPreRows), max_seq);
-    return n == 1 ? 0 : items * n * R * (D * 4 + 8);
+// Two pieces per CTA that are not whole units, and who holds what.
+int64_t kv4_prefill_workspace(int64_t B, int64_t KV, int64_t R, int64_t T, int64_t D, int64_t max_seq) {
+    return !prefill_may_cut(B, KV, R, T, max_seq) ? 0 : 2 * 148 * kPreRows * (D * 4 + 8) + (kPreCut + 1) * 8;
 }
 
 int kv4_prefill(Kv4AttendParams p, int64_t D, void *workspace, cudaStream_t st) {
     PreParams pp = {};
+    const int64_t units = prefill_units(p.B, p.KV, p.R);
+    if (units > 0x3fffffffLL) return set_error(BF16X_ERR_UNSUPPORTED, "bf16x_kv4_attend: too many query rows");
     pp.items = p.B * p.KV;
     pp.row_tiles = (p.R + kPreRows - 1) / kPreRows;
-    const int64_t ctas = (int64_t)pp.items * pp.row_tiles;
-    pp.nsplit = prefill_splits(ctas, p.max_seq);
-    if (ctas * pp.nsplit > 0x3fffffffLL) return set_error(BF16X_ERR_UNSUPPORTED, "bf16x_kv4_attend: too many query rows");
-    pp.units = (int)(ctas * pp.nsplit);
-    p.part_o = (float *)workspace;
-    p.part_ml = (float2 *)((uint8_t *)workspace + (int64_t)pp.items * pp.nsplit * p.R * D * 4);
+    pp.units = (int)units;
+    const bool may_cut = prefill_may_cut(p.B, p.KV, p.R, p.T, p.max_seq);
+    if (may_cut) {
+        const int64_t rows = 2 * 148 * kPreRows;
+        p.part_o = (float *)workspace;
+        p.part_ml = (float2 *)((uint8_t *)workspace + rows * D * 4);
+        pp.held = (int *)((uint8_t *)workspace + rows * (D * 4 + 8));
+    }
     pp.a = p;
-    const dim3 grid((unsigned)std::min(pp.units, 148));
+    const dim3 grid(148);
     const int rc = D == 64 ? launch_kv4<kv4_prefill_kernel<64>>(grid, kPreThreads, PreSmem<64>::kBytes, st, "kv4_prefill_kernel", pp)
                            : launch_kv4<kv4_prefill_kernel<128>>(grid, kPreThreads, PreSmem<128>::kBytes, st, "kv4_prefill_kernel", pp);
-    if (rc != BF16X_OK || pp.nsplit == 1) return rc;
-    const dim3 jgrid((unsigned)(((int64_t)pp.items * p.R + 7) / 8));
+    if (rc != BF16X_OK || !may_cut) return rc;
+    const dim3 jgrid((unsigned)std::min(pp.units * (kPreRows / 8), 148 * 8));
     return D == 64 ? launch_kv4<kv4_prefill_join_kernel<64>>(jgrid, 256, 0, st, "kv4_prefill_join_kernel", pp)
                    : launch_kv4<kv4_prefill_join_kernel<128>>(jgrid, 256, 0, st, "kv4_prefill_join_kernel", pp);
 }

@@ -156,6 +156,20 @@ def test_attend_many_tokens(D, T, H, KV, pos):
     _lib.check_device_status()
 
 
+@pytest.mark.parametrize("B,T,H,KV,S,pos", [
+    (20, 64, 32, 8, 64, (0, 0)),            # more units of rows than CTAs, each row tile whole
+    (40, 75, 8, 2, 120, (-75, 44)),         # two row tiles, the last with few rows; sequences that see nothing
+    (20, 64, 32, 8, 400, (-64, 336)),       # a long cache, units cut between CTAs
+    (3, 130, 4, 2, 1500, (-130, 1370)),     # few units, very different lengths
+    (2, 520, 2, 1, 2000, (1, 1480))])
+@pytest.mark.parametrize("D", [64, 128])
+def test_attend_schedules(D, B, T, H, KV, S, pos):
+    cache = _filled(B, KV, D, S, seed=T + S, stale=True)
+    q = torch.randn(B, T, H, D, generator=_gen(T + B)).to(torch.bfloat16)
+    _check(cache, q, torch.linspace(pos[0], pos[1], B).round().long())
+    _lib.check_device_status()
+
+
 @pytest.mark.parametrize("n", [1000, 4099])
 @pytest.mark.parametrize("T", [1, 3, 150])
 def test_attend_long(n, T):
