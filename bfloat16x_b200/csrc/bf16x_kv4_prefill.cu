@@ -55,6 +55,9 @@ constexpr int kPreUnitCost = 2;                       // of a unit's start and e
 template <int D>
 struct PreSmem {
     static constexpr int NG = D / 32;
+    // columns of tensor memory: S of both groups, O of both groups, and P, apart from S if there is room
+    static constexpr bool kApart = D == 64;
+    static constexpr int kPCol = kApart ? 256 + 2 * D : 0, kPStep = kApart ? 64 : 128;
     static constexpr int kSubK = kPreKeys * 128;      // [128 rows][64 columns] fp16
     static constexpr int kSubV = D * 128;             // [D rows][64 positions] fp16
     static constexpr int kK = 2 * (D / 64) * kSubK;   // offsets: Q of both groups first
@@ -222,8 +225,8 @@ __device__ __forceinline__ float pre_top(uint32_t t_s) {
     return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
 }
 
-// Its weights P = 2^(S fac + off), as fp16 over S (a chunk's P lies over scores
-// that were read before); returns their sum.
+// Its weights P = 2^(S fac + off), as fp16, over S if P has no place of its own
+// (a chunk's P lies over scores that were read before); returns their sum.
 __device__ __forceinline__ void pre_chunk(const uint32_t (&v)[32], uint32_t t_p, uint64_t f2, uint64_t o2, uint64_t (&sum2)[4]) {
     uint32_t o[16];
 #pragma unroll
@@ -242,7 +245,7 @@ __device__ __forceinline__ void pre_chunk(const uint32_t (&v)[32], uint32_t t_p,
     }
     tmem_st16(t_p, o);
 }
-__device__ __forceinline__ float pre_weights(uint32_t t_s, float fac, float off) {
+__device__ __forceinline__ float pre_weights(uint32_t t_s, uint32_t t_p, float fac, float off) {
     const uint64_t f2 = pack2(fac, fac), o2 = pack2(off, off);
     uint64_t sum2[4] = {};
     uint32_t a[32], b[32];
@@ -251,10 +254,10 @@ __device__ __forceinline__ float pre_weights(uint32_t t_s, float fac, float off)
 #pragma unroll 1
     for (int c = 0; c < 2; ++c) {                                   // the next chunk comes in while one is worked on
         tmem_ask32(t_s + 64 * c + 32, b);
-        pre_chunk(a, t_s + 32 * c, f2, o2, sum2);
+        pre_chunk(a, t_p + 32 * c, f2, o2, sum2);
         tmem_got32(b);
         if (c == 0) tmem_ask32(t_s + 64, a);
-        pre_chunk(b, t_s + 32 * c + 16, f2, o2, sum2);
+        pre_chunk(b, t_p + 32 * c + 16, f2, o2, sum2);
         if (c == 0) tmem_got32(a);
     }
     float x, y;
@@ -293,7 +296,7 @@ __device__ __forceinline__ float pre_top_any(uint32_t t_s, const PreMisc &ms, in
     }
     return mx;
 }
-__device__ __forceinline__ float pre_weights_any(uint32_t t_s, const PreMisc &ms, int slot, bool uneven, float c_row,
+__device__ __forceinline__ float pre_weights_any(uint32_t t_s, uint32_t t_p, const PreMisc &ms, int slot, bool uneven, float c_row,
                                                  float M, int vis) {
     float sum = 0.f;
 #pragma unroll 1
@@ -312,7 +315,7 @@ __device__ __forceinline__ float pre_weights_any(uint32_t t_s, const PreMisc &ms
             }
             o[i] = pack_f16x2(x[0], x[1]);
         }
-        tmem_st8(t_s + 8 * c, o);
+        tmem_st8(t_p + 8 * c, o);
     }
     return sum;
 }
@@ -437,6 +440,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const __gri
     using L = KvLayout<D>;
     using SM = PreSmem<D>;
     constexpr int NG = L::NG, NH = NG / 2, SUBS = D / 64;
+    constexpr bool kApart = SM::kApart;
     const Kv4AttendParams &p = pp.a;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -479,7 +483,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const __gri
         // ------------------------------------------------------------ softmax
         const int grp = warp >> 2, rl = (warp & 3) * 32 + lane;
         const uint32_t t_lane = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t t_s = tmem + t_lane + grp * 128, t_o = tmem + t_lane + 256 + grp * D;
+        const uint32_t t_s = tmem + t_lane + grp * 128, t_o = tmem + t_lane + 256 + grp * D,
+                       t_p = tmem + t_lane + SM::kPCol + grp * SM::kPStep;
         bool ok = true;
         int tiles = 0, mine = 0;                                    // tiles before this unit: of all, and of this group
         PreWalk walk(pp, plan, share);
@@ -584,8 +589,12 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const __gri
                         }
                     }
                 }
-                l += plain ? pre_weights(t_s, fac, dv - M) * ms.v_inv[slot][0]
-                           : pre_weights_any(t_s, ms, slot, uneven, c_row, M, vis);
+                if (kApart && j > 0 && !role_wait(&ms.pv_done[grp], (mine + j - 1) & 1, abort_flag)) {         // P is free
+                    ok = false;
+                    break;
+                }
+                l += plain ? pre_weights(t_s, t_p, fac, dv - M) * ms.v_inv[slot][0]
+                           : pre_weights_any(t_s, t_p, ms, slot, uneven, c_row, M, vis);
                 // (read before P is handed over: the slot is used again after that)
                 if (ms.any_bad[slot])
                     for (int k = 0; k < vis; ++k) bad |= (ms.bad[slot][k >> 2] >> (8 * (k & 3))) & 0xFFu;
@@ -912,12 +921,21 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const __gri
             for (int j = 0; j < un.nt && ok; ++j) {
                 const int t = tiles + j, st = t & 1;
                 for (int g = 0; g < un.groups && ok; ++g) {
-                    if (g == 0) ok = role_wait(&ms.v_full[st], (t >> 1) & 1, abort_flag);
-                    ok = ok && role_wait(&ms.p_full[g], (mine[g] + j) & 1, abort_flag);
+                    const bool last = g == un.groups - 1;
+                    if (kApart) ok = role_wait(&ms.p_full[g], (mine[g] + j) & 1, abort_flag);
+                    if (kApart && ok && j + 1 < un.nt) {            // the scores were read: the next ones
+                        if (g == 0) ok = role_wait(&ms.k_full[st ^ 1], ((t + 1) >> 1) & 1, abort_flag);
+                        if (!ok) break;
+                        tc_fence_after();
+                        qk(g, st ^ 1);
+                        if (last) umma_commit(&ms.k_empty[st ^ 1]);
+                    }
+                    if (ok && g == 0) ok = role_wait(&ms.v_full[st], (t >> 1) & 1, abort_flag);
+                    if (!kApart) ok = ok && role_wait(&ms.p_full[g], (mine[g] + j) & 1, abort_flag);
                     if (!ok) break;
                     tc_fence_after();
                     uint64_t bd = umma_desc_sw128(base + SM::kV + st * SM::kVStage);
-                    uint32_t pa = tmem + g * 128;
+                    uint32_t pa = tmem + SM::kPCol + g * SM::kPStep;
 #pragma unroll 1
                     for (int s = 0; s < 2; ++s) {
 #pragma unroll
@@ -927,15 +945,15 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const __gri
                         bd += SM::kSubV >> 4;
                     }
                     umma_commit(&ms.pv_done[g]);
-                    if (g == un.groups - 1) umma_commit(&ms.v_empty[st]);
-                    if (j + 1 == un.nt) continue;
+                    if (last) umma_commit(&ms.v_empty[st]);
+                    if (kApart || j + 1 == un.nt) continue;
                     // the next scores take the place of P: after its product is done
                     if (g == 0) ok = role_wait(&ms.k_full[st ^ 1], ((t + 1) >> 1) & 1, abort_flag);
                     ok = ok && role_wait(&ms.pv_done[g], (mine[g] + j) & 1, abort_flag);
                     if (!ok) break;
                     tc_fence_after();
                     qk(g, st ^ 1);
-                    if (g == un.groups - 1) umma_commit(&ms.k_empty[st ^ 1]);
+                    if (last) umma_commit(&ms.k_empty[st ^ 1]);
                 }
             }
             tiles += un.nt;
