@@ -83,6 +83,12 @@ constexpr float kNegInf = -__builtin_huge_valf();
 // a logit as it is held: NaN counts as -infinity, -0 as 0
 __device__ __forceinline__ float plain_logit(float x) { return x == x ? x + 0.f : kNegInf; }
 
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // w = 2^-y in steps of 2^-sh.  The difference top - l is kept exactly as a sum
 // of two fp32 numbers and multiplied by log2(e)/temperature in two parts, so y
 // = k/64 + g has some 40 correct bits; then 2^-y = 2^(-k/64) (1 - u) with the
@@ -123,6 +129,14 @@ struct Weigher {
         const int q = (int)__float_as_uint(__fmaf_rn(u, 0x1p29f, 12582912.f)) - 0x4B400000;       // u 2^29, below 2^22
         const uint32_t t = step[k & 63];
         return l == top ? 0x80000000u : t - (uint32_t)__mulhi((int)(t >> 1), q * 16);
+    }
+    // The same from the hardware's 2^x, to 2^-22 and a third of the work: for the
+    // histogram, and for the row's whole weight, of which top-p asks a share that
+    // is itself a number of 24 bits.  An integer like the others: its sums are
+    // the same in any order, and it is exact at the maximum.
+    __device__ __forceinline__ uint32_t quick(float p, int k) const {
+        const uint32_t b = __float_as_uint(ex2(-p));                // 2^-i (1 + f): i is k >> 6, or one more
+        return (b << 8 | 0x80000000u) >> (127 - (int)(b >> 23) - (k >> 6));
     }
     // acc + mant * 2^(sh - 31 - (k >> 6)), rounded
     __device__ __forceinline__ uint64_t add(uint64_t acc, uint32_t mant, int k) const {
@@ -309,19 +323,18 @@ __device__ __forceinline__ int gather(SampleCtx<W> &x, uint64_t &token) {
 }
 __device__ __forceinline__ int sort_size(int m) { return m <= 64 ? 64 : 1 << (32 - __clz(m - 1)); }
 
-// Where few tokens are listed, eight threads count for each what a sort would
+// Where few tokens are listed, n threads count for each what a sort would
 // find: `before`: how many of `tok` are smaller, and what those weigh.
-__device__ __forceinline__ void count_before(const uint64_t *tok, const uint64_t *weight, int m, uint64_t mine, int &before,
-                                             uint64_t &before_w) {
+__device__ __forceinline__ void count_before(const uint64_t *tok, const uint64_t *weight, int m, int n, uint64_t mine,
+                                             int &before, uint64_t &before_w) {
     before = 0, before_w = 0;
 #pragma unroll 4
-    for (int j = threadIdx.x & 7; j < m; j += 8) {
+    for (int j = threadIdx.x & (n - 1); j < m; j += n) {
         const bool less = tok[j] < mine;
         before += less;
         before_w += less ? weight[j] : 0;
     }
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
+    for (int o = 1; o < n; o <<= 1) {
         before += __shfl_xor_sync(0xffffffffu, before, o);
         before_w += __shfl_xor_sync(0xffffffffu, before_w, o);
     }
@@ -517,18 +530,35 @@ __device__ void resolve(SampleCtx<W> &x, int b, uint32_t count, uint32_t k, doub
         if (x.rank == 0) {
             uint64_t token, all;
             const int got = gather(x, token);
-            token = block_sort(sm, token, sort_size(got));
-            const uint32_t key = ~(uint32_t)(token >> 32);
-            const uint64_t mine = tid < got ? x.weigh(logit_of(key)) : 0;
+            int place = tid;                                        // in the order
+            uint64_t mine, upto;
+            bool lead = tid < got;
+            if (got <= W * 16) {                                    // two threads or more per token
+                const int n = got <= W * 4 ? 8 : got <= W * 8 ? 4 : 2, i = tid / n;
+                if (tid < got) {
+                    sm.all[tid] = token;
+                    sm.list[tid] = x.weigh(logit_of(~(uint32_t)(token >> 32)));
+                }
+                __syncthreads();
+                token = i < got ? sm.all[i] : ~0ull;
+                mine = i < got ? sm.list[i] : 0;
+                lead = i < got && tid % n == 0;
+                count_before(sm.all, sm.list, got, n, token, place, upto);
+                upto += before + mine;
+            } else {
+                token = block_sort(sm, token, sort_size(got));
+                mine = tid < got ? x.weigh(logit_of(~(uint32_t)(token >> 32))) : 0;
+                upto = before + block_scan(sm, mine, all);
+            }
             if (tid == 0) sm.out_move = got == 0 || (!K && target <= (double)before) ? -1 : 1;
-            const uint64_t upto = before + block_scan(sm, mine, all);
+            __syncthreads();
             const bool down = sm.out_move < 0;
             __syncthreads();
-            const bool hit = K ? (uint32_t)tid + 1 == k - count
+            const bool hit = K ? (uint32_t)place + 1 == k - count
                                : !down && (double)upto >= target && (double)(upto - mine) < target;
-            if (tid < got && hit) {                                 // one thread at most
+            if (lead && hit) {                                      // one thread at most
                 sm.out_move = 0;
-                sm.out_key = key;
+                sm.out_key = ~(uint32_t)(token >> 32);
                 sm.out_idx = (uint32_t)token;
                 sm.out_w = upto;
             }
@@ -667,7 +697,7 @@ __global__ void __launch_bounds__(W * 32, W == 16 ? 2 : 1) sample_kernel(const S
                 if (ok) atomicAdd(&sm.cnt[k], 1u);
                 return;
             }
-            const uint32_t m = weigh.mantissa(l, d, y, kf, k);
+            const uint32_t m = weigh.quick(y, k);
             if (!by_k) w = weigh.add(w, ok ? m : 0u, k);
             if (ok) {
                 atomicAdd(&sm.cnt[k], 1u);
@@ -699,7 +729,7 @@ __global__ void __launch_bounds__(W * 32, W == 16 ? 2 : 1) sample_kernel(const S
                     uint64_t mine = i < m ? sm.list[i] : 0, less;
                     token = i < m ? sm.all[i] : ~0ull;
                     int place;
-                    count_before(sm.all, sm.list, m, token, place, less);
+                    count_before(sm.all, sm.list, m, 8, token, place, less);
                     if (lead && place == top_n - 1) sm.out_w = less + mine;
                     __syncthreads();
                     listed = sm.out_w;
@@ -717,7 +747,7 @@ __global__ void __launch_bounds__(W * 32, W == 16 ? 2 : 1) sample_kernel(const S
                     sum = sm.out_w;
                     token <<= 32;
                     mine = i < m ? sm.list[i] : 0;
-                    count_before(sm.all, sm.list, m, token, place, less);
+                    count_before(sm.all, sm.list, m, 8, token, place, less);
                     const double ut = fmax((double)u, 0.0) * (double)sum;
                     const uint64_t goal = min(ut < (double)sum ? (uint64_t)ut : sum - 1, sum - 1);
                     if (finish && lead && goal >= less && goal < less + mine) p.tokens[row] = (int64_t)(token >> 32);
