@@ -340,17 +340,37 @@ __device__ __forceinline__ void count_before(const uint64_t *tok, const uint64_t
     }
 }
 
-// This lane's logit q into the CTA's list, if `take` (called by whole warps).
+// This lane's logits q0 .. q0 + 31, a bit each: those in bins before b, and in b.
 template <int W>
-__device__ __forceinline__ void list_token(SampleCtx<W> &x, float l, int q, bool take) {
+__device__ __forceinline__ void mark_bins(const SampleCtx<W> &x, int q0, int b, uint32_t &before, uint32_t &at) {
+    before = at = 0;
+    const int n = min(32, x.per - q0);
+    const auto mark = [&](float l, int i) {
+        const int k = x.weigh.bin(l);
+        before |= (k < b ? 1u : 0u) << i;
+        at |= (k == b ? 1u : 0u) << i;
+    };
+    int i = 0;
+    for (; i + 4 <= n; i += 4) {
+        float l[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) l[j] = x.logits[q0 + i + j];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mark(l[j], i + j);
+    }
+    for (; i < n; ++i) mark(x.logits[q0 + i], i);
+}
+
+// The marked ones into the CTA's list.
+template <int W>
+__device__ __forceinline__ void list_tokens(SampleCtx<W> &x, int q0, uint32_t marks) {
+    if (!marks) return;
     SampleShared<W> &sm = x.sm;
-    const uint32_t mask = __ballot_sync(0xffffffffu, take);
-    if (mask == 0) return;
-    const int lane = threadIdx.x & 31, lead = __ffs(mask) - 1;
-    uint32_t at = 0;
-    if (lane == lead) at = atomicAdd(&sm.n_list, (uint32_t)__popc(mask));
-    at = __shfl_sync(0xffffffffu, at, lead) + __popc(mask & ((1u << lane) - 1u));
-    if (take && at < (W * 32)) sm.list[at] = (uint64_t)(~key_of(l)) << 32 | (x.first + (uint32_t)q);
+    uint32_t at = atomicAdd(&sm.n_list, (uint32_t)__popc(marks));
+    for (; marks; marks &= marks - 1, ++at) {
+        const int q = q0 + __ffs(marks) - 1;
+        if (at < W * 32) sm.list[at] = (uint64_t)(~key_of(x.logits[q])) << 32 | (x.first + (uint32_t)q);
+    }
 }
 
 // The first bin at which the running count reaches k (k > 0) or the running
@@ -483,10 +503,11 @@ __device__ int next_bin(SampleCtx<W> &x, int b, int d) {
 // The exact cut at or near bin b: K: the first `k` tokens of the order (`count`
 // of them lie before the bin); else the shortest prefix that weighs `target`.
 // `sum`: the weight of the prefix; `at_bin`, `below`: the bin, and the weight
-// of this lane's tokens in the bins before it.
+// of this lane's tokens in the bins before it; `at_lo`, `at_hi`: its first and
+// last one in the bin.
 template <bool K, int W>
 __device__ void resolve(SampleCtx<W> &x, int b, uint32_t count, uint32_t k, double target, float &cut,
-                        uint32_t &cut_idx, uint64_t &sum, int &at_bin, uint64_t &below) {
+                        uint32_t &cut_idx, uint64_t &sum, int &at_bin, uint64_t &below, int &at_lo, int &at_hi) {
     SampleShared<W> &sm = x.sm;
     cg::cluster_group cl = cg::this_cluster();
     const int tid = threadIdx.x;
@@ -495,12 +516,18 @@ __device__ void resolve(SampleCtx<W> &x, int b, uint32_t count, uint32_t k, doub
         __syncthreads();
         uint64_t w = 0;
         uint32_t c = 0;
-        for_logits(x, [&](float l, int q) {
-            const int kb = x.weigh.bin(l);
-            w = x.weigh.add(w, l, kb < b);
-            c += kb == b;
-            list_token(x, l, q, kb == b);
-        });
+        at_lo = x.per, at_hi = -1;
+        for (int q0 = 0; q0 < x.per; q0 += 32) {
+            uint32_t less, at;
+            mark_bins(x, q0, b, less, at);
+            for (; less; less &= less - 1) w = x.weigh.add(w, x.logits[q0 + __ffs(less) - 1]);
+            list_tokens(x, q0, at);
+            if (at) {
+                c += __popc(at);
+                at_lo = min(at_lo, q0 + __ffs(at) - 1);
+                at_hi = q0 + 31 - __clz(at);
+            }
+        }
         at_bin = b;
         below = w;
         uint64_t before, skip;
@@ -683,6 +710,7 @@ __global__ void __launch_bounds__(W * 32, W == 16 ? 2 : 1) sample_kernel(const S
         min_p > 0.f ? max((uint64_t)1, (uint64_t)ceil(fmin((double)min_p, 1.0) * (double)(1ull << p.sh))) : 1ull;
     int at_bin = -1;                                                // the cut's bin, where it was resolved
     uint64_t below = 0;
+    int at_lo = 0, at_hi = -1;
     float cut = kNegInf;                                            // keep logits above the cut, and equal ones up to an index
     uint32_t cut_idx = 0xFFFFFFFFu;
     const bool by_k = top_k > 0 && top_k < p.V, by_p = top_p < 1.f;
@@ -711,7 +739,11 @@ __global__ void __launch_bounds__(W * 32, W == 16 ? 2 : 1) sample_kernel(const S
         uint32_t before = sm.pick_before, count = sm.pick_count;
         if (before + count <= (uint32_t)(W * 32) && b < kSampleBins - 1) {
             // ---- all that can be kept on one CTA, one token per thread
-            for_logits(x, [&](float l, int q) { list_token(x, l, q, weigh.bin(l) <= b); });
+            for (int q0 = 0; q0 < x.per; q0 += 32) {
+                uint32_t less, at;
+                mark_bins(x, q0, b + 1, less, at);
+                list_tokens(x, q0, less);
+            }
             cl.sync();
             bool finish = false;
             if (rank == 0) {
@@ -781,7 +813,7 @@ __global__ void __launch_bounds__(W * 32, W == 16 ? 2 : 1) sample_kernel(const S
         }
         uint64_t sum = total;
         if (by_k && count > 0) {
-            resolve<true>(x, b, before, (uint32_t)top_k, 0.0, cut, cut_idx, sum, at_bin, below);
+            resolve<true>(x, b, before, (uint32_t)top_k, 0.0, cut, cut_idx, sum, at_bin, below, at_lo, at_hi);
         } else if (by_k && by_p) {                                  // k reaches past every weight
             uint64_t all = 0;
             for_logits(x, [&](float l, int) { all = weigh.add(all, l); });
@@ -794,23 +826,22 @@ __global__ void __launch_bounds__(W * 32, W == 16 ? 2 : 1) sample_kernel(const S
                 b = sm.pick_bin;
                 __syncthreads();
             }
-            resolve<false>(x, b, 0, 0, target, cut, cut_idx, sum, at_bin, below);
+            resolve<false>(x, b, 0, 0, target, cut, cut_idx, sum, at_bin, below, at_lo, at_hi);
         }
     }
     // ---- the kept weight of each lane's part
-    const auto kept = [&](uint64_t acc, float l, int q) -> uint64_t {
-        const uint64_t w = weigh.add(0, l, l > cut || (l == cut && x.first + (uint32_t)q <= cut_idx));
+    const auto kept = [&](uint64_t acc, float l, uint32_t index) -> uint64_t {
+        const uint64_t w = weigh.add(0, l, l > cut || (l == cut && index <= cut_idx));
         return acc + (w >= min_w ? w : 0);
     };
     uint64_t w = 0, total, before;
     uint32_t c;
     if (at_bin >= 0 && min_w == 1) {                                // only the cut's bin is left to look at
         w = below;
-        for_logits(x, [&](float l, int q) {
-            if (weigh.bin(l) == at_bin) w = kept(w, l, q);
-        });
+        for (int q = at_lo; q <= at_hi; ++q)
+            if (weigh.bin(x.logits[q]) == at_bin) w = kept(w, x.logits[q], x.first + (uint32_t)q);
     } else {
-        for_logits(x, [&](float l, int q) { w = kept(w, l, q); });
+        for_logits(x, [&](float l, int q) { w = kept(w, l, x.first + (uint32_t)q); });
     }
     cluster_sums(x, w, 0, total, c, before);
     // ---- the first token whose running sum exceeds u * total: its lane, then the token
@@ -818,14 +849,20 @@ __global__ void __launch_bounds__(W * 32, W == 16 ? 2 : 1) sample_kernel(const S
     const uint64_t goal = min(ut < (double)total ? (uint64_t)ut : total - 1, total - 1);
     const uint64_t upto = before + warp_scan(w);
     const uint32_t over = __ballot_sync(0xffffffffu, upto > goal);
-    if (goal >= before && over && lane == __ffs(over) - 1) {        // exactly one lane of the cluster
-        uint64_t run = upto - w;
-        for (int q = 0; q < p.per; ++q) {
-            run = kept(run, x.logits[q], q);
-            if (run > goal) {
-                p.tokens[row] = (int64_t)x.first + q;
+    if (goal >= before && over) {                                   // exactly one warp of the cluster: it shares the lane's tokens
+        const int lead = __ffs(over) - 1;
+        const float *l = logits + (tid - lane + lead) * p.per;
+        const uint32_t first = (uint32_t)(base + (tid - lane + lead) * p.per);
+        uint64_t run = __shfl_sync(0xffffffffu, upto - w, lead);
+        for (int q0 = 0; q0 < p.per; q0 += 32) {
+            const uint32_t index = first + (uint32_t)(q0 + lane);
+            run += warp_scan(q0 + lane < p.per ? kept(0, l[q0 + lane], index) : 0);
+            const uint32_t hit = __ballot_sync(0xffffffffu, run > goal);
+            if (hit) {
+                if (lane == __ffs(hit) - 1) p.tokens[row] = (int64_t)index;
                 break;
             }
+            run = __shfl_sync(0xffffffffu, run, 31);
         }
     }
     cl.sync();                                        // no CTA leaves while another reads its shared memory
