@@ -563,6 +563,9 @@ struct AttendSmem {
     uint8_t ring[W][AttendCfg<D, NT>::kDepth][AttendCfg<D, NT>::kNB * KvLayout<D>::kBytes];
     uint4 frag[W][NT][D / 32][32];
     uint64_t full[W][AttendCfg<D, NT>::kDepth];
+    float2 ml[W][8 * NT];               // of the warps' parts of one unit, whose sums lie in the rings
+    int merge[W][2];                    // how many of them (0: not so), and the slot of their sum
+    static_assert(sizeof(ring[0]) >= 8 * NT * D * 4, "a part's sums");
 };
 
 __device__ __forceinline__ int64_t kv4_blocks_of(const Kv4AttendParams &p, int64_t pos0) {
@@ -651,8 +654,6 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kWarps * 32, 1)
     fence_mbar_init();
     __syncwarp();
     griddep_wait();
-    // ---- this warp's share: the CTAs in turn, so that few shares lie on many SMs
-    const int64_t share = (int64_t)warp * gridDim.x + blockIdx.x;
     const int64_t per_seq = (int64_t)p.KV * p.tiles;
     Kv4Walk con;
     int64_t total, skip;
@@ -666,7 +667,11 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kWarps * 32, 1)
     }
     if (total == 0) return;
     const Kv4Plan plan(total, p.warps);
-    if (share >= plan.shares) return;
+    // ---- this warp's share: the CTAs in turn; or, of few units, equally many one after the other
+    const uint32_t s0 = (uint32_t)plan.shares * blockIdx.x / gridDim.x,
+                   s1 = (uint32_t)plan.shares * (blockIdx.x + 1) / gridDim.x;
+    const int64_t share = p.few_units ? s0 + warp : (uint32_t)warp * gridDim.x + blockIdx.x;
+    if (share >= (p.few_units ? s1 : plan.shares)) return;
     int64_t at = plan.start(share);
     const int64_t next_at = plan.start(share + 1), work = next_at - at;     // in the cut order
     if (p.B > 1) {
@@ -697,8 +702,21 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kWarps * 32, 1)
         const int64_t unit = quot(at, con.nb + kUnitCost);
         con.kvh = (int)quot(unit, p.tiles);
         con.tile = (int)(unit - (int64_t)con.kvh * p.tiles);
-        con.enter(at - unit * (con.nb + kUnitCost), work);
+        at -= unit * (con.nb + kUnitCost);
+        con.enter(at, work);
     }
+    // One unit has all of this CTA's shares (and blocks in each): its warps join
+    // their parts before they go to memory, as long contexts of few sequences
+    // have hundreds of parts per unit (131072 positions of one sequence, 8B
+    // heads: 1776 parts, of which the second kernel took 12 us).
+    if (lane == 0) {                    // (not kept in registers over the loop)
+        const int64_t unit_at = plan.start(share) - at;
+        const bool merge = p.few_units && s1 - s0 > 1 && plan.q > kUnitCost && unit_at <= plan.start(s0) &&
+                           plan.start(s1) <= unit_at + con.nb + kUnitCost;
+        sm.merge[warp][0] = merge ? (int)(s1 - s0) : 0;
+        sm.merge[warp][1] = (int)s0 * 2 + (plan.start(s0) - unit_at <= kUnitCost ? 1 : 0);
+    }
+    __syncwarp();
     // ---- the ring: stages of NB blocks
     const Kv4Lane<D> ln;
     const uint32_t ring0 = smem_u32(sm.ring[warp][0]), bar0 = smem_u32(&sm.full[warp][0]);
@@ -775,6 +793,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kWarps * 32, 1)
             if (alive) start();
         }
         if (any) {
+            const bool merge = sm.merge[warp][0] != 0;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 float l[2];
@@ -793,6 +812,17 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kWarps * 32, 1)
                 for (int i = 0; i < 2; ++i) {
                     const int c = 8 * nt + 2 * t + i, r = row0 + c;
                     if (r >= p.R) continue;
+                    if (merge) {
+                        float *sums = reinterpret_cast<float *>(sm.ring[warp][0]) + c * D + 4 * g;
+#pragma unroll
+                        for (int j = 0; j < NG; ++j)
+                            *reinterpret_cast<float4 *>(sums + 32 * j) =
+                                make_float4(fmaf(acc.o[nt][2 * j][i], 0x1p24f, mt[i][j]), fmaf(acc.o[nt][2 * j][2 + i], 0x1p20f, mt[i][j]),
+                                            fmaf(acc.o[nt][2 * j + 1][i], 0x1p24f, mt[i][j]),
+                                            fmaf(acc.o[nt][2 * j + 1][2 + i], 0x1p20f, mt[i][j]));
+                        if (g == 0) sm.ml[warp][c] = make_float2(acc.M[nt][i], l[i]);
+                        continue;
+                    }
                     const bool whole = began && ends;
                     const float f = !whole ? 1.f : l[i] != 0.f ? 1.f / l[i] : 0.f;
                     const int tok = r / p.G, hh = r - tok * p.G;
@@ -818,8 +848,44 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kWarps * 32, 1)
         if (!more) break;
         __syncwarp();
     }
+    if (const int n = sm.merge[warp][0]; n) {                       // into the first warp's part; the others' are empty
+        asm volatile("bar.sync 1, %0;" :: "r"(n * 32) : "memory");
+        const int64_t to = (int64_t)sm.merge[warp][1] * C;
+        const int row0 = con.tile * C;
+        for (int i = threadIdx.x; i < C * (D / 4); i += n * 32) {
+            const int c = i / (D / 4), ch = i % (D / 4) * 4;
+            if (row0 + c >= p.R) break;
+            float top = kNoMax;
+            for (int w = 0; w < n; ++w) top = fmaxf(top, sm.ml[w][c].x);
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+            float l = 0.f;
+#pragma unroll 4
+            for (int w = 0; w < n; ++w) {
+                const float f = ex2(sm.ml[w][c].x - top);
+                const float4 y = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(sm.ring[w][0]) + c * D + ch);
+                l += sm.ml[w][c].y * f;
+                o = make_float4(fmaf(y.x, f, o.x), fmaf(y.y, f, o.y), fmaf(y.z, f, o.z), fmaf(y.w, f, o.w));
+            }
+            *reinterpret_cast<float4 *>(p.part_o + (to + c) * D + ch) = o;
+            if (ch == 0) p.part_ml[to + c] = make_float2(top, l);
+        }
+        if (warp > 0 && lane < C) p.part_ml[share * 2 * C + lane] = make_float2(kNoMax, 0.f);
+    }
     if (!alive)                         // a copy that was late: every slot's bounded once more before the memory goes
         for (int i = 0; i < DEPTH; ++i) mbar_wait(&sm.full[warp][(slot + i) % DEPTH], parity ^ (slot + i >= DEPTH), &g_status);
+}
+
+// N numbers, or zeros; loads that are written one after the other are issued so.
+template <int N>
+__device__ __forceinline__ void load_if(const float *src, bool take, float (&v)[N]) {
+    if constexpr (N == 4)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\t"
+                     "mov.b32 %3, 0;\n\t@p ld.global.v4.f32 {%0, %1, %2, %3}, [%4];\n\t}"
+                     : "=&f"(v[0]), "=&f"(v[1]), "=&f"(v[2]), "=&f"(v[3]) : "l"(src), "r"((uint32_t)take) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %3, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\t"
+                     "@p ld.global.v2.f32 {%0, %1}, [%2];\n\t}"
+                     : "=&f"(v[0]), "=&f"(v[1]) : "l"(src), "r"((uint32_t)take) : "memory");
 }
 
 // Units of which several warps had a part, joined in order, and rows of
@@ -852,26 +918,35 @@ __global__ void __launch_bounds__(WPR > 8 ? WPR * 32 : 256) kv4_join_kernel(cons
         const int c0 = held.x, c1 = held.y;
         const auto slot = [&](int c) { return ((int64_t)c * 2 + (c == c0 ? 1 : 0)) * C + (r - tile * C); };
         float top = kNoMax;
-#pragma unroll 4
-        for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, p.part_ml[slot(c)].x);
+        for (int base = c0; base <= c1; base += 128) {
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int c = base + 32 * i + lane;
+                x[i] = c <= c1 ? p.part_ml[slot(c)].x : kNoMax;
+            }
+            top = fmaxf(fmaxf(fmaxf(top, x[0]), fmaxf(x[1], x[2])), x[3]);
+        }
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-#pragma unroll 8
-        for (int c = c0 + sub; c <= c1; c += WPR) {
-            const int64_t at = slot(c);
-            const float2 x = p.part_ml[at];
-            const float f = ex2(x.x - top);
-            l += x.y * f;
-            const float *src = p.part_o + at * D + lane * V;
-            if constexpr (V == 4) {
-                const float4 y = *reinterpret_cast<const float4 *>(src);
-                acc[0] = fmaf(y.x, f, acc[0]);
-                acc[1] = fmaf(y.y, f, acc[1]);
-                acc[2] = fmaf(y.z, f, acc[2]);
-                acc[3] = fmaf(y.w, f, acc[3]);
-            } else {
-                const float2 y = *reinterpret_cast<const float2 *>(src);
-                acc[0] = fmaf(y.x, f, acc[0]);
-                acc[1] = fmaf(y.y, f, acc[1]);
+        // several parts' loads at a time whatever their number (one after the other they are most of the time), in short
+        // code: it is never in the instruction cache
+        constexpr int N = WPR == 32 ? 8 : 4;
+        constexpr int64_t kStep = (int64_t)WPR * 2 * C;
+        for (int base = c0 + sub; base <= c1; base += N * WPR) {
+            const int64_t at = (int64_t)base * 2 * C + (r - tile * C);          // slot 0; the first part lies in slot 1
+            const int64_t at0 = at + (base == c0 ? C : 0);
+            float x[N][2], y[N][V];
+#pragma unroll
+            for (int i = 0; i < N; ++i) load_if<2>(reinterpret_cast<const float *>(p.part_ml + (i ? at : at0) + kStep * i), base + WPR * i <= c1, x[i]);
+#pragma unroll
+            for (int i = 0; i < N; ++i)                             // (M and l of 0: no such part, or nothing was written there)
+                load_if<V>(p.part_o + ((i ? at : at0) + kStep * i) * D + lane * V, x[i][1] != 0.f || (x[i][0] != 0.f && x[i][0] != kNoMax), y[i]);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float f = ex2(fminf(x[i][0] - top, 0.f));     // (above the maximum only where there is no part)
+                l += x[i][1] * f;
+#pragma unroll
+                for (int k = 0; k < V; ++k) acc[k] = fmaf(y[i][k], f, acc[k]);
             }
         }
     }
@@ -915,7 +990,7 @@ static int attend_launch(const Kv4AttendParams &p, cudaStream_t st) {
                                                         sizeof(AttendSmem<D, NT>), st, "kv4_attend_kernel", p);
     if (rc != BF16X_OK) return rc;
     // a row has up to p.warps / units parts
-    if (units * 64 <= p.warps)
+    if (p.few_units)
         return launch_kv4<kv4_join_kernel<D, NT, 32>>(dim3((unsigned)rows), 1024, 0, st, "kv4_join_kernel", p);
     if (units * 8 <= p.warps)
         return launch_kv4<kv4_join_kernel<D, NT, 8>>(dim3((unsigned)rows), 256, 0, st, "kv4_join_kernel", p);
@@ -1008,6 +1083,7 @@ extern "C" int bf16x_kv4_attend(const uint16_t *q, int64_t ldq_b, int64_t ldq_t,
     p.q = q, p.ldq_b = ldq_b, p.ldq_t = ldq_t, p.ldq_h = ldq_h;
     p.B = (int)B, p.T = (int)T, p.H = (int)H, p.KV = (int)KV, p.G = (int)G, p.R = (int)R;
     p.tiles = (int)((R + 8 * nt - 1) / (8 * nt)), p.warps = attend_warps(nt);
+    p.few_units = B * KV * p.tiles * 64 <= p.warps;
     p.pos_stride = pos_stride, p.pos0 = pos0, p.scale_log2 = scale * 1.44269504088896340736f;
     p.blocks = blocks, p.max_seq = max_seq, p.nblk = nblk, p.out = out;
     if (R > kFewRows) return kv4_prefill(p, D, workspace, (cudaStream_t)stream);

@@ -125,6 +125,7 @@ struct Kv4AttendParams {
     int64_t ldq_b, ldq_t, ldq_h;
     int B, T, H, KV, G, R;
     int pos_stride, tiles, warps;       // row tiles per head; warps of the grid
+    int few_units;                      // a unit has the shares of several CTAs
     const int64_t *pos0;
     float scale_log2;                   // softmax scale * log2(e)
     const uint8_t *blocks;

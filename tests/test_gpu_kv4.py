@@ -181,6 +181,16 @@ def test_attend_long(n, T):
     _check(cache, q, torch.tensor(n))
 
 
+@pytest.mark.parametrize("D,T,H,KV,pos", [(64, 1, 4, 2, [80001]), (64, 1, 3, 1, [70000, 90000]), (128, 1, 8, 8, [20479]),
+                                          (128, 1, 1, 1, [-1, 150000, 17]), (64, 3, 4, 1, [99990]), (128, 4, 12, 3, [35000, 4])])
+def test_attend_few_sequences_of_many_blocks(D, T, H, KV, pos):
+    """Several CTAs per kv head: their warps join their parts before the second kernel does."""
+    cache = _filled(len(pos), KV, D, max(pos) + T, seed=KV)
+    q = (torch.randn(len(pos), T, H, D, generator=_gen(D + T)) * 1.5).to(torch.bfloat16)
+    _check(cache, q, torch.tensor(pos))
+    _lib.check_device_status()
+
+
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("T", [1, 6, 50])
 @pytest.mark.parametrize("qs,ks,vs", [(1.0, 1.0, 1e-30), (1.0, 1.0, 1e25), (1e-20, 1e20, 1.0), (1e15, 1e-15, 3e4),
