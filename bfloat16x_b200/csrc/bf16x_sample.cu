@@ -83,12 +83,6 @@ constexpr float kNegInf = -__builtin_huge_valf();
 // a logit as it is held: NaN counts as -infinity, -0 as 0
 __device__ __forceinline__ float plain_logit(float x) { return x == x ? x + 0.f : kNegInf; }
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // w = 2^-y in steps of 2^-sh.  The difference top - l is kept exactly as a sum
 // of two fp32 numbers and multiplied by log2(e)/temperature in two parts, so y
 // = k/64 + g has some 40 correct bits; then 2^-y = 2^(-k/64) (1 - u) with the
@@ -129,14 +123,6 @@ struct Weigher {
         const int q = (int)__float_as_uint(__fmaf_rn(u, 0x1p29f, 12582912.f)) - 0x4B400000;       // u 2^29, below 2^22
         const uint32_t t = step[k & 63];
         return l == top ? 0x80000000u : t - (uint32_t)__mulhi((int)(t >> 1), q * 16);
-    }
-    // The same from the hardware's 2^x, to 2^-22 and a third of the work: for the
-    // histogram, and for the row's whole weight, of which top-p asks a share that
-    // is itself a number of 24 bits.  An integer like the others: its sums are
-    // the same in any order, and it is exact at the maximum.
-    __device__ __forceinline__ uint32_t quick(float p, int k) const {
-        const uint32_t b = __float_as_uint(ex2(-p));                // 2^-i (1 + f): i is k >> 6, or one more
-        return (b << 8 | 0x80000000u) >> (127 - (int)(b >> 23) - (k >> 6));
     }
     // acc + mant * 2^(sh - 31 - (k >> 6)), rounded
     __device__ __forceinline__ uint64_t add(uint64_t acc, uint32_t mant, int k) const {
@@ -725,7 +711,7 @@ __global__ void __launch_bounds__(W * 32, W == 16 ? 2 : 1) sample_kernel(const S
                 if (ok) atomicAdd(&sm.cnt[k], 1u);
                 return;
             }
-            const uint32_t m = weigh.quick(y, k);
+            const uint32_t m = weigh.mantissa(l, d, y, kf, k);
             if (!by_k) w = weigh.add(w, ok ? m : 0u, k);
             if (ok) {
                 atomicAdd(&sm.cnt[k], 1u);
