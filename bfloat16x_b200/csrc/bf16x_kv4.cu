@@ -550,7 +550,7 @@ __device__ __forceinline__ void kv4_block(uint32_t blk, int key0, int n_keys, co
 // and one that goes on after it (slot 1), and a second kernel joins the parts.
 template <int D, int NT>
 struct AttendCfg {
-    static constexpr int kWarps = NT == 1 ? 12 : 8;                 // per CTA and SM: what the registers allow
+    static constexpr int kWarps = NT == 1 || D == 64 ? 12 : 8;      // per CTA and SM: what the registers allow
     static constexpr int kNB = NT == 1 ? 2 : 1;                     // blocks per stage
     static constexpr int kDepth = NT == 1 ? 3 : 5;                  // stages in flight per warp
 };
@@ -980,19 +980,22 @@ constexpr int64_t kFewRows = 48;
 // Column tiles of 8 rows that one warp takes, and the grid.
 static int attend_tiles(int64_t R) { return R > 8 ? 2 : 1; }
 constexpr int kAttendGrid = 148;
-static int attend_warps(int nt) { return kAttendGrid * (nt == 1 ? AttendCfg<128, 1>::kWarps : AttendCfg<128, 2>::kWarps); }
+static int attend_warps(int nt, int64_t D) {
+    return kAttendGrid * (D == 64   ? nt == 1 ? AttendCfg<64, 1>::kWarps : AttendCfg<64, 2>::kWarps
+                          : nt == 1 ? AttendCfg<128, 1>::kWarps
+                                    : AttendCfg<128, 2>::kWarps);
+}
 
 template <int D, int NT>
 static int attend_launch(const Kv4AttendParams &p, cudaStream_t st) {
-    static_assert(AttendCfg<D, NT>::kWarps == AttendCfg<128, NT>::kWarps, "attend_warps");
     const int64_t rows = (int64_t)p.B * p.KV * p.R, units = (int64_t)p.B * p.KV * p.tiles;
     const int rc = launch_kv4<kv4_attend_kernel<D, NT>>(dim3(kAttendGrid), AttendCfg<D, NT>::kWarps * 32,
                                                         sizeof(AttendSmem<D, NT>), st, "kv4_attend_kernel", p);
     if (rc != BF16X_OK) return rc;
-    // a row has up to p.warps / units parts
-    if (p.few_units)
+    // a row has up to p.warps / units parts; 32 warps for each of few rows (384 rows of 24 units: 26 us in all, 19 with 8)
+    if (p.few_units && rows <= 2 * 148)
         return launch_kv4<kv4_join_kernel<D, NT, 32>>(dim3((unsigned)rows), 1024, 0, st, "kv4_join_kernel", p);
-    if (units * 8 <= p.warps)
+    if (units * 8 <= p.warps || p.few_units)
         return launch_kv4<kv4_join_kernel<D, NT, 8>>(dim3((unsigned)rows), 256, 0, st, "kv4_join_kernel", p);
     return launch_kv4<kv4_join_kernel<D, NT, 1>>(dim3((unsigned)((rows + 7) / 8)), 256, 0, st, "kv4_join_kernel", p);
 }
@@ -1057,7 +1060,7 @@ extern "C" int64_t bf16x_kv4_attend_workspace_bytes(int64_t B, int64_t T, int64_
     if (T * (H / KV) > kFewRows) return kv4_prefill_workspace(B, KV, T * (H / KV), T, D, max_seq);
     const int nt = attend_tiles(T * (H / KV));
     const int64_t units = B * KV * ((T * (H / KV) + 8 * nt - 1) / (8 * nt));
-    return (int64_t)attend_warps(nt) * 2 * 8 * nt * (D * 4 + 8) + units * 8;
+    return (int64_t)attend_warps(nt, D) * 2 * 8 * nt * (D * 4 + 8) + units * 8;
 }
 
 extern "C" int bf16x_kv4_attend(const uint16_t *q, int64_t ldq_b, int64_t ldq_t, int64_t ldq_h, int64_t B, int64_t T,
@@ -1082,7 +1085,7 @@ extern "C" int bf16x_kv4_attend(const uint16_t *q, int64_t ldq_b, int64_t ldq_t,
     Kv4AttendParams p = {};
     p.q = q, p.ldq_b = ldq_b, p.ldq_t = ldq_t, p.ldq_h = ldq_h;
     p.B = (int)B, p.T = (int)T, p.H = (int)H, p.KV = (int)KV, p.G = (int)G, p.R = (int)R;
-    p.tiles = (int)((R + 8 * nt - 1) / (8 * nt)), p.warps = attend_warps(nt);
+    p.tiles = (int)((R + 8 * nt - 1) / (8 * nt)), p.warps = attend_warps(nt, D);
     p.few_units = B * KV * p.tiles * 64 <= p.warps;
     p.pos_stride = pos_stride, p.pos0 = pos0, p.scale_log2 = scale * 1.44269504088896340736f;
     p.blocks = blocks, p.max_seq = max_seq, p.nblk = nblk, p.out = out;
