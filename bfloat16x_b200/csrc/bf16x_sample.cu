@@ -670,7 +670,8 @@ __global__ void __launch_bounds__(W * 32, W == 16 ? 2 : 1) sample_kernel(const S
     weigh.limit = (float)p.sh + 0.75f;
     weigh.sh = p.sh;
     weigh.step = sm.step;
-    const bool none = top == kNegInf, greedy = !(temp > 0.f) || top_k == 1;
+    // (a temperature whose reciprocal leaves fp32 is the limit of 0)
+    const bool none = top == kNegInf, greedy = !(temp > 0.f) || top_k == 1 || !(weigh.chi < __int_as_float(0x7f800000));
     if (none || greedy) {
         // ---- the lowest index of the maximum
         uint32_t at = 0xFFFFFFFFu;

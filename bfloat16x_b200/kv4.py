@@ -155,6 +155,10 @@ class Kv4Cache:
         elif (out.shape != shape or out.dtype is not torch.bfloat16 or not out.is_contiguous()
               or out.device != self.device or out.data_ptr() % 16):
             raise ValueError("out must be a contiguous, 16-byte aligned bf16 tensor of q's shape")
+        elif out.numel():               # rows are written while others are still read
+            at, last = q.data_ptr(), (B - 1) * s0 + (T - 1) * s1 + (H - 1) * s2 + D
+            if at < out.data_ptr() + 2 * out.numel() and out.data_ptr() < at + 2 * last:
+                raise ValueError("out must not overlap q")
         # a workspace of its own for every call (and every captured graph): calls may overlap on several streams
         need = _workspace_bytes(B, T, H, KV, D, self.max_seq)
         ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None

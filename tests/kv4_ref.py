@@ -73,7 +73,8 @@ def attend(q, blocks, pos0, scale, max_seq):
                 p = torch.softmax(s, 0)
                 o = p @ v
                 mags = (kc.double().unflatten(-1, (-1, 32)) * kd[..., None] + km.abs()[..., None]).flatten(-2)
-                s_abs = scale * float((mags @ q[b, t, h].abs()).max())
+                # largest sum of magnitudes of a score: |scale q k| <= |scale| |q| |k|, whatever the scale's sign
+                s_abs = abs(scale) * float((mags @ q[b, t, h].abs()).max())
                 vmag = (vc.double().unflatten(-1, (-1, 32)) * vd[..., None] + vm.abs()[..., None]).flatten(-2)
                 # bf16 result; the weights times the scales in fp16 (a half step 2^-11) and in two bf16 parts;
                 # the scores' error in the exponent: fp32 sums of at most 40 terms and the final products

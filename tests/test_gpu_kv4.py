@@ -258,6 +258,47 @@ def test_attend_scale_strides_out_and_empty():
     assert cache.attend(wide[:, :0, :, :D], p.cuda()).shape == (2, 0, H, D)
     pos2 = torch.tensor([[20, 0], [40, 0]], device="cuda")[:, 0]                            # a strided vector of positions
     assert torch.equal(cache.attend(t, pos2, 0.31), a)
+    both = torch.zeros(2, 2, 3, H, D, dtype=torch.bfloat16, device="cuda")
+    both[0] = t
+    assert torch.equal(cache.attend(both[0], p.cuda(), 0.31, out=both[1]), a)
+    for bad in (both[0], both.view(-1)[H * D:][:a.numel()].view_as(a)):
+        with pytest.raises(ValueError, match="overlap"):
+            cache.attend(both[0], p.cuda(), 0.31, out=bad)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1e-30])
+@pytest.mark.parametrize("T", [1, 3, 60])
+def test_attend_unusual_scales(T, scale):
+    cache = _filled(2, 2, 64, 150, seed=43, stale=True)
+    q = torch.randn(2, T, 4, 64, generator=_gen(44)).to(torch.bfloat16)
+    _check(cache, q, torch.tensor([90, -1]), scale=scale)
+
+
+@pytest.mark.parametrize("T,S", [(60, 200), (96, 1500)])
+def test_attend_prompts_on_two_streams_and_in_graphs(T, S):
+    """The prompt kernel, its units cut and whole: two calls at once, and one captured call with moved positions."""
+    D, H, KV = 128, 8, 2
+    caches = [_filled(3, KV, D, S, seed=60 + i) for i in range(2)]
+    q = torch.randn(3, T, H, D, generator=_gen(62)).to(torch.bfloat16).cuda()
+    pos = torch.tensor([0, S - T, 50], device="cuda")
+    want = [c.attend(q, pos) for c in caches]
+    _check(caches[0], q.cpu(), pos.cpu())
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in caches], [[], []]
+    for _ in range(4):
+        for i, c in enumerate(caches):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(c.attend(q, pos))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for g, w in zip(got, want) for o in g)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = caches[0].attend(q, pos)
+    for p in ([S - T] * 3, [-T, 3, S // 2], [-5, -6, -7]):
+        pos.copy_(torch.tensor(p))
+        graph.replay()
+        assert torch.equal(out, caches[0].attend(q, pos))
+    _lib.check_device_status()
 
 
 def test_attend_layer_slices_streams_and_graphs():

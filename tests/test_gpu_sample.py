@@ -132,6 +132,18 @@ def test_sample_large(B, V, dtype):
         assert [int(got[r]) for r in rows] == want
 
 
+def test_sample_extreme_temperatures():
+    """Too small for a reciprocal in fp32: the largest logit; infinite: every token alike."""
+    x, u = _rows(3, 777, 9)
+    for t in (1e-45, 4e-39):
+        got = sample(x.cuda(), u.cuda(), temperature=torch.full((3,), t, device="cuda"), top_p=0.9)
+        assert torch.equal(got.cpu(), x.argmax(1))
+    x[:, 5] = float("-inf")
+    got = sample(x.cuda(), u.cuda(), temperature=float("inf")).cpu()
+    alike = [i for i in range(777) if i != 5]
+    assert got.tolist() == [alike[int(float(v) * 776)] for v in u]
+
+
 def test_sample_distribution_and_graph():
     """Equally spaced numbers draw each token as often as its probability says; a captured call follows its inputs."""
     V, N = 50, 4096
