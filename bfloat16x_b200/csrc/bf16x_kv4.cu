@@ -20,8 +20,12 @@ namespace bf16x {
 // Every operation is rounded by itself (no fused multiply-add), so the codes
 // do not depend on how the compiler contracts.
 //
-// D/8 lanes per (token, head), 8 channels each: a 16-byte load, and the whole
-// K word of a lane.  Bound by memory traffic for prompts, by latency for steps.
+// A CTA per token: D/8 lanes per head, 8 channels each (a 16-byte load, and the
+// whole K word of a lane), over the heads in turn, so that the angles of the
+// position are loaded once.  4 x 2047 tokens of the 8B heads (32 + 2 * 8 of 128
+// channels, 190 MB) take 48 us, 4.0 TB/s; one token 3.4 us, all latency.  Bound
+// by instructions (0.78 per cycle and scheduler, memory at a third); rounding by
+// a division per value took 118 us.
 template <int D>
 __device__ __forceinline__ void kv4_quantize8(const float (&y)[8], float &d, float &m, uint32_t &codes) {
     float lo = y[0], hi = y[0];
@@ -158,6 +162,8 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4AppendParams p
 // ---------------------------------------------------------------------- read
 // The values that positions *pos0 .. *pos0 + T - 1 stand for, d * code + m in
 // fp32 rounded to bf16; a position outside the cache reads as zeros.
+// A token's heads of K and V per CTA; 4 x 2047 tokens of 8 heads of 128
+// channels (44 MB, most of it written) take 15 us, 2.9 TB/s.
 struct Kv4ReadParams {
     const uint8_t *blocks;
     int64_t max_seq, nblk;
@@ -548,6 +554,15 @@ __device__ __forceinline__ void kv4_block(uint32_t blk, int key0, int n_keys, co
 // captured call follows them.  A warp writes a unit that it has alone; of
 // others it writes its part, at most one that began before its share (slot 0)
 // and one that goes on after it (slot 1), and a second kernel joins the parts.
+//
+// Bound by instructions: some 290 per block of 16 positions at 128 channels
+// (unpacking codes, softmax, the weights times the scales, four mma per 32
+// channels), at 0.54 per cycle and scheduler with the three warps that the
+// registers allow; about 8 us of a call are its start, the first loads and the
+// join.  8B heads: one sequence of 131071 positions (168 MB) 44 us, 3.8 TB/s;
+// 16 sequences of 17 to 16384 positions (168 MB) 41 us, 4.1 TB/s; one of 300
+// positions 9.6 us; 8 x 4 tokens behind 900 to 5001 positions at 64 channels
+// 19 us (20 with 8 warps per CTA instead of 12).
 template <int D, int NT>
 struct AttendCfg {
     static constexpr int kWarps = NT == 1 || D == 64 ? 12 : 8;      // per CTA and SM: what the registers allow

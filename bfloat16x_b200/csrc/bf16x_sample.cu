@@ -23,6 +23,13 @@
 // all tokens down to that bin are few, one CTA sorts them and finishes alone
 // (the usual top-k, and top-p over a peaked row).  Otherwise the weight above
 // the bin is summed exactly and only the bin's own tokens are sorted.
+//
+// Bound by latency for few rows (a dozen exchanges over the cluster of 1 to 2 us
+// each), by instructions for many (some 40 for a weight, of which each token
+// needs one without filters and, for top-p, one before the cut is known and one
+// if it is kept).  A row of 128256 bf16 logits: greedy 5.0 us, without filters
+// 11.5, top-k 50 14, top-p 0.9 31; 16 rows (fp32): 10.5, 23, 29, 56; 129 rows of
+// 73448: 14, 42, 39, 90 (38 MB: reading alone takes 6).
 #include <algorithm>
 #include <atomic>
 
