@@ -161,6 +161,8 @@ def test_attend_many_tokens(D, T, H, KV, pos):
     (40, 75, 8, 2, 120, (-75, 44)),         # two row tiles, the last with few rows; sequences that see nothing
     (20, 64, 32, 8, 400, (-64, 336)),       # a long cache, units cut between CTAs
     (3, 130, 4, 2, 1500, (-130, 1370)),     # few units, very different lengths
+    (3, 50, 4, 2, 3000, (-3, 2950)),        # units of one group of rows
+    (1, 130, 1, 1, 4500, (4370, 4370)),
     (2, 520, 2, 1, 2000, (1, 1480))])
 @pytest.mark.parametrize("D", [64, 128])
 def test_attend_schedules(D, B, T, H, KV, S, pos):
