@@ -157,15 +157,19 @@ struct alignas(16) SampleShared {
     uint64_t all[W * 32];                         // the cluster's (first CTA)
     uint64_t red_w[2][W];
     uint32_t red_c[2][W];
-    uint64_t cta_w[2];
-    uint32_t cta_c[2];
+    uint64_t peer_w[2][kSampleMaxCluster];        // each CTA's sums, written by it
+    uint32_t peer_c[2][kSampleMaxCluster];
     uint32_t n_list;
     uint64_t scan[W];
     uint32_t scan_c[W];
-    // results of the first CTA, read by all
+    // results of the first CTA
     uint64_t out_w;
     uint32_t out_key, out_idx;
     int out_move;
+    // the same, in every CTA
+    uint64_t got_w;
+    uint32_t got_key, got_idx;
+    int got_move;
     int pick_bin;
     int last_bin;
     uint32_t pick_before, pick_count;
@@ -214,8 +218,9 @@ __device__ __forceinline__ uint64_t warp_scan(uint64_t w) {         // inclusive
 }
 
 // Sums of w and c over the cluster; before_*: those of the CTAs and warps in
-// front of this warp.  Two slots in turn: a slot is written again only after
-// another cluster barrier, when everyone has read it.
+// front of this warp.  A CTA writes its sums to all others before the barrier,
+// so that they are read at home.  Two slots in turn: a slot is written again
+// only after another cluster barrier, when everyone has read it.
 template <int W>
 __device__ __forceinline__ void cluster_sums(SampleCtx<W> &x, uint64_t w, uint32_t c, uint64_t &tot_w, uint32_t &tot_c,
                                              uint64_t &before_w) {
@@ -233,21 +238,16 @@ __device__ __forceinline__ void cluster_sums(SampleCtx<W> &x, uint64_t w, uint32
     if (warp == 0) {
         const uint64_t a = warp_sum(lane < W ? sm.red_w[s][lane] : 0);
         const uint32_t b = __reduce_add_sync(0xffffffffu, lane < W ? sm.red_c[s][lane] : 0u);
-        if (lane == 0) {
-            sm.cta_w[s] = a;
-            sm.cta_c[s] = b;
+        if (lane < x.C) {
+            SampleShared<W> *o = cl.map_shared_rank(&sm, lane);
+            o->peer_w[s][x.rank] = a;
+            o->peer_c[s][x.rank] = b;
         }
     }
     cl.sync();
-    // lane r reads rank r: one remote access deep, not C
-    uint64_t a = 0, f = lane < warp ? sm.red_w[s][lane] : 0;
-    uint32_t n = 0;
-    if (lane < x.C) {
-        const SampleShared<W> *o = cl.map_shared_rank(&sm, lane);
-        a = o->cta_w[s];
-        n = o->cta_c[s];
-        if (lane < x.rank) f += a;
-    }
+    const uint64_t a = lane < x.C ? sm.peer_w[s][lane] : 0;
+    const uint32_t n = lane < x.C ? sm.peer_c[s][lane] : 0u;
+    const uint64_t f = (lane < warp ? sm.red_w[s][lane] : 0) + (lane < x.rank ? a : 0);
     tot_w = warp_sum(a);
     tot_c = __reduce_add_sync(0xffffffffu, n);
     before_w = warp_sum(f);
@@ -583,11 +583,16 @@ __device__ void resolve(SampleCtx<W> &x, int b, uint32_t count, uint32_t k, doub
                 sm.out_w = upto;
             }
         }
+        if (x.rank == 0) {
+            __syncthreads();
+            if (tid < x.C) {
+                SampleShared<W> *o = cl.map_shared_rank(&sm, tid);
+                o->got_move = sm.out_move, o->got_key = sm.out_key, o->got_idx = sm.out_idx, o->got_w = sm.out_w;
+            }
+        }
         cl.sync();
-        const SampleShared<W> *o = cl.map_shared_rank(&sm, 0);
-        const int move = o->out_move;
-        cut = logit_of(o->out_key), cut_idx = o->out_idx, sum = o->out_w;
-        cl.sync();
+        const int move = sm.got_move;
+        cut = logit_of(sm.got_key), cut_idx = sm.got_idx, sum = sm.got_w;
         if (move == 0) return;
         const int to = next_bin(x, b, move);
         if (to == b) {                                              // no such bin: the cut is at the end of the row
@@ -608,6 +613,7 @@ __global__ void __launch_bounds__(W * 32, W == 16 ? 2 : 1) sample_kernel(const S
     const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     griddep_launch_dependents();
+    asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");       // this CTA runs: others may write to it
     if (tid < 64) sm.step[tid] = c_step[tid], sm.start[tid] = c_bin[tid];
     for (int i = tid; i < kSampleBins; i += (W * 32)) sm.cnt[i] = sm.low[i] = 0;
     if (tid == 0) sm.n_list = 0;
@@ -659,15 +665,16 @@ __global__ void __launch_bounds__(W * 32, W == 16 ? 2 : 1) sample_kernel(const S
     const float top_p = p.top_p ? p.top_p[row] : p.top_p0, min_p = p.min_p ? p.min_p[row] : p.min_p0;
     const int32_t top_k = p.top_k ? p.top_k[row] : p.top_k0;
     const float u = p.u[row];
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
     uint32_t high = __reduce_max_sync(0xffffffffu, key_of(top));
     if (lane == 0) sm.red_c[0][warp] = high;
     __syncthreads();
     if (warp == 0) {
         high = __reduce_max_sync(0xffffffffu, lane < W ? sm.red_c[0][lane] : 0u);
-        if (lane == 0) sm.cta_c[0] = high;
+        if (lane < C) cl.map_shared_rank(&sm, lane)->peer_c[0][rank] = high;
     }
     cl.sync();
-    top = logit_of(__reduce_max_sync(0xffffffffu, lane < C ? cl.map_shared_rank(&sm, lane)->cta_c[0] : 0u));
+    top = logit_of(__reduce_max_sync(0xffffffffu, lane < C ? sm.peer_c[0][lane] : 0u));
     SampleCtx<W> x = {sm, logits + tid * p.per, p.per, C, rank, (uint32_t)(base + tid * p.per), 1, {}};
     Weigher &weigh = x.weigh;
     const double inv = 1.4426950408889634074 / (double)temp;
@@ -690,14 +697,13 @@ __global__ void __launch_bounds__(W * 32, W == 16 ? 2 : 1) sample_kernel(const S
         __syncthreads();
         if (warp == 0) {
             at = __reduce_min_sync(0xffffffffu, lane < W ? sm.red_c[1][lane] : 0xFFFFFFFFu);
-            if (lane == 0) sm.cta_c[1] = at;
+            if (lane == 0) cl.map_shared_rank(&sm, 0)->peer_c[1][rank] = at;
         }
         cl.sync();
         if (rank == 0 && warp == 0) {
-            at = __reduce_min_sync(0xffffffffu, lane < C ? cl.map_shared_rank(&sm, lane)->cta_c[1] : 0xFFFFFFFFu);
+            at = __reduce_min_sync(0xffffffffu, lane < C ? sm.peer_c[1][lane] : 0xFFFFFFFFu);
             if (lane == 0) p.tokens[row] = none ? -1 : (int64_t)at;
         }
-        cl.sync();
         return;
     }
     const uint64_t min_w =
@@ -710,7 +716,7 @@ __global__ void __launch_bounds__(W * 32, W == 16 ? 2 : 1) sample_kernel(const S
     const bool by_k = top_k > 0 && top_k < p.V, by_p = top_p < 1.f;
     if (by_k || by_p) {
         // ---- the histogram, and the row's whole weight where top-p needs it
-        uint64_t w = 0, total, skip;
+        uint64_t w = 0, total = 0, skip;
         for_logits(x, [&](float l, int) {
             float d, y, kf;
             int k;
@@ -727,7 +733,8 @@ __global__ void __launch_bounds__(W * 32, W == 16 ? 2 : 1) sample_kernel(const S
             }
         });
         uint32_t c;
-        cluster_sums(x, w, 0, total, c, skip);
+        if (by_k) cl.sync();
+        else cluster_sums(x, w, 0, total, c, skip);
         find_bin(x, by_k ? (uint32_t)top_k : 0u, fmax((double)top_p * (double)total, 1.0));
         int b = sm.pick_bin;
         uint32_t before = sm.pick_before, count = sm.pick_count;
@@ -798,11 +805,10 @@ __global__ void __launch_bounds__(W * 32, W == 16 ? 2 : 1) sample_kernel(const S
                         if (goal < run && goal >= run - one) p.tokens[row] = (int64_t)(token >> 32);     // exactly one
                     }
                 }
-                if (tid == 0) sm.out_move = finish ? 1 : 0;
+                if (tid < C) cl.map_shared_rank(&sm, tid)->got_move = finish;
             }
             cl.sync();
-            finish = cl.map_shared_rank(&sm, 0)->out_move == 1;
-            cl.sync();
+            finish = sm.got_move;
             if (finish) return;
         }
         uint64_t sum = total;
@@ -859,7 +865,6 @@ __global__ void __launch_bounds__(W * 32, W == 16 ? 2 : 1) sample_kernel(const S
             run = __shfl_sync(0xffffffffu, run, 31);
         }
     }
-    cl.sync();                                        // no CTA leaves while another reads its shared memory
 }
 
 template <int W>
