@@ -24,12 +24,13 @@
 // (the usual top-k, and top-p over a peaked row).  Otherwise the weight above
 // the bin is summed exactly and only the bin's own tokens are sorted.
 //
-// Bound by latency for few rows (a dozen exchanges over the cluster of 1 to 2 us
-// each), by instructions for many (some 40 for a weight, of which each token
-// needs one without filters and, for top-p, one before the cut is known and one
-// if it is kept).  A row of 128256 bf16 logits: greedy 5.0 us, without filters
-// 11.5, top-k 50 14, top-p 0.9 31; 16 rows (fp32): 10.5, 23, 29, 56; 129 rows of
-// 73448: 14, 42, 39, 90 (38 MB: reading alone takes 6).
+// Bound by latency for few rows (up to a dozen exchanges over the cluster of 0.5
+// to 2 us each), by instructions for many (some 40 for a weight, of which each
+// token needs one without filters and, for top-p, one before the cut is known
+// and one if it is kept).  A row of 128256 bf16 logits: greedy 4.7 us, without
+// filters 10.6, top-k 50 with or without top-p 13, top-p 0.9 alone 31; 16 rows
+// (fp32): 9.4, 21, 26, 54; 129 rows of 73448: 12, 40, 37, 86 (38 MB: reading
+// alone takes 6).
 #include <algorithm>
 #include <atomic>
 
@@ -715,18 +716,18 @@ __global__ void __launch_bounds__(W * 32, W == 16 ? 2 : 1) sample_kernel(const S
     uint32_t cut_idx = 0xFFFFFFFFu;
     const bool by_k = top_k > 0 && top_k < p.V, by_p = top_p < 1.f;
     if (by_k || by_p) {
-        // ---- the histogram, and the row's whole weight where top-p needs it
+        // ---- the histogram (behind top-k only of counts: mostly few tokens are left), and the row's whole weight
         uint64_t w = 0, total = 0, skip;
         for_logits(x, [&](float l, int) {
             float d, y, kf;
             int k;
             const bool ok = weigh.place(l, d, y, kf, k);
-            if (!by_p) {
+            if (by_k) {
                 if (ok) atomicAdd(&sm.cnt[k], 1u);
                 return;
             }
             const uint32_t m = weigh.mantissa(l, d, y, kf, k);
-            if (!by_k) w = weigh.add(w, ok ? m : 0u, k);
+            w = weigh.add(w, ok ? m : 0u, k);
             if (ok) {
                 atomicAdd(&sm.cnt[k], 1u);
                 atomicAdd(&sm.low[k], (uint32_t)max((int)(sm.start[k & 63] - m), 0) >> 10);
@@ -822,6 +823,14 @@ __global__ void __launch_bounds__(W * 32, W == 16 ? 2 : 1) sample_kernel(const S
         if (by_p) {
             const double target = fmax((double)top_p * (double)sum, 1.0);
             if (by_k) {
+                for_logits(x, [&](float l, int) {                   // the histogram's weights
+                    float d, y, kf;
+                    int k;
+                    const bool ok = weigh.place(l, d, y, kf, k);
+                    const uint32_t m = weigh.mantissa(l, d, y, kf, k);
+                    if (ok) atomicAdd(&sm.low[k], (uint32_t)max((int)(sm.start[k & 63] - m), 0) >> 10);
+                });
+                cl.sync();
                 find_bin(x, 0u, target);
                 b = sm.pick_bin;
                 __syncthreads();
