@@ -420,9 +420,13 @@ def peer_heap_bytes(model: LlamaModel) -> int:
 
 class NextToken:
     """The choice of the next token from logits: the largest, or drawn with
-    ``sampling`` from random numbers of ``generator`` (a device generator)."""
+    ``sampling`` from random numbers of ``generator`` (a device generator).
+    The ranks of a tensor-parallel model have the same logits and must draw the
+    same numbers: each needs a generator of the same seed."""
 
-    def __init__(self, batch: int, device, sampling: SamplingParams | None = None, generator=None):
+    def __init__(self, batch: int, device, sampling: SamplingParams | None = None, generator=None, tp: int = 1):
+        if tp > 1 and sampling is not None and generator is None:
+            raise ValueError("tensor-parallel ranks need a generator of the same seed each")
         self.sampling, self.generator = sampling, generator
         self.u = torch.zeros(batch, dtype=torch.float32, device=device)
 
@@ -455,7 +459,7 @@ class GraphDecoder:
         self.tok = tok.reshape(-1, 1).clone()
         self.pos = torch.as_tensor(pos, dtype=torch.long).to(dev, copy=True)
         self.next = torch.zeros_like(self.tok)
-        self.chooser = NextToken(self.tok.shape[0], dev, sampling, generator)
+        self.chooser = NextToken(self.tok.shape[0], dev, sampling, generator, model.tp)
         s = torch.cuda.Stream(dev)
         s.wait_stream(torch.cuda.current_stream(dev))
         with torch.cuda.stream(s):
@@ -541,7 +545,7 @@ def generate(model: LlamaModel, prompt: torch.Tensor, new_tokens: int, use_graph
         if pos.shape != (prompt.shape[0],) or int(pos.min()) < 1 or int(pos.max()) > P:
             raise ValueError(f"lengths must be {prompt.shape[0]} numbers in 1..{P}")
         pos0 = pos - P
-    chooser = NextToken(prompt.shape[0], dev, sampling, generator)
+    chooser = NextToken(prompt.shape[0], dev, sampling, generator, model.tp)
     a, b = torch.cuda.Event(True), torch.cuda.Event(True)
     a.record()
     logits = model(prompt, pos0)

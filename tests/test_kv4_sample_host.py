@@ -7,7 +7,8 @@ import torch
 
 from bfloat16x_b200 import _lib
 from bfloat16x_b200.kv4 import Kv4Cache, kv4_blocks
-from bfloat16x_b200.sampling import sample
+from bfloat16x_b200.llama_e2e import NextToken
+from bfloat16x_b200.sampling import SamplingParams, sample
 
 
 def test_block_sizes():
@@ -46,6 +47,15 @@ def test_cpu_tensors_are_refused():
         c.read(p, 1)
     with pytest.raises(_lib.Bf16xError, match="CUDA"):
         sample(torch.zeros(1, 5), torch.zeros(1))
+
+
+def test_tensor_parallel_ranks_must_draw_alike():
+    with pytest.raises(ValueError, match="same seed"):
+        NextToken(2, "cpu", SamplingParams(), None, tp=2)
+    a, b = (NextToken(2, "cpu", SamplingParams(), torch.Generator().manual_seed(5), tp=2) for _ in range(2))
+    a.draw()
+    b.draw()
+    assert torch.equal(a.u, b.u) and NextToken(2, "cpu", None, None, tp=2).sampling is None
 
 
 def _err():
