@@ -876,19 +876,69 @@ __global__ void __launch_bounds__(W * 32, W == 16 ? 2 : 1) sample_kernel(const S
     }
 }
 
+// CTAs per row, and warps per CTA: 32, one CTA per SM, or 16, two per SM, which
+// fill each other's waits.  The pair with the least (waves of clusters) * (40 +
+// tokens per thread): a thread's start, exchanges and searches cost about as much
+// as 40 tokens (16 without filters, 70 for top-p).  A wave of 32 warps takes 0.9
+// of one of 2 x 16; a last wave of 16 that leaves every CTA its SM 0.6, as the
+// SMs come free one by one, and a first one that is nearly empty 0.75.  How many
+// clusters run at once is the device's to say: clusters of 8 with one CTA per SM
+// leave SMs out, and 16 of them took two waves.  Measured, 32 warps against 16
+// with twice the CTAs: 129 rows of 73448, top-p: 77 us and 88 (two full waves
+// each); 40 rows of 128256: 79 and 68 (the second wave nearly empty).
+struct SampleShape {
+    int ctas, warps;
+};
+template <int W>
+static int sample_slots(int dev, int lg) {              // clusters of 2^lg CTAs that run at once
+    static std::atomic<int> known[64][4];
+    if (dev < 64)
+        if (const int n = known[dev][lg].load(std::memory_order_relaxed)) return n;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(1u << lg);
+    cfg.blockDim = dim3(W * 32);
+    cfg.dynamicSmemBytes = W == 32 ? 200 * 1024 : 112 * 1024;
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 1u << lg;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, sample_kernel<W>, &cfg) != cudaSuccess || n < 1) {
+        cudaGetLastError();
+        n = std::max(1, (W == 32 ? 148 : 296) >> lg);
+    }
+    if (dev < 64) known[dev][lg].store(n, std::memory_order_relaxed);
+    return n;
+}
+static SampleShape sample_shape(int dev, int64_t B, int64_t V) {
+    SampleShape best = {kSampleMaxCluster, 32};
+    int64_t least = INT64_MAX;
+    for (int warps = 32; warps >= 16; warps /= 2)
+        for (int lg = 0; 1 << lg <= kSampleMaxCluster; ++lg) {
+            const int64_t threads = (int64_t)warps * 32 << lg, per = ((V + threads - 1) / threads) | 1;
+            const int64_t smem = per * warps * 128 + (int64_t)(warps == 32 ? sizeof(SampleShared<32>) : sizeof(SampleShared<16>));
+            if (V > (int64_t)kSampleMaxKeys << lg || smem > (warps == 32 ? 227 : 112) * 1024) continue;
+            const int64_t slots = warps == 32 ? sample_slots<32>(dev, lg) : sample_slots<16>(dev, lg);
+            const int64_t full = B / slots, rest = B % slots;
+            const int64_t waves = warps == 32 ? (full + (rest > 0)) * 90
+                                              : full * 100 + (rest == 0               ? 0
+                                                              : full && 2 * rest <= slots ? 60
+                                                              : 4 * rest <= slots     ? 75
+                                                                                      : 100);
+            if (waves * (40 + per) < least) {
+                least = waves * (40 + per);
+                best = {1 << lg, warps};
+            }
+        }
+    return best;
+}
+
 template <int W>
 static int sample_launch(SampleParams p, int64_t B, int C, cudaStream_t st) {
     p.per = (int)((p.V + (int64_t)C * W * 32 - 1) / ((int64_t)C * W * 32)) | 1;
     const size_t smem = sizeof(SampleShared<W>) + (size_t)p.per * W * 32 * 4;
-    static std::atomic<uint64_t> raised{0};
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
-    if (e == cudaSuccess && !(raised.load(std::memory_order_relaxed) & bit)) {
-        e = cudaFuncSetAttribute(sample_kernel<W>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
-        if (e == cudaSuccess) raised.fetch_or(bit, std::memory_order_relaxed);
-    }
-    if (e != cudaSuccess) return set_error(BF16X_ERR_CUDA, "bf16x_sample: shared memory: %s", cudaGetErrorString(e));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(B * C));
     cfg.blockDim = dim3(W * 32);
@@ -903,7 +953,7 @@ static int sample_launch(SampleParams p, int64_t B, int C, cudaStream_t st) {
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    e = cudaLaunchKernelEx(&cfg, sample_kernel<W>, p);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, sample_kernel<W>, p);
     if (e != cudaSuccess) return set_error(BF16X_ERR_CUDA, "bf16x_sample: launch: %s", cudaGetErrorString(e));
     return check_launch("sample_kernel");
 }
@@ -924,9 +974,17 @@ extern "C" int bf16x_sample(const void *logits, int dtype, int64_t ld, int64_t B
     if (B > (1 << 24)) return set_error(BF16X_ERR_UNSUPPORTED, "bf16x_sample: too many rows");
     if (B == 0) return BF16X_OK;
     if (!logits || !u || !tokens) return set_error(BF16X_ERR_INVALID, "bf16x_sample: null pointer");
-    // CTAs per row: as the row's size asks, and more while the GPU has room
-    int C = 1;
-    while (C < kSampleMaxCluster && (B * C < 2 * 148 || V > (int64_t)C * kSampleMaxKeys)) C *= 2;
+    static std::atomic<uint64_t> raised{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (e == cudaSuccess && !(raised.load(std::memory_order_relaxed) & bit)) {
+        e = cudaFuncSetAttribute(sample_kernel<32>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(sample_kernel<16>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+        if (e == cudaSuccess) raised.fetch_or(bit, std::memory_order_relaxed);
+    }
+    if (e != cudaSuccess) return set_error(BF16X_ERR_CUDA, "bf16x_sample: shared memory: %s", cudaGetErrorString(e));
+    const SampleShape shape = sample_shape(dev, B, V);
     SampleParams p = {};
     p.logits = logits, p.ld = ld, p.V = V, p.bf16 = dtype == BF16X_DTYPE_BF16;
     int lg = 0;
@@ -935,6 +993,6 @@ extern "C" int bf16x_sample(const void *logits, int dtype, int64_t ld, int64_t B
     p.u = u, p.temperature = temperature, p.top_p = top_p, p.min_p = min_p, p.top_k = top_k;
     p.temperature0 = temperature0, p.top_p0 = top_p0, p.min_p0 = min_p0, p.top_k0 = top_k0;
     p.tokens = tokens;
-    // one CTA per SM: 32 warps; else two of 16, which fill each other's waits
-    return B * C <= 148 ? sample_launch<32>(p, B, C, (cudaStream_t)stream) : sample_launch<16>(p, B, C, (cudaStream_t)stream);
+    return shape.warps == 32 ? sample_launch<32>(p, B, shape.ctas, (cudaStream_t)stream)
+                             : sample_launch<16>(p, B, shape.ctas, (cudaStream_t)stream);
 }
