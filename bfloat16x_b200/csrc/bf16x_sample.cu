@@ -885,7 +885,10 @@ __global__ void __launch_bounds__(W * 32, W == 16 ? 2 : 1) sample_kernel(const S
 // clusters run at once is the device's to say: clusters of 8 with one CTA per SM
 // leave SMs out, and 16 of them took two waves.  Measured, 32 warps against 16
 // with twice the CTAs: 129 rows of 73448, top-p: 77 us and 88 (two full waves
-// each); 40 rows of 128256: 79 and 68 (the second wave nearly empty).
+// each); 40 rows of 128256: 79 and 68 (the second wave nearly empty).  With
+// settings per row, rows take different times and the next begin as one ends:
+// no wave is rounded up (16 such rows of 128256: 37 us with 8 CTAs, of which 14
+// clusters run at once, and 53 with 4; 16 rows of one setting, top-p: 50 and 39).
 struct SampleShape {
     int ctas, warps;
 };
@@ -912,7 +915,7 @@ static int sample_slots(int dev, int lg) {              // clusters of 2^lg CTAs
     if (dev < 64) known[dev][lg].store(n, std::memory_order_relaxed);
     return n;
 }
-static SampleShape sample_shape(int dev, int64_t B, int64_t V) {
+static SampleShape sample_shape(int dev, int64_t B, int64_t V, bool mixed) {
     SampleShape best = {kSampleMaxCluster, 32};
     int64_t least = INT64_MAX;
     for (int warps = 32; warps >= 16; warps /= 2)
@@ -922,7 +925,8 @@ static SampleShape sample_shape(int dev, int64_t B, int64_t V) {
             if (V > (int64_t)kSampleMaxKeys << lg || smem > (warps == 32 ? 227 : 112) * 1024) continue;
             const int64_t slots = warps == 32 ? sample_slots<32>(dev, lg) : sample_slots<16>(dev, lg);
             const int64_t full = B / slots, rest = B % slots;
-            const int64_t waves = warps == 32 ? (full + (rest > 0)) * 90
+            const int64_t waves = mixed         ? std::max<int64_t>(100, 100 * B / slots) * (warps == 32 ? 90 : 100) / 100
+                                  : warps == 32 ? (full + (rest > 0)) * 90
                                               : full * 100 + (rest == 0               ? 0
                                                               : full && 2 * rest <= slots ? 60
                                                               : 4 * rest <= slots     ? 75
@@ -984,7 +988,7 @@ extern "C" int bf16x_sample(const void *logits, int dtype, int64_t ld, int64_t B
         if (e == cudaSuccess) raised.fetch_or(bit, std::memory_order_relaxed);
     }
     if (e != cudaSuccess) return set_error(BF16X_ERR_CUDA, "bf16x_sample: shared memory: %s", cudaGetErrorString(e));
-    const SampleShape shape = sample_shape(dev, B, V);
+    const SampleShape shape = sample_shape(dev, B, V, temperature || top_k || top_p || min_p);
     SampleParams p = {};
     p.logits = logits, p.ld = ld, p.V = V, p.bf16 = dtype == BF16X_DTYPE_BF16;
     int lg = 0;
