@@ -29,7 +29,7 @@
 // token needs one without filters and, for top-p, one before the cut is known
 // and one if it is kept).  A row of 128256 bf16 logits: greedy 4.7 us, without
 // filters 10.6, top-k 50 with or without top-p 13, top-p 0.9 alone 31; 16 rows
-// (fp32): 9.4, 21, 26, 54; 129 rows of 73448: 12, 40, 37, 86 (38 MB: reading
+// (fp32): 5.6, 16, 17, 39; 129 rows of 73448: 12, 36, 35, 76 (38 MB: reading
 // alone takes 6).
 #include <algorithm>
 #include <atomic>
