@@ -39,8 +39,8 @@
 // next scores, 1000 each, half of that the time until an MMA's end is seen.
 // (At 64 channels P has columns of its own, so the next scores need not wait
 // for the product: 4700.)  A call's start and end take 12 us.  8B heads: a
-// prompt of 2048 tokens 60 us, 570 TFLOP/s of the useful half; 512 tokens behind
-// 7680 108 us, 617 TFLOP/s.  3 x 511 tokens of 8 heads of 64 channels behind up
+// prompt of 2048 tokens 61 us, 560 TFLOP/s of the useful half; 512 tokens behind
+// 7680 109 us, 610 TFLOP/s.  3 x 511 tokens of 8 heads of 64 channels behind up
 // to 7003 positions 45 us, 237 TFLOP/s.
 #include <algorithm>
 
@@ -1035,7 +1035,7 @@ static int64_t prefill_units(int64_t B, int64_t KV, int64_t R) { return B * KV *
 // or up to four per CTA over a long cache.  A prompt from its first token on (a
 // cache of at most twice its tokens) with more units than CTAs goes well in whole
 // units, of which the longest go with the shortest: planning and a second kernel
-// made 2048 tokens of the 8B heads 4 us slower (60 -> 64); 3 x 511 tokens of 8
+// made 2048 tokens of the 8B heads 3 us slower (61 -> 64); 3 x 511 tokens of 8
 // heads of 64 channels behind 333 to 7003 positions, 48 units, went from 63 us
 // with equal cuts of each unit to 47.  (The costs' sum has to fit 31 bits.)
 static bool prefill_may_cut(int64_t B, int64_t KV, int64_t R, int64_t T, int64_t max_seq) {
