@@ -339,7 +339,8 @@ int bf16x_silu_mul(const uint16_t *gu, int64_t rows, int64_t F, uint16_t *out, v
  * bf16x_kv4_attend: out[b][t][h] = softmax(scale * q . K) V over positions 0 ..
  *   pos0[b] + t of kv head h / (H / KV), out [B][T][H][D] bf16; a row that sees
  *   no position (padding, or past the cache) is zeros.  q strides in elements,
- *   multiples of 8; everything 16-byte aligned.  workspace:
+ *   multiples of 8; everything 16-byte aligned; out must not overlap q.
+ *   workspace:
  *   bf16x_kv4_attend_workspace_bytes(...) bytes that no other call in flight
  *   uses; its contents never need initialising. */
 int64_t bf16x_kv4_block_bytes(int64_t head_dim);
@@ -361,8 +362,8 @@ int bf16x_kv4_attend(const uint16_t *q, int64_t ldq_b, int64_t ldq_t, int64_t ld
  * top_p (< 1) the shortest prefix that reaches top_p of what top_k kept, min_p
  * (> 0) the tokens that weigh at least min_p times the heaviest; the token is
  * the first kept one, in index order, whose running weight exceeds u times
- * the kept weight.  temperature <= 0: the largest logit (the lowest index of
- * equal ones).  NaN logits count as -infinity; a row without any logit above
+ * the kept weight.  temperature <= 0, or too small for a reciprocal in fp32: the
+ * largest logit (the lowest index of equal ones).  NaN logits count as -infinity; a row without any logit above
  * -infinity gives -1.  Each setting is a device array of B values or, where
  * that is NULL, one value for all.  V <= 327680.  Results do not depend on the
  * order of any sum. */
