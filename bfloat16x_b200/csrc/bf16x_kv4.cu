@@ -799,7 +799,9 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kWarps * 32, 1)
         const int64_t lim = min(pos0 + min(row0 + C - 1, p.R - 1) / p.G + 1, p.max_seq);
         const int part = (int)(con.end - con.blk) * kKvBlock;
         const int n_keys = (int)max(min(lim - origin, (int64_t)part), (int64_t)0);
-        const int all_see = (int)max(min(pos0 + row0 / p.G + 1 - origin, (int64_t)n_keys), (int64_t)0);
+        // (a tile with a row past the cache goes masked throughout: that row sees nothing, its last one lies furthest)
+        const bool past = pos0 + min(row0 + C - 1, p.R - 1) / p.G >= p.max_seq;
+        const int all_see = past ? 0 : (int)max(min(pos0 + row0 / p.G + 1 - origin, (int64_t)n_keys), (int64_t)0);
         Kv4Acc<D, NT> acc;
         kv4_acc_init(acc);
         if (any) {
