@@ -499,7 +499,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const __gri
             const int row = un.row0 + grp * 128 + rl;
             const bool have = row < p.R;
             const int tok = have ? row / p.G : 0, hh = have ? row - tok * p.G : 0;
-            if (grp == 0 && un.t0 == 0 && un.kvh == 0 && have && hh == 0 && un.pos0 + tok >= p.max_seq)
+            if (un.t0 == 0 && un.kvh == 0 && have && hh == 0 && un.pos0 + tok >= p.max_seq)
                 atomicOr(&g_status, kErrBadIndex);
             if (grp >= un.groups) {
                 tiles += un.nt;

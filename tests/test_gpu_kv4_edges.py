@@ -46,3 +46,22 @@ def test_rows_past_a_full_cache_are_zeros(D, S, T, H, KV, pos):
     past = [(b, t) for b, p in enumerate(pos) for t in range(T) if p + t >= S]
     assert past and not any(bool(got[b, t].any()) for b, t in past)
     assert _lib.device_status() & 16
+
+
+# the end of the cache within rows 0..127 and 128..255 of a unit of the prompt kernel; 1500 and 400 positions may be
+# cut between CTAs, 200 tokens of 150 sequences go in whole units
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B,S,T,H,KV,pos", [(2, 1500, 60, 4, 1, [1460, 1400]), (1, 400, 200, 1, 1, [250]),
+                                            (1, 400, 200, 1, 1, [399]), (1, 400, 70, 4, 1, [331]),
+                                            (150, 210, 200, 1, 1, [0] * 149 + [60])])
+def test_attend_alone_reports_rows_past_the_cache(D, B, S, T, H, KV, pos):
+    cache = _full(B, KV, D, S, seed=S + T)
+    assert _lib.device_status() == 0
+    q = torch.randn(B, T, H, D, generator=_gen(T + D)).to(torch.bfloat16)
+    got = cache.attend(q.cuda(), torch.tensor(pos, device="cuda"))
+    assert _lib.device_status() == 16
+    for b, p in enumerate(pos):
+        assert not got[b, max(S - p, 0):].any() and bool(got[b, :S - p].any())
+    inside = [p - max(0, p + T - S) for p in pos]                   # the same, all inside: nothing to report
+    cache.attend(q.cuda(), torch.tensor(inside, device="cuda"))
+    assert _lib.device_status() == 0
