@@ -422,13 +422,18 @@ class NextToken:
     """The choice of the next token from logits: the largest, or drawn with
     ``sampling`` from random numbers of ``generator`` (a device generator).
     The ranks of a tensor-parallel model have the same logits and must draw the
-    same numbers: each needs a generator of the same seed."""
+    same numbers: each needs a generator of the same seed.
+
+    A row with no logit above -infinity (all NaN, say) has no token to draw.
+    Token 0 goes on in its place, so that what is fed back is always an index
+    of the embedding, and ``check`` raises."""
 
     def __init__(self, batch: int, device, sampling: SamplingParams | None = None, generator=None, tp: int = 1):
         if tp > 1 and sampling is not None and generator is None:
             raise ValueError("tensor-parallel ranks need a generator of the same seed each")
         self.sampling, self.generator = sampling, generator
         self.u = torch.zeros(batch, dtype=torch.float32, device=device)
+        self.lowest = torch.zeros(batch, dtype=torch.long, device=device)      # -1: some step had nothing to draw
 
     def draw(self) -> None:
         """New random numbers for the next choice (kept out of captured steps)."""
@@ -440,7 +445,19 @@ class NextToken:
         if self.sampling is None:
             return logits.argmax(-1, keepdim=True)
         s = self.sampling
-        return sample(logits, self.u, s.temperature, s.top_k, s.top_p, s.min_p).unsqueeze(1)
+        drawn = sample(logits, self.u, s.temperature, s.top_k, s.top_p, s.min_p)
+        torch.minimum(self.lowest, drawn, out=self.lowest)
+        return drawn.clamp_(min=0).unsqueeze(1)
+
+    def check(self) -> None:
+        """Raises if a choice since the last check had nothing to draw from (waits for the device)."""
+        if self.sampling is None:
+            return
+        bad = self.lowest.tolist()
+        self.lowest.zero_()
+        if min(bad, default=0) < 0:
+            raise _lib.Bf16xError("no logit above -infinity to draw from in sequences "
+                                  f"{[i for i, t in enumerate(bad) if t < 0]}")
 
 
 class GraphDecoder:
@@ -480,6 +497,10 @@ class GraphDecoder:
         self.graph.replay()
         self.tok.copy_(self.next)
         self.pos += 1
+
+    def check(self) -> None:
+        """Raises if a step since the last check had no token to draw (NextToken.check)."""
+        self.chooser.check()
 
 
 @torch.no_grad()
@@ -533,7 +554,7 @@ def generate(model: LlamaModel, prompt: torch.Tensor, new_tokens: int, use_graph
     steps, greedy or drawn with ``sampling`` (random numbers of ``generator``).
     ``lengths`` (4-bit cache): the prompts' own lengths, each padded on the
     left to P tokens.  Returns (tokens [new_tokens, batch], prefill ms, decode
-    ms/token)."""
+    ms/token).  Raises if a drawn token had nothing to draw from (NextToken)."""
     dev = prompt.device
     P = prompt.shape[1]
     pos0 = torch.zeros((), dtype=torch.long, device=dev)
@@ -562,6 +583,7 @@ def generate(model: LlamaModel, prompt: torch.Tensor, new_tokens: int, use_graph
             out.append(dec.tok.clone())
             dec.step()
         b.record()
+        dec.check()
     else:
         a.record()
         for _ in range(new_tokens):
@@ -571,6 +593,7 @@ def generate(model: LlamaModel, prompt: torch.Tensor, new_tokens: int, use_graph
             pos = pos + 1
         b.record()
     torch.cuda.synchronize(dev)
+    chooser.check()
     return torch.cat(out, dim=1).t().contiguous(), prefill_ms, a.elapsed_time(b) / max(new_tokens, 1)
 
 

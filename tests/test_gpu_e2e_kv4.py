@@ -7,7 +7,7 @@ import torch.nn.functional as F
 
 from bfloat16x_b200 import _lib, llama_e2e
 from bfloat16x_b200.kv4 import Kv4Cache
-from bfloat16x_b200.llama_e2e import CONFIGS, LlamaModel, SamplingParams, generate, pack_model
+from bfloat16x_b200.llama_e2e import CONFIGS, LlamaModel, NextToken, SamplingParams, generate, pack_model
 from tests.gpu_util import rel_l2
 
 pytestmark = pytest.mark.gpu
@@ -106,3 +106,28 @@ def test_sampling_with_the_bf16_cache_and_refusals():
         model(prompt, torch.zeros(1, dtype=torch.long, device="cuda"))
     with pytest.raises(ValueError, match="kv_bits"):
         llama_e2e.LlamaModel(cfg, 64, "cuda", kv_bits=8)
+
+
+@pytest.mark.parametrize("kv_bits", [4, 16])
+@pytest.mark.parametrize("use_graph", [True, False])
+def test_logits_of_nan_raise(kv_bits, use_graph):
+    """No token can be drawn: token 0 is fed instead, and the call raises."""
+    cfg = CONFIGS["tiny"]
+    model = LlamaModel(cfg, 64, "cuda", seed=6, batch=2, kv_bits=kv_bits)
+    prompt = _prompt(2, 20, cfg.vocab, 5)
+    chooser = NextToken(2, "cuda", SamplingParams(temperature=0.7))
+    logits = torch.randn(2, cfg.vocab, generator=torch.Generator().manual_seed(3)).cuda()
+    logits[1] = float("nan")
+    tok = chooser.choose(logits)
+    assert tok.shape == (2, 1) and int(tok[1]) == 0
+    with pytest.raises(_lib.Bf16xError, match=r"sequences \[1\]"):
+        chooser.check()
+    with torch.no_grad():
+        model.norm.weight.fill_(float("nan"))
+    with pytest.raises(_lib.Bf16xError, match=r"sequences \[0, 1\]"):
+        generate(model, prompt, 4, use_graph, SamplingParams(temperature=0.7, top_k=5))
+    with torch.no_grad():
+        model.norm.weight.fill_(1.0)
+    a, b = (generate(model, prompt, 4, g, SamplingParams(temperature=0.7, top_k=1))[0] for g in (use_graph, True))
+    assert torch.equal(a, b)
+    _lib.check_device_status()

@@ -5,7 +5,7 @@ import ctypes
 import pytest
 import torch
 
-from bfloat16x_b200 import _lib
+from bfloat16x_b200 import _lib, llama_e2e
 from bfloat16x_b200.kv4 import Kv4Cache, kv4_blocks
 from bfloat16x_b200.llama_e2e import NextToken
 from bfloat16x_b200.sampling import SamplingParams, sample
@@ -56,6 +56,26 @@ def test_tensor_parallel_ranks_must_draw_alike():
     a.draw()
     b.draw()
     assert torch.equal(a.u, b.u) and NextToken(2, "cpu", None, None, tp=2).sampling is None
+
+
+def test_rows_without_a_token_are_fed_an_index_and_reported(monkeypatch):
+    """What sample() gives for rows of NaN never goes on to the embedding."""
+    drawn = iter([[5, 0, 3], [-1, 2, -1], [1, 1, 1], [4, 4, 4]])
+    monkeypatch.setattr(llama_e2e, "sample", lambda *a: torch.tensor(next(drawn)))
+    c = NextToken(3, "cpu", SamplingParams())
+    logits = torch.zeros(3, 8)
+    assert c.choose(logits).tolist() == [[5], [0], [3]]
+    c.check()
+    assert c.choose(logits).tolist() == [[0], [2], [0]]
+    assert c.choose(logits).tolist() == [[1], [1], [1]]
+    with pytest.raises(_lib.Bf16xError, match=r"sequences \[0, 2\]"):
+        c.check()
+    c.check()                                        # reported once
+    c.choose(logits)
+    c.check()
+    greedy = NextToken(3, "cpu")
+    assert greedy.choose(torch.full((3, 8), float("nan"))).lt(8).all()
+    greedy.check()
 
 
 def _err():
