@@ -553,7 +553,8 @@ def generate(model: LlamaModel, prompt: torch.Tensor, new_tokens: int, use_graph
     """Generation: prefill ``prompt`` [batch, P], then ``new_tokens`` decode
     steps, greedy or drawn with ``sampling`` (random numbers of ``generator``).
     ``lengths`` (4-bit cache): the prompts' own lengths, each padded on the
-    left to P tokens.  Returns (tokens [new_tokens, batch], prefill ms, decode
+    left to P tokens.  There, prompt and new tokens must fit the cache (each
+    step writes its own token too).  Returns (tokens [new_tokens, batch], prefill ms, decode
     ms/token).  Raises if a drawn token had nothing to draw from (NextToken)."""
     dev = prompt.device
     P = prompt.shape[1]
@@ -566,6 +567,9 @@ def generate(model: LlamaModel, prompt: torch.Tensor, new_tokens: int, use_graph
         if pos.shape != (prompt.shape[0],) or int(pos.min()) < 1 or int(pos.max()) > P:
             raise ValueError(f"lengths must be {prompt.shape[0]} numbers in 1..{P}")
         pos0 = pos - P
+    longest = int(pos.max()) if model.cache_kv4 is not None else 0
+    if longest and longest + new_tokens > model.max_seq:
+        raise ValueError(f"{longest} prompt tokens and {new_tokens} new ones do not fit the cache's {model.max_seq} positions")
     chooser = NextToken(prompt.shape[0], dev, sampling, generator, model.tp)
     a, b = torch.cuda.Event(True), torch.cuda.Event(True)
     a.record()

@@ -131,3 +131,17 @@ def test_logits_of_nan_raise(kv_bits, use_graph):
     a, b = (generate(model, prompt, 4, g, SamplingParams(temperature=0.7, top_k=1))[0] for g in (use_graph, True))
     assert torch.equal(a, b)
     _lib.check_device_status()
+
+
+def test_generation_up_to_the_last_position():
+    cfg = CONFIGS["tiny"]
+    prompt = _prompt(2, 20, cfg.vocab, 5)
+    long, short = (LlamaModel(cfg, n, "cuda", seed=6, batch=2, kv_bits=4) for n in (64, 25))
+    assert torch.equal(generate(long, prompt, 5)[0], generate(short, prompt, 5)[0])
+    assert torch.equal(generate(long, prompt, 13, lengths=[12, 7])[0], generate(short, prompt, 13, lengths=[12, 7])[0])
+    _lib.check_device_status()
+    with pytest.raises(ValueError, match="do not fit"):
+        generate(short, prompt, 6)
+    with pytest.raises(ValueError, match="do not fit"):
+        generate(short, prompt, 14, lengths=[12, 7])
+    _lib.check_device_status()

@@ -1,6 +1,7 @@
 """Refusals of the 4-bit cache and of sampling that need no GPU: wrong shapes,
 types and devices raise before anything is launched."""
 import ctypes
+import types
 
 import pytest
 import torch
@@ -76,6 +77,14 @@ def test_rows_without_a_token_are_fed_an_index_and_reported(monkeypatch):
     greedy = NextToken(3, "cpu")
     assert greedy.choose(torch.full((3, 8), float("nan"))).lt(8).all()
     greedy.check()
+
+
+def test_generate_refuses_what_does_not_fit_the_4bit_cache():
+    model = types.SimpleNamespace(cache_kv4=[None], max_seq=24, tp=1)       # refused before the model is called
+    prompt = torch.zeros(2, 20, dtype=torch.long)
+    for new, lengths in ((5, None), (400, None), (8, [17, 3]), (5, [1, 20])):
+        with pytest.raises(ValueError, match="do not fit"):
+            llama_e2e.generate(model, prompt, new, lengths=lengths)
 
 
 def _err():
