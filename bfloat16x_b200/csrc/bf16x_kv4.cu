@@ -243,13 +243,19 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
 //   S^T [16 positions][8 rows] = K Q^T,  P = 2^(S' - M),  O^T [D][8 rows] += V^T P^T
 // with the codes as operands: per 32-channel group j
 //   S  += dK_j (codes Q_j) + mK_j sum(Q_j),   O_j += codes (P dV_j),  O_j += mV_j P.
-// Q, each row scaled by a power of two, is exact in fp16; P dV is rounded to
-// fp16.  The minima go through one more mma each (bf16, exact on the m side, the
+// Q, each row scaled by a power of two, is exact in fp16 (but for channels below
+// 2^-26 of the row's largest, which are off by 2^-34 of that at most); P dV is
+// rounded to fp16.  The minima go through one more mma each (bf16, exact on the m side, the
 // other side split into three or two bf16 parts).  (fp8 operands for the K codes
 // would halve their mma's, but sm_100a's mma.sync widens e4m3 to fp16 first.)
 // P dV has to fit fp16 whatever the scale of V, so the running reference M of
-// a row is the maximum of S' + log2(max_j dV_j), not of S' alone; it is
-// raised only when a term exceeds it by more than 2^8.
+// a row is that of the maximum of S' + log2(max_j dV_j), not of S' alone, and is
+// raised only when a term exceeds it by too much (kRescale).  A group of channels
+// whose scale is 2^-8 of its position's largest or less would lose bits of P dV_j,
+// in the end all of them, to fp16's subnormals: blocks that hold such a position
+// take each group's products apart, P dV_j scaled by a power of two of the row
+// and group, and add them in fp32 (kv4_add_apart).  Looking for it costs 1 % of a
+// call whose groups are alike.
 template <int D, int NT>
 struct Kv4Rows {
     static constexpr int NG = D / 32;
@@ -392,9 +398,36 @@ __device__ __forceinline__ void kv4_words(uint32_t at, uint32_t (&w)[NG]) {     
     }
 }
 
-// log2 of a position's largest V scale for the reference: not below -100, so
-// that P <= 2^108 and its sums stay finite.
-__device__ __forceinline__ float kv4_ref_exp(float d) { return fmaxf(lg2(d), -100.f); }
+// log2 of a position's largest V scale for the reference: not below -92, so
+// that P <= 2^107 and its sums stay finite.
+__device__ __forceinline__ float kv4_ref_exp(float d) { return fmaxf(lg2(d), -92.f); }
+constexpr int kApart = 8 << 23;         // ratio of a position's V scales above which its groups are taken apart, as fp32 bits
+
+// One group's products with x = P dV_j (positions g, g + 8; columns 2t, 2t+1),
+// scaled so that each column's largest is in [2^14, 2^15).
+__device__ __forceinline__ void kv4_add_apart(float (&o0)[4], float (&o1)[4], uint32_t w0, uint32_t w1, float (&x)[4]) {
+    float back[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        float top = fmaxf(x[i], x[2 + i]);
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const int ex = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 15);
+        const float up = __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
+        x[i] *= up;
+        x[2 + i] *= up;
+        back[i] = __uint_as_float((uint32_t)(127 - 14 + ex) << 23);
+    }
+    const uint32_t b0 = movmatrix(pack_f16x2(x[0], x[1])), b1 = movmatrix(pack_f16x2(x[2], x[3]));
+    const uint32_t h0 = w0 >> 8, h1 = w1 >> 8;
+    float c[4];
+    mma_f16(c, w0 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x000F000Fu, w1 & 0x00F000F0u, b0, b1, 0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o0[k] = fmaf(c[k], back[k & 1], o0[k]);
+    mma_f16(c, h0 & 0x000F000Fu, h0 & 0x00F000F0u, h1 & 0x000F000Fu, h1 & 0x00F000F0u, b0, b1, 0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o1[k] = fmaf(c[k], back[k & 1], o1[k]);
+}
 
 // Where this lane's parts of a block lie.
 template <int D>
@@ -414,12 +447,69 @@ struct Kv4Lane {
     }
 };
 
+// The weights P = 2^(S' - M) of kv4_block, and what they add to the sums; APART:
+// each group's products by themselves.
+template <int D, int NT, int NB, bool MASK, bool APART>
+__device__ __forceinline__ void kv4_products(uint32_t blk, int key0, int n_keys, const Kv4Lane<D> &ln, const float (&s)[NB][NT][4],
+                                             const float (&v)[NB][2][D / 32], const float (&unit)[NT][2], Kv4Acc<D, NT> &acc) {
+    using L = KvLayout<D>;
+    constexpr int NG = L::NG;
+    constexpr float kInf = __builtin_huge_valf();
+    const int t = ln.t;
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+        const uint32_t at = blk + n * L::kBytes;
+        uint32_t w0[NG], w1[NG];
+        kv4_words<NG>(at + ln.codes + L::kV, w0);
+        kv4_words<NG>(at + ln.codes + L::kV + 32 * NG * 4, w1);
+        // rows g >= NG of this mma are not used: they may hold any finite numbers (the last group's minima)
+        uint32_t vm0 = lds32(at + ln.vmin), vm1 = lds32(at + ln.vmin + 16 * NG);
+        if (MASK) {
+            const int a = key0 + 16 * n + 2 * t, c = a + 8;
+            vm0 = a + 1 < n_keys ? vm0 : a < n_keys ? vm0 & 0xFFFFu : 0u;
+            vm1 = c + 1 < n_keys ? vm1 : c < n_keys ? vm1 & 0xFFFFu : 0u;
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            float pr[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) pr[i] = ex2(fmaf(s[n][nt][i], unit[nt][i & 1], -acc.M[nt][i & 1]));
+            acc.l[nt][0] += pr[0] + pr[2];
+            acc.l[nt][1] += pr[1] + pr[3];
+            const uint32_t a = pack_bf16x2(pr[0], pr[1]), c = pack_bf16x2(pr[2], pr[3]);
+            const uint32_t al = pack_bf16x2(pr[0] - bf_lo(a), pr[1] - bf_hi(a)),
+                           cl = pack_bf16x2(pr[2] - bf_lo(c), pr[3] - bf_hi(c));
+            mma_bf16(acc.mt[nt], vm0, vm0, vm1, vm1, movmatrix(a), movmatrix(c));
+            mma_bf16(acc.mt[nt], vm0, vm0, vm1, vm1, movmatrix(al), movmatrix(cl));
+#pragma unroll
+            for (int j = 0; j < NG; ++j) {
+                float x[4] = {pr[0] * v[n][0][j], pr[1] * v[n][0][j], pr[2] * v[n][1][j], pr[3] * v[n][1][j]};
+                if (MASK) {                                         // 0 * NaN: a masked position stays out of its row
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[i] = s[n][nt][i] == -kInf ? 0.f : x[i];
+                }
+                if constexpr (APART) {
+                    kv4_add_apart(acc.o[nt][2 * j], acc.o[nt][2 * j + 1], w0[j], w1[j], x);
+                } else {
+                    const uint32_t b0 = movmatrix(pack_f16x2(x[0], x[1])), b1 = movmatrix(pack_f16x2(x[2], x[3]));
+                    const uint32_t h0 = w0[j] >> 8, h1 = w1[j] >> 8;
+                    mma_f16(acc.o[nt][2 * j], w0[j] & 0x000F000Fu, w0[j] & 0x00F000F0u, w1[j] & 0x000F000Fu,
+                            w1[j] & 0x00F000F0u, b0, b1);
+                    mma_f16(acc.o[nt][2 * j + 1], h0 & 0x000F000Fu, h0 & 0x00F000F0u, h1 & 0x000F000Fu,
+                            h1 & 0x00F000F0u, b0, b1);
+                }
+            }
+        }
+    }
+}
+
 // NB consecutive blocks at shared address `blk`, the first position of the
 // first at key0 (relative to the tile's first row, like rows.last).  MASK: some
 // row of the tile does not see all of them; positions from n_keys on are not
-// read as numbers.
+// read as numbers.  Without MASK, blocks whose groups need to be taken apart are
+// left undone (false): short code is what most of them need.
 template <int D, int NT, int NB, bool MASK>
-__device__ __forceinline__ void kv4_block(uint32_t blk, int key0, int n_keys, const Kv4Lane<D> &ln,
+__device__ __forceinline__ bool kv4_block(uint32_t blk, int key0, int n_keys, const Kv4Lane<D> &ln,
                                           const Kv4Rows<D, NT> &rows, Kv4Acc<D, NT> &acc) {
     using L = KvLayout<D>;
     constexpr int NG = L::NG;
@@ -466,6 +556,7 @@ __device__ __forceinline__ void kv4_block(uint32_t blk, int key0, int n_keys, co
     }
     // ---- V's scales, and the reference of each row
     float v[NB][2][NG], e[NB][2];
+    int spread = 0;
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
@@ -475,10 +566,16 @@ __device__ __forceinline__ void kv4_block(uint32_t blk, int key0, int n_keys, co
 #pragma unroll
                 for (int j = 0; j < NG; ++j) v[n][i][j] = ok[n][i] ? v[n][i][j] : 0.f;
             }
+            float lo = fminf(v[n][i][0], v[n][i][1]);
             e[n][i] = fmaxf(v[n][i][0], v[n][i][1]);
-            if constexpr (NG == 4) e[n][i] = fmaxf(e[n][i], fmaxf(v[n][i][2], v[n][i][3]));
+            if constexpr (NG == 4) {
+                lo = min3(lo, v[n][i][2], v[n][i][3]);
+                e[n][i] = max3(e[n][i], v[n][i][2], v[n][i][3]);
+            }
+            spread = max(spread, __float_as_int(e[n][i]) - __float_as_int(lo));
             e[n][i] = kv4_ref_exp(e[n][i]);
         }
+    const bool apart = spread > kApart;
     bool raise = false;
     float top[NT][2], unit[NT][2];
 #pragma unroll
@@ -502,7 +599,10 @@ __device__ __forceinline__ void kv4_block(uint32_t blk, int key0, int n_keys, co
             raise |= top[nt][i] > acc.M[nt][i] + kRescale;
         }
     }
-    if (__any_sync(0xffffffffu, raise)) {
+    bool any_apart = false;
+    if (__any_sync(0xffffffffu, raise || apart)) {                  // (one vote for two rare cases)
+        any_apart = __any_sync(0xffffffffu, apart);
+        if (!MASK && any_apart) return false;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             float a[2];
@@ -511,7 +611,7 @@ __device__ __forceinline__ void kv4_block(uint32_t blk, int key0, int n_keys, co
                 float x = top[nt][i];
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-                x = fmaxf(x, acc.M[nt][i]);
+                x = fmaxf(x - kRefTerm, acc.M[nt][i]);
                 a[i] = ex2(acc.M[nt][i] - x);
                 acc.M[nt][i] = x;
                 acc.l[nt][i] *= a[i];
@@ -525,47 +625,14 @@ __device__ __forceinline__ void kv4_block(uint32_t blk, int key0, int n_keys, co
         }
     }
     // ---- P, and O
-#pragma unroll
-    for (int n = 0; n < NB; ++n) {
-        const uint32_t at = blk + n * L::kBytes;
-        uint32_t w0[NG], w1[NG];
-        kv4_words<NG>(at + ln.codes + L::kV, w0);
-        kv4_words<NG>(at + ln.codes + L::kV + 32 * NG * 4, w1);
-        // rows g >= NG of this mma are not used: they may hold any finite numbers (the last group's minima)
-        uint32_t vm0 = lds32(at + ln.vmin), vm1 = lds32(at + ln.vmin + 16 * NG);
-        if (MASK) {
-            const int a = key0 + 16 * n + 2 * t, c = a + 8;
-            vm0 = a + 1 < n_keys ? vm0 : a < n_keys ? vm0 & 0xFFFFu : 0u;
-            vm1 = c + 1 < n_keys ? vm1 : c < n_keys ? vm1 & 0xFFFFu : 0u;
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            float pr[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) pr[i] = ex2(fmaf(s[n][nt][i], unit[nt][i & 1], -acc.M[nt][i & 1]));
-            acc.l[nt][0] += pr[0] + pr[2];
-            acc.l[nt][1] += pr[1] + pr[3];
-            const uint32_t a = pack_bf16x2(pr[0], pr[1]), c = pack_bf16x2(pr[2], pr[3]);
-            const uint32_t al = pack_bf16x2(pr[0] - bf_lo(a), pr[1] - bf_hi(a)),
-                           cl = pack_bf16x2(pr[2] - bf_lo(c), pr[3] - bf_hi(c));
-            mma_bf16(acc.mt[nt], vm0, vm0, vm1, vm1, movmatrix(a), movmatrix(c));
-            mma_bf16(acc.mt[nt], vm0, vm0, vm1, vm1, movmatrix(al), movmatrix(cl));
-#pragma unroll
-            for (int j = 0; j < NG; ++j) {
-                float x[4] = {pr[0] * v[n][0][j], pr[1] * v[n][0][j], pr[2] * v[n][1][j], pr[3] * v[n][1][j]};
-                if (MASK) {                                         // 0 * NaN: a masked position stays out of its row
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) x[i] = s[n][nt][i] == -kInf ? 0.f : x[i];
-                }
-                const uint32_t b0 = movmatrix(pack_f16x2(x[0], x[1])), b1 = movmatrix(pack_f16x2(x[2], x[3]));
-                const uint32_t h0 = w0[j] >> 8, h1 = w1[j] >> 8;
-                mma_f16(acc.o[nt][2 * j], w0[j] & 0x000F000Fu, w0[j] & 0x00F000F0u, w1[j] & 0x000F000Fu,
-                        w1[j] & 0x00F000F0u, b0, b1);
-                mma_f16(acc.o[nt][2 * j + 1], h0 & 0x000F000Fu, h0 & 0x00F000F0u, h1 & 0x000F000Fu, h1 & 0x00F000F0u,
-                        b0, b1);
-            }
+    if constexpr (MASK) {
+        if (any_apart) {
+            kv4_products<D, NT, NB, MASK, true>(blk, key0, n_keys, ln, s, v, unit, acc);
+            return true;
         }
     }
+    kv4_products<D, NT, NB, MASK, false>(blk, key0, n_keys, ln, s, v, unit, acc);
+    return true;
 }
 
 // The schedule.  A unit is one row tile of one (sequence, kv head); its work is
@@ -812,9 +879,7 @@ __global__ void __launch_bounds__(AttendCfg<D, NT>::kWarps * 32, 1)
                 if (alive) alive = mbar_wait(&sm.full[warp][slot], parity, &g_status);
                 if (alive) {
                     const uint32_t blk = ring0 + slot * NB * L::kBytes;
-                    if (key0 + NB * kKvBlock <= all_see) {
-                        kv4_block<D, NT, NB, false>(blk, key0, n_keys, ln, rows, acc);
-                    } else {
+                    if (key0 + NB * kKvBlock > all_see || !kv4_block<D, NT, NB, false>(blk, key0, n_keys, ln, rows, acc)) {
                         for (int n = 0; n < NB; ++n)
                             if (key0 + n * kKvBlock < n_keys)
                                 kv4_block<D, NT, 1, true>(blk + n * L::kBytes, key0 + n * kKvBlock, n_keys, ln, rows, acc);

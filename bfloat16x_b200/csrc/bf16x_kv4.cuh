@@ -63,6 +63,17 @@ __device__ __forceinline__ float lg2(float x) {
     return r;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+    float d;
+    asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 // bf16 in the low / high half of a word, as fp32
 __device__ __forceinline__ float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
@@ -136,7 +147,11 @@ struct Kv4AttendParams {
     int2 *held;                         // [unit]: the first and last share that hold blocks of it
 };
 
-constexpr float kRescale = 8.f;         // log2 of how far a term may exceed the reference
+// A row's reference M is kept so that its largest term P dV is 2^kRefTerm when M
+// is set and at most 2^kRescale before it is raised: fp16 is used from the top, so
+// that a term of 2^-25 of the largest still has its 11 bits, and a long tail of
+// smaller ones (2^17 positions) is off by 2^-19 of the largest at most.
+constexpr float kRefTerm = 11.f, kRescale = 15.f;
 constexpr float kNoMax = -3.0e38f;
 
 // Launch as a programmatic dependent of the previous kernel of the stream.  The

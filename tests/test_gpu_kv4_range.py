@@ -1,0 +1,97 @@
+"""Attention over the 4-bit cache where sizes differ within a position: groups
+of channels of keys and of values that differ by powers of ten, and long tails
+of small weights behind one strong score, against the 64-bit formulas and the
+same per-channel bound as everywhere."""
+import pytest
+import torch
+
+from bfloat16x_b200 import _lib
+from bfloat16x_b200.kv4 import Kv4Cache
+from tests import kv4_ref
+
+pytestmark = pytest.mark.gpu
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _cache(k, v):
+    """k, v [B, S, KV, D] -> a cache that holds them."""
+    B, S, KV, D = k.shape
+    cache = Kv4Cache.empty(B, S, KV, D, "cuda")
+    kv = torch.cat((k, v), 2).to(torch.bfloat16).reshape(B, S, -1).cuda()
+    cache.append(kv, torch.zeros(1, dtype=torch.long, device="cuda"), 0)
+    return cache
+
+
+def _check(cache, q, pos0, scale=None):
+    got = cache.attend(q.cuda(), torch.tensor(pos0, device="cuda"), scale)
+    scale = q.shape[3] ** -0.5 if scale is None else scale
+    ref, bound = kv4_ref.attend(q, cache.blocks, pos0, scale, cache.max_seq)
+    over = (got.cpu().double() - ref).abs() / bound.clamp(min=1e-300)
+    worst = float(over.max())
+    assert worst <= 1, f"{worst} of the bound"
+    assert torch.equal(got, cache.attend(q.cuda(), torch.tensor(pos0, device="cuda"), scale))
+    _lib.check_device_status()
+
+
+def _groups(S, D, how, seed):
+    """Powers of ten for the groups of a position [S, 1, D]: the same in all positions, or drawn for each."""
+    n = D // 32
+    if how == "fixed":
+        e = torch.tensor([0, -3, -5, -2][:n]).expand(S, n)
+    else:
+        e = torch.tensor([0, -3, -5, -20])[torch.randint(0, 3 if how == "drawn" else 4, (S, n), generator=_gen(seed))]
+    return (10.0 ** e.double()).repeat_interleave(32, 1)[:, None]
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T", [1, 6])
+@pytest.mark.parametrize("how", ["fixed", "drawn", "far"])
+def test_value_groups_of_uneven_size(D, T, how):
+    S, KV = 150, 2
+    k, v = torch.randn(2, S, KV, D, generator=_gen(1)), torch.randn(2, S, KV, D, generator=_gen(2))
+    v = v.double() * _groups(S, D, how, 3)
+    q = (torch.randn(2, T, 4, D, generator=_gen(4)) * 2).to(torch.bfloat16)
+    _check(_cache(k, v), q, [S - T, S // 2 - T + 1])
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T", [1, 6])
+@pytest.mark.parametrize("values", [False, True])
+def test_key_groups_of_uneven_size(D, T, values):
+    """Each group has its share of the scores: the queries are large where the keys are small."""
+    S, KV = 150, 2
+    k, v = torch.randn(2, S, KV, D, generator=_gen(5)), torch.randn(2, S, KV, D, generator=_gen(6))
+    size = _groups(1, D, "fixed", 0)
+    q = torch.randn(2, T, 4, D, generator=_gen(7)).double()
+    if values:
+        v = v * size
+    _check(_cache(k * size, v), (q / size).to(torch.bfloat16), [S - T, S // 2 - T + 1])
+
+
+@pytest.mark.parametrize("T", [1, 5])
+def test_key_groups_drawn(T):
+    """Positions whose large groups differ: most weight lies where a large query meets a large key."""
+    S, D = 150, 128
+    k, v = torch.randn(1, S, 1, D, generator=_gen(8)), torch.randn(1, S, 1, D, generator=_gen(9))
+    q = torch.randn(1, T, 4, D, generator=_gen(10)).double() * _groups(1, D, "drawn", 11)
+    _check(_cache(k * _groups(S, D, "drawn", 12), v), q.to(torch.bfloat16), [S - T], 0.3)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T,S", [(1, 100000), (3, 40000)])
+@pytest.mark.parametrize("down", [(0, 3, 6, 8), (0, 5, 7, 12), (20, 0, 10, 15)])
+def test_long_tail_behind_a_strong_score(D, T, S, down):
+    """One position 2^20 above all others, which together weigh as much as S / 2^20; groups of 2^-down."""
+    n = D // 32
+    k = torch.zeros(1, S, 1, D)
+    k[0, 0] = 1.0
+    strong = 20 * 0.693147 / D
+    size = (2.0 ** -torch.tensor(down[:n], dtype=torch.float64)).repeat_interleave(32)
+    v = (1 + torch.rand(1, 1, 1, D, generator=_gen(13))).expand(1, S, 1, D).double().clone()
+    v[0, 0] = torch.randn(1, D, generator=_gen(14)) * 1e-3
+    q = torch.full((1, T, 2, D), 1.0)
+    q[:, :, 1] = 0.9
+    _check(_cache(k, v * size), q.to(torch.bfloat16), [S - T], strong)
