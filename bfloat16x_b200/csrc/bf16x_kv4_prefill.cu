@@ -25,9 +25,13 @@
 // turns codes (subnormal fp16, see bf16x_kv4.cuh) into values, rounded once (2^-12).
 // dk enters the scores' factor.  dv enters the exponent, P' = 2^(S c + dv - M),
 // and its inverse the sum l of the P'; M is raised, and O scaled, only when a
-// term exceeds it by more than 2^8.  dk and dv are one number per tile, unless
-// its positions differ by more than 2^6 in size: then each position has its own
-// (fp16 would lose the small ones), which costs the softmax a third more work.
+// term exceeds it by too much (kRescale).  dk and dv are one number per tile, unless
+// its positions differ by more than 2^6 in size, or their groups of channels by
+// more than 2^7: then each position has its own (fp16 would lose the small ones),
+// which costs the softmax three times the work.  A group that is 2^-7 of its own
+// position's largest or less falls into fp16's subnormals with any dv.  A piece of a
+// unit that holds such a position is done once more behind the others, by mma.sync
+// on the codes (bf16x_kv4_rows.cuh), which takes any sizes.
 //
 // A V group that is not finite reads as zeros here, and the rows that see its
 // position get NaN in its 32 channels at the end: 0 * NaN would reach the rows
@@ -48,6 +52,7 @@
 #include <cuda_runtime.h>
 
 #include "bf16x_kv4.cuh"
+#include "bf16x_kv4_rows.cuh"
 #include "bf16x_umma.cuh"
 #include "bf16x_wait.cuh"
 
@@ -58,6 +63,11 @@ constexpr int kPreKeys = 128;                         // positions per tile
 constexpr int kPreThreads = 13 * 32;
 constexpr int kPreCut = 4 * 148;                      // units, up to which they may be cut
 constexpr int kPreUnitCost = 2;                       // of a unit's start and end, in tiles
+constexpr int kPreRedo = 1024;                        // (of more pieces per CTA some are done again without need)
+// log2 of where a row's largest term lies when M is set.  It may grow by 2^8 before M is raised: to raise it costs a wait
+// for the product and a pass over O (from 2^11, with 2^4 to go, 2048 tokens of the 8B heads took 66 us instead of 62).
+constexpr float kPreTerm = kRescale - 8.f;
+constexpr int kPreSpread = 7;                         // log2 of how far groups of channels may differ in size
 
 template <int D>
 struct PreSmem {
@@ -84,11 +94,12 @@ struct PreMisc {
     uint64_t dq[2], m_full[4];                        // the converting warps among themselves; a tile's numbers below
     uint32_t tmem;
     int abort_flag;
-    int red[2][4][4];
-    int uneven[4];                                    // of tile j at j % 4: each position has its own dk and dv
+    int red[2][4][8];
+    int uneven[4];                                    // of tile j at j % 4: 1: each position has its own dk and dv, 2: fp16 is not enough
     float k_fac[4][kPreKeys], v_exp[4][kPreKeys], v_inv[4][kPreKeys];      // 2^dk, dv, 2^-dv; else the first only
     uint32_t any_bad[4];
     uint32_t bad[4][kPreKeys / 4];                    // per position a byte: its V groups that are not finite
+    uint32_t redo[kPreRedo / 32], any_redo;           // pieces that fp16 is not enough for: piece n of the CTA at n % kPreRedo
 };
 static_assert(sizeof(PreMisc) <= 7424, "PreMisc");
 struct PrePlan {
@@ -436,6 +447,74 @@ __device__ __forceinline__ int pre_plan(const PreParams &pp, PrePlan &plan) {
     return cut ? share : 0;
 }
 
+// A piece once more, by mma.sync: its rows eight at a time, one warp each, over
+// rings of blocks where Q, K and V were.  (A function of its own: within the kernel
+// its registers made the tiles' loops spill.)  2048 tokens of the 8B heads take 470
+// us if all of their pieces need it for their keys, 680 for their values, 61
+// without; looking for such positions costs 1 %.
+template <int D>
+struct PreRing {
+    static constexpr int kDepth = 3;
+    uint8_t block[kDepth][KvLayout<D>::kBytes];
+    uint4 frag[1][D / 32][32];
+};
+template <int D>
+__device__ __noinline__ void pre_redo(const Kv4AttendParams &p, const PreUnit &un, PreRing<D> &ring) {
+    using L = KvLayout<D>;
+    constexpr int NG = L::NG, DEPTH = PreRing<D>::kDepth;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int64_t origin = (int64_t)un.t0 * kPreKeys;
+    const uint8_t *src = p.blocks + (((int64_t)un.b * p.KV + un.kvh) * p.nblk + (int64_t)un.t0 * (kPreKeys / kKvBlock)) * L::kBytes;
+    const Kv4Lane<D> ln;
+    for (int row0 = un.row0 + 8 * warp; row0 < min(un.row0 + kPreRows, p.R); row0 += 8 * (kPreThreads / 32)) {
+        Kv4Rows<D, 1> rows;
+        kv4_load_rows<D, 1>(p, un.b, un.kvh, row0, un.pos0, origin, ring.frag, rows);
+        Kv4Acc<D, 1> acc;
+        kv4_acc_init(acc);
+        const int64_t lim = min(un.pos0 + min(row0 + 7, p.R - 1) / p.G + 1, p.max_seq) - origin;
+        const int n_keys = (int)max(min(lim, (int64_t)un.nt * kPreKeys), (int64_t)0), count = (n_keys + kKvBlock - 1) / kKvBlock;
+        const auto ask = [&](int i) {
+            if (i < count)
+                for (int c = lane; c < L::kBytes / 16; c += 32)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+                                 :: "r"(smem_u32(ring.block[i % DEPTH]) + 16 * c), "l"(src + (int64_t)i * L::kBytes + 16 * c) : "memory");
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        for (int i = 0; i < DEPTH; ++i) ask(i);
+        for (int i = 0; i < count; ++i) {
+            asm volatile("cp.async.wait_group %0;" :: "n"(DEPTH - 1) : "memory");
+            __syncwarp();
+            kv4_block<D, 1, 1, true>(smem_u32(ring.block[i % DEPTH]), i * kKvBlock, n_keys, ln, rows, acc);
+            __syncwarp();
+            ask(i + DEPTH);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float l = acc.l[0][i];
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+            float mt[NG];
+#pragma unroll
+            for (int j = 0; j < NG; ++j) mt[j] = __shfl_sync(0xffffffffu, acc.mt[0][i], 4 * j + t);
+            const int r = row0 + 2 * t + i;
+            if (r >= p.R) continue;
+            const bool part = un.slot >= 0;
+            const int64_t in_slot = (int64_t)un.slot * kPreRows + r - un.row0;
+            const int tok = r / p.G, hh = r - tok * p.G;
+            uint16_t *dst = p.out + (((int64_t)un.b * p.T + tok) * p.H + un.kvh * p.G + hh) * D + 4 * g;
+            const float f = part ? 1.f : l != 0.f ? 1.f / l : 0.f;
+#pragma unroll
+            for (int j = 0; j < NG; ++j) {
+                const float4 o = kv4_sums(acc, 0, i, j, mt[j], f);
+                if (part) *reinterpret_cast<float4 *>(p.part_o + in_slot * D + 32 * j + 4 * g) = o;
+                else *reinterpret_cast<uint2 *>(dst + 32 * j) = make_uint2(pack_bf16x2(o.x, o.y), pack_bf16x2(o.z, o.w));
+            }
+            if (part && g == 0) p.part_ml[in_slot] = make_float2(acc.M[0][i], l);
+        }
+        __syncwarp();                   // (the rows' fragments and the ring are used again)
+    }
+}
+
 template <int D>
 __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const __grid_constant__ PreParams pp) {
     using L = KvLayout<D>;
@@ -465,8 +544,10 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const __gri
         for (int i = 0; i < 2; ++i) mbar_init(&ms.dq[i], 4);
         for (int i = 0; i < 4; ++i) mbar_init(&ms.m_full[i], 4);
         ms.abort_flag = 0;
+        ms.any_redo = 0;
         fence_mbar_init();
     }
+    if (tid < kPreRedo / 32) ms.redo[tid] = 0;
     if (warp == 12) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                      :: "r"(smem_u32(&ms.tmem)), "r"(512) : "memory");
@@ -488,8 +569,9 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const __gri
                        t_p = tmem + t_lane + SM::kPCol + grp * SM::kPStep;
         bool ok = true;
         int tiles = 0, mine = 0;                                    // tiles before this unit: of all, and of this group
+        int piece = 0;
         PreWalk walk(pp, plan, share);
-        for (PreUnit un; ok && walk.next(pp, un);) {
+        for (PreUnit un; ok && walk.next(pp, un); ++piece) {
             const int row = un.row0 + grp * 128 + rl;
             const bool have = row < p.R;
             const int tok = have ? row / p.G : 0, hh = have ? row - tok * p.G : 0;
@@ -555,6 +637,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const __gri
             // a row that sees nothing here (padding, no row) goes along as if it saw all, and is zeros at the end
             float M = kNoMax, l = 0.f;
             uint32_t bad = 0;
+            int redo = 0;
             for (int j = 0; j < un.nt; ++j) {
                 const int g = tiles + j, slot = g & 3;
                 // (the scores first: a group that sat out a unit may be phases ahead of m_full)
@@ -567,11 +650,13 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const __gri
                 const int vis = sees ? (int)min(max(sees - (int64_t)j * kPreKeys, (int64_t)0), (int64_t)kPreKeys) : kPreKeys;
                 const float fac = c_row * ms.k_fac[slot][0], dv = ms.v_exp[slot][0];
                 // (a factor of zero would make NaN of the scores that are masked by -inf)
-                const bool uneven = ms.uneven[slot], plain = !uneven && !__any_sync(0xffffffffu, !(fac > 0.f));
+                const int sizes = ms.uneven[slot];
+                redo |= sizes & 2;
+                const bool uneven = sizes & 1, plain = !uneven && !__any_sync(0xffffffffu, !(fac > 0.f));
                 if (plain && __any_sync(0xffffffffu, vis < kPreKeys)) pre_mask(t_s, vis);
                 const float x_top = plain ? fmaf(pre_top(t_s), fac, dv) : pre_top_any(t_s, ms, slot, uneven, c_row, vis);
                 if (__any_sync(0xffffffffu, x_top > M + kRescale)) {
-                    const float to = x_top > M ? x_top : M, a = ex2(M - to);
+                    const float to = fmaxf(x_top - kPreTerm, M), a = ex2(M - to);
                     M = to;
                     l *= a;
                     if (j > 0) {                                    // O is complete up to the last tile: its PV is done
@@ -608,6 +693,10 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const __gri
             mine += un.nt;
             if (ok && un.nt > 0) ok = role_wait(&ms.pv_done[grp], (mine - 1) & 1, abort_flag);
             if (!ok) break;
+            if (redo && tid == 0) {
+                ms.redo[piece / 32 % (kPreRedo / 32)] |= 1u << (piece % 32);
+                ms.any_redo = 1;
+            }
             tc_fence_after();
             // ---- out, by way of Q's place (its products are done): 128 bytes of 4 rows per store
             const bool part = un.slot >= 0;
@@ -754,6 +843,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const __gri
         int ke = kNone, ve = kNone;                                 // 2^e is above the position's largest value
         const auto survey = [&](int j, int live) {                  // the raw scales of tile j; writes the warp's exponents
             float kmax = 0.f, vmax = 0.f;
+            uint32_t kmin = ~0u, vmin = ~0u;                        // of the groups that are not zeros: bits - 1
             bad_k = bad_v = 0;
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
@@ -768,16 +858,23 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const __gri
                     bad_v |= 1u << g;
                     vd[g] = vm[g] = 0.f;
                 }
-                kmax = fmaxf(kmax, fmaxf(fabsf(km[g]), fabsf(fmaf(15.f, kd[g], km[g]))));
-                vmax = fmaxf(vmax, fmaxf(fabsf(vm[g]), fabsf(fmaf(15.f, vd[g], vm[g]))));
+                const float kt = fmaxf(fabsf(km[g]), fabsf(fmaf(15.f, kd[g], km[g]))),
+                            vt = fmaxf(fabsf(vm[g]), fabsf(fmaf(15.f, vd[g], vm[g])));
+                kmax = fmaxf(kmax, kt), vmax = fmaxf(vmax, vt);
+                kmin = min(kmin, __float_as_uint(kt) - 1u), vmin = min(vmin, __float_as_uint(vt) - 1u);
             }
-            ke = kmax > 0.f ? min(max((int)(__float_as_uint(kmax) >> 23) - 126, -100), 110) : kNone;
-            ve = vmax > 0.f ? min(max((int)(__float_as_uint(vmax) >> 23) - 126, -100), 110) : kNone;
+            // (V not below 2^-96: 2^-dv times the weights' sum stays finite)
+            const auto exponent = [](uint32_t bits, int least) { return min(max((int)(bits >> 23) - 126, least), 110); };
+            ke = kmax > 0.f ? exponent(__float_as_uint(kmax), -100) : kNone;
+            ve = vmax > 0.f ? exponent(__float_as_uint(vmax), -96) : kNone;
+            const int kg = kmax > 0.f ? exponent(kmin + 1u, -100) : kNone, vg = vmax > 0.f ? exponent(vmin + 1u, -96) : kNone;
             const int a = __reduce_max_sync(0xffffffffu, ke == kNone ? -100 : ke), c = __reduce_min_sync(0xffffffffu, ke),
                       d = __reduce_max_sync(0xffffffffu, ve == kNone ? -100 : ve), f = __reduce_min_sync(0xffffffffu, ve);
+            const int k = __reduce_min_sync(0xffffffffu, kg), v = __reduce_min_sync(0xffffffffu, vg);
+            const bool far = __any_sync(0xffffffffu, ke - kg > kPreSpread || ve - vg > kPreSpread);
             if (lane == 0) {
                 int *red = ms.red[j & 1][dw];
-                red[0] = a, red[1] = c, red[2] = d, red[3] = f;
+                red[0] = a, red[1] = c, red[2] = d, red[3] = f, red[4] = k, red[5] = v, red[6] = far;
             }
             ms.bad[j & 3][lane] = 0;                                // every warp the same
             if (lane == 0) ms.any_bad[j & 3] = 0;
@@ -786,13 +883,14 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const __gri
         uint32_t kd24[NH], kmh[NH];                                 // K's scales * 2^24 and minima of this position, fp16 pairs
         const auto scale = [&](int j) {                             // after all warps' exponents of tile j
             const int slot = j & 3;
-            int k_hi = -100, k_lo = kNone, v_hi = -100, v_lo = kNone;
+            int k_hi = -100, k_lo = kNone, v_hi = -100, v_lo = kNone, k_grp = kNone, v_grp = kNone, far = 0;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int *red = ms.red[j & 1][i];
                 k_hi = max(k_hi, red[0]), k_lo = min(k_lo, red[1]), v_hi = max(v_hi, red[2]), v_lo = min(v_lo, red[3]);
+                k_grp = min(k_grp, red[4]), v_grp = min(v_grp, red[5]), far |= red[6];
             }
-            const bool uneven = k_hi - k_lo > 6 || v_hi - v_lo > 6;
+            const bool uneven = !far && (k_hi - k_lo > 6 || v_hi - v_lo > 6 || k_hi - k_grp > kPreSpread || v_hi - v_grp > kPreSpread);
             // 2^-dk times the largest value is at most 2^-6
             const int dk = (uneven && ke != kNone ? ke : k_hi) + 6, dv = (uneven && ve != kNone ? ve : v_hi) + 6;
             const float k0 = __uint_as_float((uint32_t)(127 - dk) << 23), k24 = k0 * 0x1p24f,
@@ -813,7 +911,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const __gri
                 atomicOr(&ms.bad[slot][key >> 2], bad_v << (8 * (key & 3)));
                 ms.any_bad[slot] = 1;
             }
-            if (key == 0) ms.uneven[slot] = uneven;
+            if (key == 0) ms.uneven[slot] = (int)uneven | far << 1;
             if (uneven || key == 0) {
                 ms.k_fac[slot][key] = __uint_as_float((uint32_t)(127 + dk) << 23);
                 ms.v_exp[slot][key] = (float)dv;
@@ -971,6 +1069,13 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv4_prefill_kernel(const __gri
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512) : "memory");
     }
+    // ---- pieces that fp16 is not enough for
+    static_assert(sizeof(PreRing<D>) % 16 == 0 && sizeof(PreRing<D>) * (kPreThreads / 32) <= SM::kScale, "PreRing");
+    if (!ms.any_redo || ms.abort_flag) return;
+    PreWalk walk(pp, plan, share);
+    int piece = 0;
+    for (PreUnit un; walk.next(pp, un); ++piece)
+        if (ms.redo[piece / 32 % (kPreRedo / 32)] >> (piece % 32) & 1u) pre_redo<D>(p, un, reinterpret_cast<PreRing<D> *>(smem)[warp]);
 }
 
 // The sums of the units that were cut, joined: one warp per row.

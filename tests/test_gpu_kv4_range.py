@@ -47,7 +47,7 @@ def _groups(S, D, how, seed):
 
 
 @pytest.mark.parametrize("D", [64, 128])
-@pytest.mark.parametrize("T", [1, 6])
+@pytest.mark.parametrize("T", [1, 6, 60])
 @pytest.mark.parametrize("how", ["fixed", "drawn", "far"])
 def test_value_groups_of_uneven_size(D, T, how):
     S, KV = 150, 2
@@ -58,7 +58,7 @@ def test_value_groups_of_uneven_size(D, T, how):
 
 
 @pytest.mark.parametrize("D", [64, 128])
-@pytest.mark.parametrize("T", [1, 6])
+@pytest.mark.parametrize("T", [1, 6, 60])
 @pytest.mark.parametrize("values", [False, True])
 def test_key_groups_of_uneven_size(D, T, values):
     """Each group has its share of the scores: the queries are large where the keys are small."""
@@ -71,7 +71,7 @@ def test_key_groups_of_uneven_size(D, T, values):
     _check(_cache(k * size, v), (q / size).to(torch.bfloat16), [S - T, S // 2 - T + 1])
 
 
-@pytest.mark.parametrize("T", [1, 5])
+@pytest.mark.parametrize("T", [1, 60])
 def test_key_groups_drawn(T):
     """Positions whose large groups differ: most weight lies where a large query meets a large key."""
     S, D = 150, 128
@@ -81,7 +81,7 @@ def test_key_groups_drawn(T):
 
 
 @pytest.mark.parametrize("D", [64, 128])
-@pytest.mark.parametrize("T,S", [(1, 100000), (3, 40000)])
+@pytest.mark.parametrize("T,S", [(1, 100000), (3, 40000), (60, 12000)])
 @pytest.mark.parametrize("down", [(0, 3, 6, 8), (0, 5, 7, 12), (20, 0, 10, 15)])
 def test_long_tail_behind_a_strong_score(D, T, S, down):
     """One position 2^20 above all others, which together weigh as much as S / 2^20; groups of 2^-down."""
@@ -95,3 +95,40 @@ def test_long_tail_behind_a_strong_score(D, T, S, down):
     q = torch.full((1, T, 2, D), 1.0)
     q[:, :, 1] = 0.9
     _check(_cache(k, v * size), q.to(torch.bfloat16), [S - T], strong)
+
+
+# (B, T, H, KV, S, first positions): units that go whole and cut, some sequences with groups far apart and some without,
+# in the first tiles only or in the last ones
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B,T,H,KV,S,pos", [(20, 64, 32, 8, 64, (0, 0)), (40, 75, 8, 2, 120, (-75, 44)), (3, 130, 4, 2, 1500, (-130, 1370)),
+                                            (1, 300, 4, 1, 2500, (2200, 2200)), (2, 520, 2, 1, 2000, (1, 1480))])
+def test_prompts_of_which_parts_have_groups_far_apart(D, B, T, H, KV, S, pos):
+    k, v = torch.randn(B, S, KV, D, generator=_gen(21)), torch.randn(B, S, KV, D, generator=_gen(22))
+    far = torch.rand(B, 1, KV, 1, generator=_gen(23)) < 0.5
+    at = torch.arange(S)[None, :, None, None]
+    v[..., 32:64] *= torch.where(far & (at < 100), 2.0 ** -12, 1.0)
+    k[..., :32] *= torch.where(far & (at >= max(S - 140, 100)), 2.0 ** -11, 1.0)
+    q = torch.randn(B, T, H, D, generator=_gen(24)).to(torch.bfloat16)
+    _check(_cache(k, v), q, torch.linspace(pos[0], pos[1], B).round().long().tolist())
+
+
+@pytest.mark.parametrize("T", [60, 130])
+def test_captured_prompt_follows_the_sizes_in_the_cache(T):
+    """One captured call over a cache whose groups are alike, then far apart, then alike."""
+    D, H, KV, S = 128, 4, 2, 600
+    k, v = torch.randn(1, S, KV, D, generator=_gen(25)), torch.randn(1, S, KV, D, generator=_gen(26))
+    w = v.clone()
+    w[..., 64:96] *= 1e-4
+    cache, other = _cache(k, v), _cache(k, w)
+    plain = cache.blocks.clone()
+    q = torch.randn(1, T, H, D, generator=_gen(27)).to(torch.bfloat16).cuda()
+    pos = torch.tensor(S - T, device="cuda")
+    want = [cache.attend(q, pos), other.attend(q, pos)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = cache.attend(q, pos)
+    for i, blocks in enumerate((plain, other.blocks, plain, other.blocks)):
+        cache.blocks.copy_(blocks)
+        graph.replay()
+        assert torch.equal(out, want[i % 2])
+    _lib.check_device_status()
