@@ -17,8 +17,8 @@
 // same in any order.  With ~1e5 kept tokens, fp32 weights would move about
 // one draw in a hundred to a neighbour.
 //
-// One cluster of C CTAs per row; each holds its part of the row as ordered
-// 32-bit keys in shared memory and the logits are read once.  A histogram of
+// One cluster of C CTAs per row; each holds its part of the row as fp32 logits
+// in shared memory, so the row is read once.  A histogram of
 // (top - l) in 1/64 octaves of weight then says in which bin a cut lies.  If
 // all tokens down to that bin are few, one CTA sorts them and finishes alone
 // (the usual top-k, and top-p over a peaked row).  Otherwise the weight above
@@ -104,8 +104,8 @@ struct Weigher {
     float limit;                                      // weights of less than about half a step are 0
     int sh;
     const uint32_t *step;
-    // k = y in 1/64 octaves, rounded: fp32 operations each rounded by itself, so it never falls as the logit does
-        // y, and k as a number and an integer; false for weights of 0
+    // y (p), and k = y in 1/64 octaves, rounded, as a number and an integer; false for weights of 0.  Each fp32
+    // operation is rounded by itself, so k never falls as the logit does.
     __device__ __forceinline__ bool place(float l, float &s, float &p, float &kf, int &k) const {
         s = l == top ? 0.f : __fsub_rn(top, l);                     // (infinity less infinity)
         p = __fmul_rn(s, chi);

@@ -25,10 +25,6 @@ __device__ __forceinline__ void umma_commit(uint64_t *bar) {
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-__device__ __forceinline__ void named_bar_sync(int id, int n) {
-    asm volatile("bar.sync %0, %1;" :: "r"(id), "r"(n) : "memory");
-}
-
 // Byte offset of element (row, col) inside a 128-row x 64-column K-major
 // 128-byte-swizzled tile (16-byte chunk index XOR row % 8).
 __device__ __forceinline__ uint32_t sw128_offset(uint32_t row, uint32_t col) {
