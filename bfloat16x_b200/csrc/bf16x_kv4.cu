@@ -25,8 +25,9 @@ namespace bf16x {
 // whole K word of a lane), over the heads in turn, so that the angles of the
 // position are loaded once.  4 x 2047 tokens of the 8B heads (32 + 2 * 8 of 128
 // channels, 190 MB) take 48 us, 4.0 TB/s; one token 3.4 us, all latency.  Bound
-// by instructions (0.78 per cycle and scheduler, memory at a third); rounding by
-// a division per value took 118 us.
+// by instructions (0.78 per cycle and scheduler, memory at a third), one value
+// each: arithmetic on fp32 pairs and minima of bf16 pairs would be fewer and
+// round the same.  Rounding by a division per value took 118 us.
 template <int D>
 __device__ __forceinline__ void kv4_quantize8(const float (&y)[8], float &d, float &m, uint32_t &codes) {
     float lo = y[0], hi = y[0];
@@ -167,6 +168,8 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4AppendParams p
 // thread before its first use: 4 x 2047 tokens of 8 heads of 128 channels (44
 // MB, most of it written) take 10.2 us, 4.3 TB/s (one token per CTA 13.7, eight
 // 9.7; K and V in turn within a warp, and a conversion per code, 14.7 with one).
+// Bound by instructions (0.75 per cycle and scheduler, one value each) and its
+// start.
 struct Kv4ReadParams {
     const uint8_t *blocks;
     int64_t max_seq, nblk;
@@ -251,10 +254,11 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
 // others it writes its part, at most one that began before its share (slot 0)
 // and one that goes on after it (slot 1), and a second kernel joins the parts.
 //
-// Bound by instructions: some 290 per block of 16 positions at 128 channels
-// (unpacking codes, softmax, the weights times the scales, four mma per 32
-// channels), at 0.54 per cycle and scheduler with the three warps that the
-// registers allow; about 8 us of a call are its start, the first loads and the
+// Bound by latency: some 290 instructions per block of 16 positions at 128
+// channels (unpacking codes, softmax, the weights times the scales, four mma per
+// 32 channels) follow one another in one chain per warp, and the three warps per
+// scheduler that the registers allow issue 0.54 per cycle; DRAM is at half.  About
+// 8 us of a call are its start, the first loads and the
 // join.  8B heads: one sequence of 131071 positions (168 MB) 44 us, 3.8 TB/s;
 // 16 sequences of 17 to 16384 positions (168 MB) 41 us, 4.1 TB/s; one of 300
 // positions 9.6 us; 8 x 4 tokens behind 900 to 5001 positions at 64 channels

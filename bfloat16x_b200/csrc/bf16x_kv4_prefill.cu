@@ -28,7 +28,7 @@
 // term exceeds it by too much (kRescale).  dk and dv are one number per tile, unless
 // its positions differ by more than 2^6 in size, or their groups of channels by
 // more than 2^7: then each position has its own (fp16 would lose the small ones),
-// which costs the softmax three times the work.  A group that is 2^-7 of its own
+// which makes the softmax slow (12000 cycles a tile, not 3200).  A group that is 2^-7 of its own
 // position's largest or less falls into fp16's subnormals with any dv.  A piece of a
 // unit that holds such a position is done once more behind the others, by mma.sync
 // on the codes (bf16x_kv4_rows.cuh), which takes any sizes.
@@ -43,9 +43,9 @@
 // next scores, 1000 each, half of that the time until an MMA's end is seen.
 // (At 64 channels P has columns of its own, so the next scores need not wait
 // for the product: 4700.)  A call's start and end take 12 us.  8B heads: a
-// prompt of 2048 tokens 61 us, 560 TFLOP/s of the useful half; 512 tokens behind
+// prompt of 2048 tokens 62 us, 556 TFLOP/s of the useful half; 512 tokens behind
 // 7680 109 us, 610 TFLOP/s.  3 x 511 tokens of 8 heads of 64 channels behind up
-// to 7003 positions 45 us, 237 TFLOP/s.
+// to 7003 positions 46 us, 234 TFLOP/s.
 #include <algorithm>
 
 #include <cuda_fp16.h>

@@ -138,7 +138,8 @@ class Kv4Cache:
         """Causal attention of q [batch, T, heads, head_dim] (bf16, heads a
         multiple of kv_heads) over the cache: the row at position pos0[b] + t
         sees positions 0 .. pos0[b] + t.  scale: default head_dim ** -0.5.
-        Returns bf16 like q (zeros for a row that sees nothing)."""
+        Returns bf16 like q (zeros for a row that sees nothing or whose
+        position lies past the cache).  The cache has no gradient."""
         self._check(q, "q")
         KV, D = self.kv_heads, self.head_dim
         shape = q.shape

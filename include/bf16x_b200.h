@@ -333,12 +333,15 @@ int bf16x_silu_mul(const uint16_t *gu, int64_t rows, int64_t F, uint16_t *out, v
  *   ld_b, ld_t in elements, multiples of 8): q and k heads turned pairwise by
  *   cos/sin (fp32 [>= max_seq][D/2], both NULL: not turned), q to q_out
  *   [B][T][H][D], k and v into the cache; q rows of positions outside the
- *   cache are zeros.  A group of 32 that holds an infinity or NaN reads as NaN.
+ *   cache are zeros.  A group of 32 that holds an infinity or NaN, or whose
+ *   span leaves fp32, reads as NaN.
  * bf16x_kv4_read: k_out, v_out [B][T][KV][D] bf16: the values the cache holds,
  *   zeros outside it.
  * bf16x_kv4_attend: out[b][t][h] = softmax(scale * q . K) V over positions 0 ..
  *   pos0[b] + t of kv head h / (H / KV), out [B][T][H][D] bf16; a row that sees
- *   no position (padding, or past the cache) is zeros.  q strides in elements,
+ *   no position (padding, or past the cache) is zeros.  Groups of channels and
+ *   positions may differ in size: values between 2^-100 and 2^100, within 2^80 of
+ *   one another, keep the accuracy of bf16.  q strides in elements,
  *   multiples of 8; everything 16-byte aligned; out must not overlap q.
  *   workspace:
  *   bf16x_kv4_attend_workspace_bytes(...) bytes that no other call in flight

@@ -41,6 +41,8 @@ def _groups(S, D, how, seed):
     n = D // 32
     if how == "fixed":
         e = torch.tensor([0, -3, -5, -2][:n]).expand(S, n)
+    elif how == "wide":
+        e = torch.tensor([0, -24, 3, -13][:n]).expand(S, n)             # 2^-80 and 2^10 beside 1
     else:
         e = torch.tensor([0, -3, -5, -20])[torch.randint(0, 3 if how == "drawn" else 4, (S, n), generator=_gen(seed))]
     return (10.0 ** e.double()).repeat_interleave(32, 1)[:, None]
@@ -48,7 +50,7 @@ def _groups(S, D, how, seed):
 
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("T", [1, 6, 60])
-@pytest.mark.parametrize("how", ["fixed", "drawn", "far"])
+@pytest.mark.parametrize("how", ["fixed", "drawn", "far", "wide"])
 def test_value_groups_of_uneven_size(D, T, how):
     S, KV = 150, 2
     k, v = torch.randn(2, S, KV, D, generator=_gen(1)), torch.randn(2, S, KV, D, generator=_gen(2))
