@@ -340,8 +340,9 @@ int bf16x_silu_mul(const uint16_t *gu, int64_t rows, int64_t F, uint16_t *out, v
  * bf16x_kv4_attend: out[b][t][h] = softmax(scale * q . K) V over positions 0 ..
  *   pos0[b] + t of kv head h / (H / KV), out [B][T][H][D] bf16; a row that sees
  *   no position (padding, or past the cache) is zeros.  Groups of channels and
- *   positions may differ in size: values between 2^-100 and 2^100, within 2^80 of
- *   one another, keep the accuracy of bf16.  q strides in elements,
+ *   positions may differ in size: the accuracy is bf16's for values between
+ *   2^-100 and 2^100 that lie within 2^80 of one another, and for channels of q
+ *   down to 2^-26 of their row's largest.  q strides in elements,
  *   multiples of 8; everything 16-byte aligned; out must not overlap q.
  *   workspace:
  *   bf16x_kv4_attend_workspace_bytes(...) bytes that no other call in flight

@@ -134,3 +134,37 @@ def test_captured_prompt_follows_the_sizes_in_the_cache(T):
         graph.replay()
         assert torch.equal(out, want[i % 2])
     _lib.check_device_status()
+
+
+def test_many_pieces_of_a_cta_some_of_them_far_apart():
+    """24 units per CTA: every third sequence has groups far apart; a few sequences of each kind against the formulas."""
+    B, KV, T, H, D = 300, 4, 130, 16, 64
+    k, v = torch.randn(B, T, KV, D, generator=_gen(31)), torch.randn(B, T, KV, D, generator=_gen(32))
+    v[1::3, ..., 32:] *= 2.0 ** -12
+    cache = _cache(k, v)
+    q = torch.randn(B, T, H, D, generator=_gen(33)).to(torch.bfloat16)
+    got = cache.attend(q.cuda(), torch.zeros(1, dtype=torch.long, device="cuda")).cpu()
+    for b in (0, 1, 151, B - 2):
+        ref, bound = kv4_ref.attend(q[b:b + 1], cache.blocks[b:b + 1], [0], D ** -0.5, T)
+        worst = float(((got[b:b + 1].double() - ref).abs() / bound).max())
+        assert worst <= 1, f"sequence {b}: {worst} of the bound"
+    _lib.check_device_status()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T", [3, 9, 60])
+@pytest.mark.parametrize("part", [0, 1])
+def test_nan_beside_groups_far_apart(D, T, part):
+    """An infinity in the keys or values of a position reaches only the rows that see it, in whatever form they go."""
+    n = 200
+    kv = torch.randn(1, n, 2, D, generator=_gen(34))
+    kv[:, :, 1, :32] *= 2.0 ** -12
+    kv[0, n - 2, part, D - 1] = float("inf")
+    cache = _cache(kv[:, :, :1], kv[:, :, 1:])
+    q = torch.randn(1, T, 2, D, generator=_gen(35)).to(torch.bfloat16)
+    got = cache.attend(q.cuda(), torch.tensor([n - T], device="cuda")).cpu()
+    ref, bound = kv4_ref.attend(q[:, :T - 2], cache.blocks, [n - T], D ** -0.5, n)
+    assert bool(((got[:, :T - 2].double() - ref).abs() <= bound).all())
+    seen = got[:, T - 2:].isnan()
+    assert bool(seen.all()) if part == 0 else bool(seen[..., D - 32:].all() and not seen[..., :D - 32].any())
+    _lib.check_device_status()
